@@ -19,6 +19,7 @@ DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I8, DTYPE_I32 = 0, 1, 2, 3, 4
 GELU_NONE, GELU_ERF, GELU_TANH = 0, 1, 2
 MODE_REF, MODE_BLOCK64 = 0, 1
 QDIV_IEEE, QDIV_FULL = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4
 ABI_VERSION = 1
 NOALLOC_SCRATCH_BYTES = 32 << 20
 
@@ -71,6 +72,27 @@ _SIGNATURES = {
     "dc_attn_int8_fwd_noalloc": (ctypes.c_int, [_c_p, _c_p, _c_p, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_i64,
                                                 _c_i64, _c_i64p, _c_i64p, _c_i64p, ctypes.c_float, ctypes.c_int,
                                                 _c_p, _c_i64p, _c_p]),
+    "dc_linear": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64,
+                                 ctypes.c_int, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p]),
+    "dc_gated_linear": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p,
+                                       _c_i64, ctypes.c_int, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p]),
+    "dc_act_grad_workspace": (ctypes.c_int, [_c_i64, _c_i64, ctypes.POINTER(ctypes.c_size_t)]),
+    "dc_act_grad": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p,
+                                   ctypes.c_size_t, ctypes.c_int, _c_i64, _c_i64, ctypes.c_int, _c_p]),
+    "dc_linear_dx": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, ctypes.c_int, _c_i64,
+                                    _c_i64, _c_i64, _c_p]),
+    "dc_linear_dw": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, ctypes.c_int, _c_i64, _c_i64,
+                                    _c_i64, _c_p]),
+    "dc_layer_norm": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, ctypes.c_int, _c_p, _c_i64, _c_p, _c_p, ctypes.c_int,
+                                     _c_i64, _c_i64, ctypes.c_float, _c_p]),
+    "dc_layer_norm_grad_workspace": (ctypes.c_int, [_c_i64, _c_i64, ctypes.POINTER(ctypes.c_size_t)]),
+    "dc_layer_norm_grad": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, ctypes.c_int, _c_p, _c_p, _c_p, _c_i64,
+                                          _c_p, _c_p, _c_p, ctypes.c_size_t, ctypes.c_int, _c_i64, _c_i64, _c_p]),
+    "dc_embedding": (ctypes.c_int, [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p,
+                                    _c_i64, ctypes.c_int, _c_p]),
+    "dc_embedding_grad_workspace": (ctypes.c_int, [_c_i64, _c_i64, _c_i64, ctypes.POINTER(ctypes.c_size_t)]),
+    "dc_embedding_grad": (ctypes.c_int, [_c_p, _c_i64, _c_p, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_i64,
+                                         ctypes.c_float, _c_p, _c_p, ctypes.c_size_t, ctypes.c_int, _c_p]),
     "dc_selftest_exp2": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_i64, _c_p]),
     "dc_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_longlong, _c_p, _c_p]),
 }
@@ -123,7 +145,8 @@ def i64_array(values) -> ctypes.Array:
 
 
 def device_error(clear: bool = True) -> int:
-    """The device-global error word set by bounded in-kernel waits (0 = none)."""
+    """The device-global error word (0 = none): 1 and 2 from bounded in-kernel waits, 3 from an
+    embedding lookup that met a token id outside its table."""
     code = ctypes.c_uint(0)
     check(load().dc_device_error(ctypes.byref(code), 1 if clear else 0))
     return int(code.value)

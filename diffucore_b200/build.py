@@ -1,29 +1,34 @@
 """Builds the sm_100a shared library ``libdiffucore_b200.so`` in-tree with nvcc.
 
-The library is one translation unit (``csrc/dc_api.cu`` includes the kernel headers) built
-for ``sm_100a`` only, with the CUDA runtime linked statically so the ``.so`` loads through
-ctypes next to PyTorch's own runtime. ``python -m diffucore_b200.build`` rebuilds it.
+The library has one translation unit per group of entry points (``csrc/dc_api.cu``: the W8A8 and
+INT8 attention path, ``csrc/text_api.cu``: the text operators; each includes its kernel headers),
+compiled side by side for ``sm_100a`` only and linked with the CUDA runtime statically, so the
+``.so`` loads through ctypes next to PyTorch's own runtime. ``python -m diffucore_b200.build``
+rebuilds what changed, ``--force`` everything.
 """
 
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "libdiffucore_b200.so"
+OBJECTS = PKG / "_build"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
-    "--shared", "-Xcompiler", "-fPIC",
-    "-cudart", "static",
+    "-Xcompiler", "-fPIC",
 ]
+LINK_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "--shared", "-cudart", "static"]
 
 
 def _nvcc() -> str:
@@ -48,17 +53,45 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > built for p in _sources())
 
 
-def build_library(force: bool = False, verbose: bool = False) -> Path:
-    """Compile ``csrc/dc_api.cu`` into ``libdiffucore_b200.so`` unless it is up to date."""
-    if not force and not needs_build():
-        return LIB
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), str(CSRC / "dc_api.cu")]
+def _includes(path: Path, seen: set[Path]) -> set[Path]:
+    """``path`` and every file it includes by a quoted name, recursively."""
+    if path not in seen and path.exists():
+        seen.add(path)
+        for name in re.findall(r'^#include "([^"]+)"', path.read_text(), flags=re.M):
+            _includes((path.parent / name).resolve(), seen)
+    return seen
+
+
+def _compile(src: Path, force: bool, verbose: bool) -> Path:
+    obj = OBJECTS / (src.stem + ".o")
+    if not force and obj.exists():
+        built = obj.stat().st_mtime
+        if all(p.stat().st_mtime <= built for p in _includes(src.resolve(), set())):
+            return obj
+    tmp = obj.with_suffix(".o.tmp")
+    _run([_nvcc(), *NVCC_FLAGS, "-c", "-o", str(tmp), str(src)], verbose)
+    os.replace(tmp, obj)
+    return obj
+
+
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    """Compile ``csrc/*.cu`` and link ``libdiffucore_b200.so`` unless it is up to date."""
+    if not force and not needs_build():
+        return LIB
+    OBJECTS.mkdir(exist_ok=True)
+    sources = sorted(CSRC.glob("*.cu"))
+    with ThreadPoolExecutor(len(sources)) as pool:
+        objects = list(pool.map(lambda src: _compile(src, force, verbose), sources))
+    tmp = LIB.with_suffix(".so.tmp")
+    _run([_nvcc(), *LINK_FLAGS, "-o", str(tmp), *map(str, objects)], verbose)
     os.replace(tmp, LIB)
     return LIB
 

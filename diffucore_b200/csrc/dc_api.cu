@@ -17,6 +17,7 @@
 
 // Size of the fixed scratch behind dc_attn_int8_fwd_noalloc (32 MiB per GPU).
 constexpr size_t kNoAllocScratch = static_cast<size_t>(DC_NOALLOC_SCRATCH_BYTES);
+#include "host.cuh"
 #include "sm100.cuh"
 #include "quant.cuh"
 #include "rowquant.cuh"
@@ -26,95 +27,11 @@ constexpr size_t kNoAllocScratch = static_cast<size_t>(DC_NOALLOC_SCRATCH_BYTES)
 
 namespace {
 
-thread_local char g_err[512] = "";
-
 // Division arithmetic of every per-row quantizer launch (DC_QDIV_IEEE / DC_QDIV_FULL), set by
 // dc_set_quant_division; read when a launch is enqueued.
 std::atomic<int> g_quant_div{DC_QDIV_IEEE};
 
 int quant_full_div() { return g_quant_div.load(std::memory_order_relaxed) == DC_QDIV_FULL ? 1 : 0; }
-
-int fail(const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return DC_ERR_INVALID;
-}
-
-int cuda_fail(cudaError_t e, const char* what) {
-  snprintf(g_err, sizeof(g_err), "%s: %s", what, cudaGetErrorString(e));
-  return DC_ERR_CUDA;
-}
-
-#define DC_CHECK_LAUNCH(what)                          \
-  do {                                                 \
-    cudaError_t e_ = cudaGetLastError();               \
-    if (e_ != cudaSuccess) return cuda_fail(e_, what); \
-  } while (0)
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
-// rank-N tiled map; dims/strides innermost first, strides in bytes for dims 1..N-1.
-int make_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
-             const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swz) {
-  EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return fail("cuTensorMapEncodeTiled is not available from the CUDA driver");
-  if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return fail("TMA base address is not 16-byte aligned");
-  cuuint64_t d[5], s[4];
-  cuuint32_t b[5], e[5];
-  for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; e[i] = 1; }
-  for (int i = 0; i + 1 < rank; ++i) {
-    if (strides_bytes[i] % 16 != 0) return fail("TMA stride %llu bytes is not a multiple of 16",
-                                                (unsigned long long)strides_bytes[i]);
-    s[i] = strides_bytes[i];
-  }
-  CUresult r = fn(map, dt, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
-  return DC_OK;
-}
-
-int sm_count() {
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
-}
-
-int check_sm100() {
-  int dev = 0, major = 0, minor = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return fail("no CUDA device");
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-  if (major != 10 || minor != 0) return fail("device is sm_%d%d; this library is built for sm_100a only", major, minor);
-  return DC_OK;
-}
-
-template <typename K>
-int set_smem(K kernel, int bytes) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-  return DC_OK;
-}
-
-inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 // ------------------------------------------------------------------------------ quantizer
 
@@ -879,10 +796,10 @@ int dc_set_quant_division(int mode) {
 
 int dc_quant_division(void) { return g_quant_div.load(std::memory_order_relaxed); }
 
-const char* dc_last_error(void) { return g_err; }
+const char* dc_last_error(void) { return dc::err_text; }
 
 int dc_device_error(unsigned int* code, int clear) {
-  unsigned int v = 0;
+  unsigned int v = 0, text = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, dc::g_device_error, sizeof(v));
   if (e != cudaSuccess) return cuda_fail(e, "reading the device error word");
   if (clear) {
@@ -890,6 +807,8 @@ int dc_device_error(unsigned int* code, int clear) {
     e = cudaMemcpyToSymbol(dc::g_device_error, &zero, sizeof(zero));
     if (e != cudaSuccess) return cuda_fail(e, "clearing the device error word");
   }
+  if (int r = dc::text_device_error(&text, clear)) return r;
+  if (v == 0) v = text;
   if (code) *code = v;
   return DC_OK;
 }

@@ -1,0 +1,640 @@
+// 16-bit GEMMs of the text operators on the sm_100a tensor core (bf16 / fp16 operands, fp32
+// accumulators in TMEM):
+//   forward   y[M, N]  = act(x[M, K] . w[N, K]^T + bias) + residual
+//   gated     h[M, N]  = act(x . wg^T + bg) * (x . wu^T + bu)
+//   d input   dx[M, K] = dz[M, N] . w[N, K]            (gated: dg . wg + du . wu, one accumulator)
+//   d weight  dw[N, K] = dz[M, N]^T . x[M, K]          (gated: both weights in one launch)
+// All four are one contraction D[m, n] = sum_k A(m, k) B(n, k); they differ in whether an operand
+// is stored with k contiguous (K-major: x, w forward) or with its row index contiguous (MN-major:
+// dz and x in the weight gradient, w in the input gradient). The tensor core reads either layout
+// from 128-byte-swizzled tiles, so no operand is transposed in memory.
+//
+// Two kernels share the layouts and the epilogue arithmetic:
+//   hgemm_pair_kernel     persistent, 256 x 256 tiles on a CTA pair (cta_group::2), two
+//                         accumulators in TMEM so one tile's epilogue overlaps the next's MMAs
+//   hgemm_cluster_kernel  128 x 128 tiles, two CTAs per SM, the contraction of a tile divided over
+//                         a cluster of up to 8 CTAs whose fp32 partials meet in shared memory
+// A gated tile's accumulator holds the gate in its first half of the columns and the up
+// projection in the second (the pair's even CTA stages wg rows, the odd CTA wu rows), so both
+// projections, the activation and the product are one pass over x.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+#include "sm100.cuh"
+
+namespace dc {
+
+enum Act : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
+enum HEpi : int { kEpiLinear = 0, kEpiGated = 1 };
+
+constexpr int kHBK = 64;                // contraction elements per swizzle atom (128 bytes)
+constexpr int kHEpiWarps = 8;
+constexpr int kHThreads = 64 + 32 * kHEpiWarps;
+constexpr int kHAtom = 128 * 128;       // bytes of one operand atom: 128 rows (or columns) x 64 k
+
+struct HGemmParams {
+  int M, N;                // output rows and columns (gated: columns of h)
+  int tiles_m, tiles_n, num_tiles, group_m;
+  int kb0, kb1;            // k-blocks read from the operands' first and second maps
+  int m_split;             // tiles with tm >= m_split read A's second map and write out1
+  int splits;              // cluster kernel: CTAs per tile
+  void* out;
+  void* out1;
+  int64_t ldo;
+  const void* bias;        // [N] in the output dtype, or null
+  const void* bias1;       // gated: the up projection's
+  const void* residual;    // [M, N], or null
+  int64_t ldr;
+  float* z0;               // pre-activation values kept for the backward pass (fp32), or null
+  float* z1;
+  int64_t ldz;
+  int act;
+  int bf16;                // operands, bias, residual and output: bf16 (else fp16)
+  int out_vec, res_vec;    // rows of out / residual are 16-byte aligned
+  int a_rows;              // cluster kernel: rows of A one box loads
+};
+
+__device__ __forceinline__ float h_to_f(uint32_t bits, int bf16) {
+  return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b, int bf16) {
+  if (bf16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Activations in fp32. The tanh form of GELU is x * sigmoid(2 u) with u = sqrt(2/pi)(x + 0.044715 x^3)
+// (0.5 (1 + tanh u) = sigmoid(2 u)), which loses nothing for negative x.
+__device__ __forceinline__ float sigmoid_f(float x) { return 1.0f / (1.0f + __expf(-x)); }
+__device__ __forceinline__ float act_value(float z, int act) {
+  switch (act) {
+    case kActRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);
+    case kActSilu: return z * sigmoid_f(z);
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case kActGeluTanh: return z * sigmoid_f(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    default: return z;
+  }
+}
+// Every value of a block through one activation; the switch stays outside the unrolled loops.
+template <int N, typename F>
+__device__ __forceinline__ void each_value(float (&v)[N], F f) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = f(v[j]);
+}
+template <int N>
+__device__ __forceinline__ void act_values(float (&v)[N], int act) {
+  switch (act) {
+    case kActRelu: each_value(v, [](float z) { return act_value(z, kActRelu); }); break;
+    case kActSilu: each_value(v, [](float z) { return act_value(z, kActSilu); }); break;
+    case kActGelu: each_value(v, [](float z) { return act_value(z, kActGelu); }); break;
+    case kActGeluTanh: each_value(v, [](float z) { return act_value(z, kActGeluTanh); }); break;
+    default: break;
+  }
+}
+// (activation, derivative)
+__device__ __forceinline__ float2 act_value_grad(float z, int act) {
+  switch (act) {
+    case kActRelu: return make_float2(z > 0.0f ? z : (z != z ? z : 0.0f), z > 0.0f ? 1.0f : 0.0f);
+    case kActSilu: {
+      const float s = sigmoid_f(z);
+      return make_float2(z * s, s * (1.0f + z * (1.0f - s)));
+    }
+    case kActGelu: {
+      const float c = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+      return make_float2(z * c, c + z * __expf(-0.5f * z * z) * 0.39894228040143268f);
+    }
+    case kActGeluTanh: {
+      const float s = sigmoid_f(1.5957691216057308f * (z + 0.044715f * z * z * z));
+      const float du = 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+      const float q = s * (1.0f - s);            // 0 for a large |z|, where du may have overflowed
+      return make_float2(z * s, q == 0.0f ? s : s + z * q * du);
+    }
+    default: return make_float2(z, 1.0f);
+  }
+}
+
+// ------------------------------------------------------------------ operand tiles
+
+// TMA loads of one 64-deep atom. K-major: one box of 64 k x `rows` rows at (k, row). MN-major:
+// boxes of 64 row indices x 64 k at (row + 64 i, k), 8 KB apart.
+template <bool MN, bool PAIR>
+__device__ __forceinline__ void load_atom(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, uint32_t pair_bar,
+                                          int k, int row, int rows) {
+  if (MN) {
+    for (int i = 0; i < rows / 64; ++i) {
+      if (PAIR) tma_load_2d_pair(dst + i * 8192, map, pair_bar, row + 64 * i, k);
+      else tma_load_2d(dst + i * 8192, map, bar, row + 64 * i, k);
+    }
+  } else {
+    if (PAIR) tma_load_2d_pair(dst, map, pair_bar, k, row);
+    else tma_load_2d(dst, map, bar, k, row);
+  }
+}
+
+// Descriptor of the 16-deep step `ks` of an atom. K-major: 32 bytes along the 128-byte rows,
+// 8-row groups 1024 bytes apart. MN-major: 16 k-rows of 128 bytes further, 8-k groups 1024 bytes
+// apart, the next 64 row indices 8192 bytes away.
+template <bool MN>
+__device__ __forceinline__ uint64_t atom_desc(uint32_t saddr, int ks) {
+  return MN ? smem_desc(saddr + ks * 2048, 8192, 1024) : smem_desc(saddr + ks * 32, 16, 1024);
+}
+
+__host__ __device__ constexpr uint32_t idesc_h(int M, int N, bool a_mn, bool b_mn) {
+  return idesc_f16(M, N, false, b_mn) | ((a_mn ? 1u : 0u) << 15);
+}
+constexpr uint32_t kIdescBF16 = (1u << 7) | (1u << 10);
+
+// Column-grouped tile order: `group_m` tile rows at a time, all tile columns of a group before the
+// next, rows fastest, so the tiles in flight share few A and B panels.
+__device__ __forceinline__ void tile_coords(const HGemmParams& p, int tile, int& tm, int& tn) {
+  const int per_group = p.group_m * p.tiles_n;
+  const int g = tile / per_group, r = tile - g * per_group;
+  const int first = g * p.group_m;
+  const int gm = min(p.group_m, p.tiles_m - first);
+  tm = first + r % gm;
+  tn = r / gm;
+}
+
+// ------------------------------------------------------------------ pair kernel epilogue
+
+// A warp's block of 32 rows x 64 bytes in shared memory, 16-byte units swizzled so that both the
+// row-per-lane and the row-segment accesses spread over all banks.
+__device__ __forceinline__ int block_unit(int row, int u) { return row * 4 + (u ^ ((row >> 1) & 3)); }
+
+// Write the staged block to rows of `dst` (row pitch in bytes): `rows` rows, `bytes` of each row.
+// ES is the element size for ragged edges and unaligned rows.
+template <int ES>
+__device__ __forceinline__ void block_store(const uint4* tile, uint8_t* dst, int64_t pitch, int rows, int bytes,
+                                            bool vec) {
+  const int lane = lane_id();
+  if (vec && bytes == 64) {
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int rr = 8 * it + (lane >> 2), u = lane & 3;
+      if (rr < rows) *reinterpret_cast<uint4*>(dst + rr * pitch + 16 * u) = tile[block_unit(rr, u)];
+    }
+  } else {
+    constexpr int kPer = 64 / ES;               // elements per row of the block
+    constexpr int kRows = 32 / kPer;            // rows per step
+    const int e = lane % kPer, sub = lane / kPer;
+    if (e * ES < bytes) {
+      for (int r = sub; r < rows; r += kRows) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(&tile[block_unit(r, e * ES / 16)]) + e * ES % 16;
+        if (ES == 2) *reinterpret_cast<uint16_t*>(dst + r * pitch + e * ES) = *reinterpret_cast<const uint16_t*>(src);
+        else *reinterpret_cast<uint32_t*>(dst + r * pitch + e * ES) = *reinterpret_cast<const uint32_t*>(src);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void block_load16(uint4* tile, const uint8_t* src, int64_t pitch, int rows, int bytes,
+                                             bool vec) {
+  const int lane = lane_id();
+  if (vec && bytes == 64) {
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int rr = 8 * it + (lane >> 2), u = lane & 3;
+      if (rr < rows) tile[block_unit(rr, u)] = *reinterpret_cast<const uint4*>(src + rr * pitch + 16 * u);
+    }
+  } else if (lane * 2 < bytes) {
+    for (int r = 0; r < rows; ++r) {
+      uint8_t* d = reinterpret_cast<uint8_t*>(&tile[block_unit(r, lane >> 3)]) + (lane & 7) * 2;
+      *reinterpret_cast<uint16_t*>(d) = *reinterpret_cast<const uint16_t*>(src + r * pitch + lane * 2);
+    }
+  }
+}
+
+// 32 x 32 fp32 values (one row per lane) to `z`, 16 columns at a time.
+__device__ __forceinline__ void store_z(uint4* tile, const float (&v)[32], float* z, int64_t ldz, int rows, int cols) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (16 * h < cols) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        tile[block_unit(lane, u)] = make_uint4(__float_as_uint(v[16 * h + 4 * u]), __float_as_uint(v[16 * h + 4 * u + 1]),
+                                               __float_as_uint(v[16 * h + 4 * u + 2]), __float_as_uint(v[16 * h + 4 * u + 3]));
+      __syncwarp();
+      block_store<4>(tile, reinterpret_cast<uint8_t*>(z + 16 * h), ldz * 4, rows, min(64, 4 * (cols - 16 * h)), true);
+      __syncwarp();
+    }
+  }
+}
+
+// ------------------------------------------------------------------ pair kernel
+
+constexpr int kPairBN = 256;
+constexpr int kPairStages = 3;
+constexpr int kPairAtoms = 2;                                      // 64-deep atoms per stage
+constexpr int kPairStage = 2 * kPairAtoms * kHAtom;                // bytes per CTA: A and B atoms
+constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+
+template <bool AMN, bool BMN, int EPI>
+__global__ void __launch_bounds__(kHThreads, 1)
+hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
+                  const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
+                  const HGemmParams p) {
+  constexpr int kHalf = kPairBN / 2;             // accumulator columns per epilogue warp
+  constexpr int kOutCols = EPI == kEpiGated ? kPairBN / 2 : kPairBN;   // output columns per tile
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full_bar[kPairStages];
+  __shared__ __align__(8) uint64_t empty_bar[kPairStages];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ __align__(16) float col_bias[kHEpiWarps][kHalf];
+  __shared__ __align__(16) uint4 epi_tile[kHEpiWarps][128];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = warp_id(), lane = lane_id();
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int unit = static_cast<int>(blockIdx.x >> 1), units = static_cast<int>(gridDim.x >> 1);
+  const int num_kb = p.kb0 + p.kb1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * kHEpiWarps); }
+    mbar_init(&drain_bar, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) { tma_prefetch_desc(&map_a0); tma_prefetch_desc(&map_b0); }
+  if (warp == 1) { tmem_alloc_pair(&tmem_base_slot, 2 * kPairBN); tmem_relinquish_pair(); }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_slot;
+  volatile int* abort = &abort_flag;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = unit; tile < p.num_tiles && ok; tile += units) {
+        int tm, tn;
+        tile_coords(p, tile, tm, tn);
+        const bool second = tm >= p.m_split;
+        const int arow = (second ? tm - p.m_split : tm) * 256 + rank * 128;
+        const int brow = EPI == kEpiGated ? tn * kOutCols : tn * kPairBN + rank * 128;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort)) { ok = false; break; }
+          const bool seg = kb >= p.kb0;
+          const CUtensorMap* ma = seg || second ? &map_a1 : &map_a0;
+          const CUtensorMap* mb = (EPI == kEpiGated ? rank != 0 : seg) ? &map_b1 : &map_b0;
+          uint8_t* sa = smem + stage * kPairStage;
+          uint8_t* sb = sa + kPairAtoms * kHAtom;
+          const uint32_t bar = cluster_addr(&full_bar[stage], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kPairStage);
+#pragma unroll
+          for (int at = 0; at < kPairAtoms; ++at) {
+            const int k = (kb - (seg ? p.kb0 : 0)) * (kPairAtoms * kHBK) + at * kHBK;
+            load_atom<AMN, true>(sa + at * kHAtom, ma, nullptr, bar, k, arow, 128);
+            load_atom<BMN, true>(sb + at * kHAtom, mb, nullptr, bar, k, brow, 128);
+          }
+          if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) {
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // loads already issued land before the CTA exits
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer (even CTA, lane 0)
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_h(256, kPairBN, AMN, BMN) | (p.bf16 ? kIdescBF16 : 0u);
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int tile = unit; tile < p.num_tiles && ok; tile += units, ++local) {
+        const int buf = local & 1;
+        const uint32_t acc_phase = (local >> 1) & 1;
+        if (!mbar_wait_cluster(&acc_empty[buf], acc_phase ^ 1, abort)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * kPairBN;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * kPairStage);
+          const uint32_t sb = sa + kPairAtoms * kHAtom;
+#pragma unroll
+          for (int k = 0; k < kPairAtoms * 4; ++k) {
+            const uint64_t ad = atom_desc<AMN>(sa + (k / 4) * kHAtom, k % 4);
+            const uint64_t bd = atom_desc<BMN>(sb + (k / 4) * kHAtom, k % 4);
+            mma_f16_ss_pair(d_tmem, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
+          }
+          mma_commit_pair_both(&empty_bar[stage]);
+          if (kb == num_kb - 1) mma_commit_pair_both(&acc_full[buf]);
+          if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+        }
+      }
+      mma_commit_pair(&drain_bar);
+      mbar_wait(&drain_bar, 0, nullptr, 1000000);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- epilogue (8 warps)
+    const int ew = warp - 2;
+    const int quarter = warp & 3;               // TMEM lane quarter this warp may access
+    const int half = ew >> 2;                   // which half of the tile's output columns
+    float* my_bias = col_bias[ew];
+    uint4* tile_s = epi_tile[ew];
+    constexpr int kWarpCols = kOutCols / 2;     // output columns per warp
+    int local = 0;
+    for (int tile = unit; tile < p.num_tiles; tile += units, ++local) {
+      int tm, tn;
+      tile_coords(p, tile, tm, tn);
+      const int buf = local & 1;
+      const uint32_t acc_phase = (local >> 1) & 1;
+      const int ncol0 = tn * kOutCols + half * kWarpCols;
+      __syncwarp();
+      for (int i = lane; i < kWarpCols; i += 32) {
+        const int n = ncol0 + i;
+        my_bias[i] = p.bias != nullptr && n < p.N ? h_to_f(reinterpret_cast<const uint16_t*>(p.bias)[n], p.bf16) : 0.0f;
+        if (EPI == kEpiGated)
+          my_bias[kWarpCols + i] =
+              p.bias1 != nullptr && n < p.N ? h_to_f(reinterpret_cast<const uint16_t*>(p.bias1)[n], p.bf16) : 0.0f;
+      }
+      __syncwarp();
+      const bool ok = mbar_wait(&acc_full[buf], acc_phase, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const bool second = tm >= p.m_split;
+      const int64_t row0 = static_cast<int64_t>(second ? tm - p.m_split : tm) * 256 + rank * 128 + quarter * 32;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.M - row0));   // may be <= 0
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kPairBN + half * kWarpCols;
+      uint8_t* out = reinterpret_cast<uint8_t*>(second ? p.out1 : p.out);
+#pragma unroll 1
+      for (int c = 0; c < kWarpCols; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c, r);
+        tmem_wait_ld();
+        const int col0 = ncol0 + c;
+        const int cols = min(32, p.N - col0);
+        if (cols <= 0 || rows <= 0) continue;             // warp-uniform
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + my_bias[c + j];
+        if (p.z0 != nullptr) store_z(tile_s, v, p.z0 + row0 * p.ldz + col0, p.ldz, rows, cols);
+        act_values(v, p.act);
+        if (EPI == kEpiGated) {
+          float u[32];
+          tmem_ld32(taddr + kOutCols + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(r[j]) + my_bias[kWarpCols + c + j];
+          if (p.z1 != nullptr) store_z(tile_s, u, p.z1 + row0 * p.ldz + col0, p.ldz, rows, cols);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= u[j];
+        } else if (p.residual != nullptr) {
+          block_load16(tile_s, reinterpret_cast<const uint8_t*>(p.residual) + (row0 * p.ldr + col0) * 2, p.ldr * 2,
+                       rows, 2 * cols, p.res_vec);
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint4 w = tile_s[block_unit(lane, u)];
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[8 * u + 2 * i] += h_to_f(ws[i] & 0xFFFFu, p.bf16);
+              v[8 * u + 2 * i + 1] += h_to_f(ws[i] >> 16, p.bf16);
+            }
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          tile_s[block_unit(lane, u)] =
+              make_uint4(pack_h2(v[8 * u], v[8 * u + 1], p.bf16), pack_h2(v[8 * u + 2], v[8 * u + 3], p.bf16),
+                         pack_h2(v[8 * u + 4], v[8 * u + 5], p.bf16), pack_h2(v[8 * u + 6], v[8 * u + 7], p.bf16));
+        __syncwarp();
+        block_store<2>(tile_s, out + (row0 * p.ldo + col0) * 2, p.ldo * 2, rows, 2 * cols, p.out_vec);
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * kPairBN);
+  }
+}
+
+// ------------------------------------------------------------------ cluster kernel
+
+constexpr int kClBN = 128;
+constexpr int kClStages = 3;
+constexpr int kClStage = 2 * kHAtom;
+constexpr int kClSmem = kClStages * kClStage + 1024;
+static_assert(kClStages * kClStage >= 128 * kClBN * 4, "the fp32 partial tile reuses the stages");
+
+// Four 16-bit values at `src` (vector access when `vec`), zero past `n` of them.
+__device__ __forceinline__ float4 load4(const uint16_t* src, int n, bool vec, int bf16) {
+  uint32_t a = 0, b = 0;
+  if (vec && n >= 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(src);
+    a = u.x; b = u.y;
+  } else {
+    if (n > 0) a = src[0];
+    if (n > 1) a |= static_cast<uint32_t>(src[1]) << 16;
+    if (n > 2) b = src[2];
+    if (n > 3) b |= static_cast<uint32_t>(src[3]) << 16;
+  }
+  return make_float4(h_to_f(a & 0xFFFFu, bf16), h_to_f(a >> 16, bf16), h_to_f(b & 0xFFFFu, bf16), h_to_f(b >> 16, bf16));
+}
+
+// One CTA of a cluster computes its share of a tile's k-blocks; the fp32 partials are left in
+// shared memory and each CTA of the cluster adds up and finishes its share of the rows, in the
+// order of the CTAs (the same sums on every call).
+template <bool AMN, bool BMN, int EPI>
+__global__ void __launch_bounds__(kHThreads, 2)
+hgemm_cluster_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
+                     const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
+                     const HGemmParams p) {
+  constexpr int kOutCols = EPI == kEpiGated ? kClBN / 2 : kClBN;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full_bar[kClStages];
+  __shared__ __align__(8) uint64_t empty_bar[kClStages];
+  __shared__ __align__(8) uint64_t acc_full;
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = warp_id(), lane = lane_id();
+  const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  int tm, tn;
+  tile_coords(p, static_cast<int>(blockIdx.x) / p.splits, tm, tn);
+  const bool second = tm >= p.m_split;
+  const int row0 = (second ? tm - p.m_split : tm) * 128;
+  const int num_kb = p.kb0 + p.kb1;
+  const int kb_begin = static_cast<int>(static_cast<int64_t>(num_kb) * rank / p.splits);
+  const int kb_end = static_cast<int>(static_cast<int64_t>(num_kb) * (rank + 1) / p.splits);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kClStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    mbar_init(&acc_full, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) { tma_prefetch_desc(&map_a0); tma_prefetch_desc(&map_b0); }
+  if (warp == 1) { tmem_alloc(&tmem_base_slot, kClBN); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_slot;
+  volatile int* abort = &abort_flag;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t a_bytes = AMN ? kHAtom : static_cast<uint32_t>(p.a_rows) * 128;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort)) { ok = false; break; }
+        const bool seg = kb >= p.kb0;
+        const CUtensorMap* ma = seg || second ? &map_a1 : &map_a0;
+        const int k = (kb - (seg ? p.kb0 : 0)) * kHBK;
+        uint8_t* sa = smem + stage * kClStage;
+        uint8_t* sb = sa + kHAtom;
+        mbar_arrive_expect_tx(&full_bar[stage], a_bytes + kHAtom);
+        load_atom<AMN, false>(sa, ma, &full_bar[stage], 0, k, row0, 128);
+        if (EPI == kEpiGated) {
+          load_atom<BMN, false>(sb, &map_b0, &full_bar[stage], 0, k, tn * kOutCols, kOutCols);
+          load_atom<BMN, false>(sb + kHAtom / 2, &map_b1, &full_bar[stage], 0, k, tn * kOutCols, kOutCols);
+        } else {
+          load_atom<BMN, false>(sb, seg ? &map_b1 : &map_b0, &full_bar[stage], 0, k, tn * kClBN, kClBN);
+        }
+        if (++stage == kClStages) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) {
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_h(128, kClBN, AMN, BMN) | (p.bf16 ? kIdescBF16 : 0u);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&full_bar[stage], phase, abort)) break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + stage * kClStage);
+        const uint32_t sb = sa + kHAtom;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_f16_ss(tmem_base, atom_desc<AMN>(sa, k), atom_desc<BMN>(sb, k), idesc,
+                     (kb != kb_begin || k != 0) ? 1u : 0u);
+        mma_commit(&empty_bar[stage]);
+        if (++stage == kClStages) { stage = 0; phase ^= 1; }
+      }
+      mma_commit(&acc_full);
+    }
+    __syncwarp();
+  }
+  // Every thread: the accumulator is complete, and with it every load and every MMA of this CTA.
+  bool ok = mbar_wait(&acc_full, 0, nullptr);
+  ok = __all_sync(0xffffffffu, ok && *abort == 0);
+  tc_fence_after();
+  // Partial tile in shared memory: row r at r * 512 bytes, 16-byte units XORed with r & 7.
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp >= 2) {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int r = quarter * 32 + lane;
+#pragma unroll
+    for (int c = half * (kClBN / 2); c < (half + 1) * (kClBN / 2); c += 32) {
+      uint32_t v[32];
+      tmem_ld32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; j += 4)
+        reinterpret_cast<uint4*>(part)[r * 32 + (((c + j) >> 2) ^ (r & 7))] = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    }
+  }
+  tc_fence_before();
+  if (p.splits > 1) cluster_sync();
+  else __syncthreads();
+  if (ok) {
+    const int rows = min(128, p.M - row0);
+    const int per = (rows + p.splits - 1) / p.splits;
+    const int r_begin = rank * per, r_end = min(rows, r_begin + per);
+    const uint32_t part_u = smem_u32(part);
+    uint16_t* out = reinterpret_cast<uint16_t*>(second ? p.out1 : p.out);
+    constexpr int kUnits = kOutCols / 4;
+    auto sum4 = [&](int r, int u) {
+      const int off = r * 32 + (u ^ (r & 7));
+      if (p.splits == 1) return reinterpret_cast<const float4*>(part)[off];
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < p.splits; ++c) {
+        uint32_t a;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(part_u + off * 16), "r"(c));
+        const float4 t = ld_cluster_f4(a);
+        s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+      }
+      return s;
+    };
+    for (int i = r_begin * kUnits + static_cast<int>(threadIdx.x); i < r_end * kUnits; i += kHThreads) {
+      const int r = i / kUnits, u = i % kUnits;
+      const int col = tn * kOutCols + 4 * u;
+      const int n = p.N - col;                           // columns left, from this unit on
+      if (n <= 0) continue;
+      const int64_t row = row0 + r;
+      float4 s = sum4(r, u);
+      if (p.bias != nullptr) {
+        const float4 b = load4(reinterpret_cast<const uint16_t*>(p.bias) + col, n, false, p.bf16);
+        s.x += b.x; s.y += b.y; s.z += b.z; s.w += b.w;
+      }
+      if (p.z0 != nullptr) {
+        float* z = p.z0 + row * p.ldz + col;             // rows of z are padded to 4 floats
+        *reinterpret_cast<float4*>(z) = s;
+      }
+      s = make_float4(act_value(s.x, p.act), act_value(s.y, p.act), act_value(s.z, p.act), act_value(s.w, p.act));
+      if (EPI == kEpiGated) {
+        float4 t = sum4(r, u + kUnits);
+        if (p.bias1 != nullptr) {
+          const float4 b = load4(reinterpret_cast<const uint16_t*>(p.bias1) + col, n, false, p.bf16);
+          t.x += b.x; t.y += b.y; t.z += b.z; t.w += b.w;
+        }
+        if (p.z1 != nullptr) *reinterpret_cast<float4*>(p.z1 + row * p.ldz + col) = t;
+        s.x *= t.x; s.y *= t.y; s.z *= t.z; s.w *= t.w;
+      } else if (p.residual != nullptr) {
+        const float4 b = load4(reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr + col, n, p.res_vec, p.bf16);
+        s.x += b.x; s.y += b.y; s.z += b.z; s.w += b.w;
+      }
+      const uint32_t lo = pack_h2(s.x, s.y, p.bf16), hi = pack_h2(s.z, s.w, p.bf16);
+      uint16_t* dst = out + row * p.ldo + col;
+      if (p.out_vec && n >= 4) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      } else {
+        dst[0] = static_cast<uint16_t>(lo);
+        if (n > 1) dst[1] = static_cast<uint16_t>(lo >> 16);
+        if (n > 2) dst[2] = static_cast<uint16_t>(hi);
+        if (n > 3) dst[3] = static_cast<uint16_t>(hi >> 16);
+      }
+    }
+  }
+  // No CTA leaves while another may still read its partials.
+  if (p.splits > 1) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kClBN);
+  }
+}
+
+}  // namespace dc

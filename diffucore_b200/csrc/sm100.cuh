@@ -12,14 +12,15 @@
 
 namespace dc {
 
-// Device-global error word. 0 = no error; otherwise the first code recorded. The library is
-// one translation unit (dc_api.cu includes every kernel header), so it is defined here.
-__device__ unsigned int g_device_error = 0;
+// Device-global error word. 0 = no error; otherwise the first code recorded. Each translation unit
+// has its own (dc_api.cu, text_api.cu); dc_device_error() reads and clears both.
+static __device__ unsigned int g_device_error = 0;
 
 enum DeviceErrorCode : unsigned int {
   kErrNone = 0,
   kErrWaitTimeout = 1,     // an mbarrier wait ran past its cycle limit
   kErrSelfTest = 2,        // the timeout self-test recorded its expected expiry
+  kErrTokenId = 3,         // an embedding kernel met a token id outside its table
 };
 
 // ~2 s at 1.9 GHz. Long enough that a healthy pipeline never reaches it.
@@ -274,6 +275,14 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Four floats of a CTA's shared memory in the cluster (`addr` from cluster_addr).
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // Arrive on an mbarrier of another CTA in the cluster (`addr` from cluster_addr).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(addr) : "memory");
@@ -334,6 +343,14 @@ __device__ __forceinline__ void mma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc,
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void mma_f16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
 }
 

@@ -1,0 +1,609 @@
+// C entry points of the text operators: dense and gated projections, layer norm and token
+// embedding with their gradients. Same conventions as dc_api.cu: an int status, caller-owned outputs
+// and workspaces, every launch on the caller's stream, nothing synchronizes.
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
+#include <cstring>
+
+#include "host.cuh"
+#include "sm100.cuh"
+#include "hgemm.cuh"
+#include "textgrad.cuh"
+#include "norm.cuh"
+#include "embed.cuh"
+
+namespace dc {
+int text_device_error(unsigned int* code, int clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code));
+  if (e != cudaSuccess) return cuda_fail(e, "reading the device error word");
+  if (clear && *code) {
+    const unsigned int zero = 0;
+    e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+    if (e != cudaSuccess) return cuda_fail(e, "clearing the device error word");
+  }
+  return DC_OK;
+}
+}  // namespace dc
+
+namespace {
+
+cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t elem_size(int dtype) { return dtype == DC_DTYPE_F32 ? 4 : 2; }
+
+// ------------------------------------------------------------------------------ projections
+
+// An operand of the contraction as the tensor core sees it: `rows` row indices x `k` contraction
+// indices; mn: stored [k][rows] (the row index contiguous), else [rows][k].
+struct Operand {
+  const void* p = nullptr;
+  int64_t ld = 0;
+  int64_t rows = 0, k = 0;
+};
+
+int operand_map(CUtensorMap* map, const Operand& o, bool mn, int box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(mn ? o.rows : o.k), static_cast<uint64_t>(mn ? o.k : o.rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(o.ld) * 2};
+  const uint32_t box[2] = {64, static_cast<uint32_t>(mn ? 64 : box_rows)};
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, o.p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int check_operand(const char* what, const char* name, const void* p, int64_t ld, int64_t cols) {
+  if (p == nullptr) return fail("%s: %s is null", what, name);
+  if (!aligned(p, 16) || ld % 8) return fail("%s: %s needs a 16-byte aligned base and rows of a multiple of 16 bytes", what, name);
+  if (ld < cols) return fail("%s: leading dimension of %s smaller than its row", what, name);
+  return DC_OK;
+}
+
+int check_dims(const char* what, int dtype, int64_t M, int64_t N, int64_t K) {
+  if (dtype != DC_DTYPE_BF16 && dtype != DC_DTYPE_F16) return fail("%s: dtype must be bf16 or fp16", what);
+  if (M < 0 || N <= 0 || K <= 0) return fail("%s: bad shape M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
+  if (M > (1ll << 30) || N > (1ll << 30) || K > (1ll << 30)) return fail("%s: dimension above 2^30", what);
+  return DC_OK;
+}
+
+int check_act(const char* what, int act) {
+  if (act < dc::kActNone || act > dc::kActGeluTanh) return fail("%s: unknown activation %d", what, act);
+  return DC_OK;
+}
+
+// DC_HGEMM_PAIR = "0" / "1": force the cluster / the pair kernel (both compute every shape).
+int pair_override() {
+  const char* env = getenv("DC_HGEMM_PAIR");
+  if (env == nullptr || (strcmp(env, "0") != 0 && strcmp(env, "1") != 0)) return -1;
+  return env[0] - '0';
+}
+
+// One contraction: A rows x B rows, over one or two segments of k (a0 . b0 + a1 . b1), or, with
+// `stacked`, two A operands of equal shape whose rows follow one another (their products go to
+// p.out and p.out1).
+template <bool AMN, bool BMN, int EPI>
+int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const Operand& b1, bool stacked,
+                 dc::HGemmParams p, cudaStream_t st) {
+  const int n_out = EPI == dc::kEpiGated ? 2 * p.N : p.N;       // accumulator columns
+  const int sms = sm_count();
+  const int64_t pair_tiles = ceil_div(p.M, 256) * (stacked ? 2 : 1) * ceil_div(n_out, dc::kPairBN);
+  const int forced = pair_override();
+  const bool pair = forced >= 0 ? forced == 1 : p.M > 256 && pair_tiles * 4 >= sms;
+  const int tile_m = pair ? 256 : 128;
+  const int tile_n = (pair ? dc::kPairBN : dc::kClBN) / (EPI == dc::kEpiGated ? 2 : 1);
+  const int bk = pair ? dc::kPairAtoms * dc::kHBK : dc::kHBK;
+  const int half_m = static_cast<int>(ceil_div(p.M, tile_m));
+  p.tiles_m = half_m * (stacked ? 2 : 1);
+  p.tiles_n = static_cast<int>(ceil_div(p.N, tile_n));
+  p.m_split = stacked ? half_m : INT32_MAX;
+  p.group_m = 8;
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  if (tiles * 8 > INT32_MAX) return fail("projection: too many tiles");
+  p.num_tiles = static_cast<int>(tiles);
+  p.kb0 = static_cast<int>(ceil_div(a0.k, bk));
+  p.kb1 = !stacked && a1.p != nullptr ? static_cast<int>(ceil_div(a1.k, bk)) : 0;
+  p.a_rows = static_cast<int>(std::min<int64_t>(128, round_up(std::min<int64_t>(p.M, 128), 8)));
+  p.out_vec = aligned(p.out, 16) && (p.out1 == nullptr || aligned(p.out1, 16)) && p.ldo % 8 == 0;
+  p.res_vec = p.residual != nullptr && aligned(p.residual, 16) && p.ldr % 8 == 0;
+  const int box_a = pair ? 128 : p.a_rows;
+  const int box_b = EPI == dc::kEpiGated && !pair ? dc::kClBN / 2 : 128;
+  CUtensorMap ma0, ma1, mb0, mb1;
+  int r;
+  if ((r = operand_map(&ma0, a0, AMN, box_a))) return r;
+  if ((r = operand_map(&mb0, b0, BMN, box_b))) return r;
+  if (a1.p == nullptr) ma1 = ma0;
+  else if ((r = operand_map(&ma1, a1, AMN, box_a))) return r;
+  if (b1.p == nullptr) mb1 = mb0;
+  else if ((r = operand_map(&mb1, b1, BMN, box_b))) return r;
+
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(dc::kHThreads);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  if (pair) {
+    auto kernel = dc::hgemm_pair_kernel<AMN, BMN, EPI>;
+    if ((r = set_smem(kernel, dc::kPairSmem))) return r;
+    p.splits = 1;
+    attr[0].val.clusterDim.x = 2;
+    cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min(p.num_tiles, sms / 2)));
+    cfg.dynamicSmemBytes = dc::kPairSmem;
+    e = cudaLaunchKernelEx(&cfg, kernel, ma0, ma1, mb0, mb1, p);
+  } else {
+    auto kernel = dc::hgemm_cluster_kernel<AMN, BMN, EPI>;
+    if ((r = set_smem(kernel, dc::kClSmem))) return r;
+    p.splits = 1;
+    while (p.splits < 8 && 2 * p.splits * tiles <= 2 * sms && (p.kb0 + p.kb1) / (2 * p.splits) >= 4) p.splits *= 2;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits));
+    cfg.dynamicSmemBytes = dc::kClSmem;
+    e = cudaLaunchKernelEx(&cfg, kernel, ma0, ma1, mb0, mb1, p);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "projection launch");
+  DC_CHECK_LAUNCH("projection launch");
+  return DC_OK;
+}
+
+int check_z(const char* what, const float* z, int64_t ldz, int64_t N) {
+  if (z == nullptr) return DC_OK;
+  if (!aligned(z, 16) || ldz % 4 || ldz < round_up(N, 4))
+    return fail("%s: kept pre-activations need 16-byte aligned rows of at least N rounded up to 4", what);
+  return DC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+              int64_t ldr, void* y, int64_t ldy, float* z, int64_t ldz, int dtype, int64_t M, int64_t N, int64_t K,
+              int act, void* stream) {
+  int r;
+  if ((r = check_dims("linear", dtype, M, N, K)) || (r = check_act("linear", act))) return r;
+  if (M == 0) return DC_OK;
+  if ((r = check_operand("linear", "x", x, ldx, K)) || (r = check_operand("linear", "w", w, ldw, K))) return r;
+  if (y == nullptr) return fail("linear: y is null");
+  if (!aligned(y, 2) || !aligned(bias, 2) || !aligned(residual, 2)) return fail("linear: pointers must be aligned to their element size");
+  if (ldy < N || (residual != nullptr && ldr < 0)) return fail("linear: leading dimension smaller than the row");
+  if ((r = check_z("linear", z, ldz, N)) || (r = check_sm100())) return r;
+  dc::HGemmParams p = {};
+  p.M = static_cast<int>(M); p.N = static_cast<int>(N);
+  p.out = y; p.ldo = ldy; p.bias = bias; p.residual = residual; p.ldr = ldr;
+  p.z0 = z; p.ldz = ldz; p.act = act; p.bf16 = dtype == DC_DTYPE_BF16;
+  return launch_hgemm<false, false, dc::kEpiLinear>({x, ldx, M, K}, {}, {w, ldw, N, K}, {}, false, p, as_stream(stream));
+}
+
+int dc_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
+                    const void* b_gate, const void* b_up, void* h, int64_t ldh, float* z_gate, float* z_up,
+                    int64_t ldz, int dtype, int64_t M, int64_t N, int64_t K, int act, void* stream) {
+  int r;
+  if ((r = check_dims("gated_linear", dtype, M, N, K)) || (r = check_act("gated_linear", act))) return r;
+  if (M == 0) return DC_OK;
+  if ((r = check_operand("gated_linear", "x", x, ldx, K)) || (r = check_operand("gated_linear", "w_gate", w_gate, ldwg, K)) ||
+      (r = check_operand("gated_linear", "w_up", w_up, ldwu, K)))
+    return r;
+  if (h == nullptr) return fail("gated_linear: h is null");
+  if (!aligned(h, 2) || !aligned(b_gate, 2) || !aligned(b_up, 2)) return fail("gated_linear: pointers must be aligned to their element size");
+  if (ldh < N) return fail("gated_linear: leading dimension smaller than the row");
+  if ((z_gate == nullptr) != (z_up == nullptr)) return fail("gated_linear: z_gate and z_up go together");
+  if ((r = check_z("gated_linear", z_gate, ldz, N)) || (r = check_z("gated_linear", z_up, ldz, N)) || (r = check_sm100())) return r;
+  dc::HGemmParams p = {};
+  p.M = static_cast<int>(M); p.N = static_cast<int>(N);
+  p.out = h; p.ldo = ldh; p.bias = b_gate; p.bias1 = b_up;
+  p.z0 = z_gate; p.z1 = z_up; p.ldz = ldz; p.act = act; p.bf16 = dtype == DC_DTYPE_BF16;
+  return launch_hgemm<false, false, dc::kEpiGated>({x, ldx, M, K}, {}, {w_gate, ldwg, N, K}, {w_up, ldwu, N, K}, false,
+                                                   p, as_stream(stream));
+}
+
+int dc_linear_dx(const void* dz, const void* dz1, int64_t lddz, const void* w, int64_t ldw, const void* w1, int64_t ldw1,
+                 void* dx, int64_t lddx, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  int r;
+  if ((r = check_dims("linear_dx", dtype, M, N, K))) return r;
+  if (M == 0) return DC_OK;
+  if ((r = check_operand("linear_dx", "dz", dz, lddz, N)) || (r = check_operand("linear_dx", "w", w, ldw, K))) return r;
+  if ((dz1 == nullptr) != (w1 == nullptr)) return fail("linear_dx: dz1 and w1 go together");
+  if (dz1 != nullptr && ((r = check_operand("linear_dx", "dz1", dz1, lddz, N)) || (r = check_operand("linear_dx", "w1", w1, ldw1, K)))) return r;
+  if (dx == nullptr || !aligned(dx, 2)) return fail("linear_dx: dx is null or not aligned to its element size");
+  if (lddx < K) return fail("linear_dx: leading dimension smaller than the row");
+  if ((r = check_sm100())) return r;
+  dc::HGemmParams p = {};
+  p.M = static_cast<int>(M); p.N = static_cast<int>(K);
+  p.out = dx; p.ldo = lddx; p.bf16 = dtype == DC_DTYPE_BF16;
+  return launch_hgemm<false, true, dc::kEpiLinear>({dz, lddz, M, N}, {dz1, lddz, M, N}, {w, ldw, K, N}, {w1, ldw1, K, N},
+                                                   false, p, as_stream(stream));
+}
+
+int dc_linear_dw(const void* dz, const void* dz1, int64_t lddz, const void* x, int64_t ldx, void* dw, void* dw1,
+                 int64_t lddw, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  int r;
+  if ((r = check_dims("linear_dw", dtype, M, N, K))) return r;
+  if (M == 0) return fail("linear_dw: no rows to sum (M = 0): the gradient is zero");
+  if ((r = check_operand("linear_dw", "dz", dz, lddz, N)) || (r = check_operand("linear_dw", "x", x, ldx, K))) return r;
+  if ((dz1 == nullptr) != (dw1 == nullptr)) return fail("linear_dw: dz1 and dw1 go together");
+  if (dz1 != nullptr && (r = check_operand("linear_dw", "dz1", dz1, lddz, N))) return r;
+  if (dw == nullptr || !aligned(dw, 2) || !aligned(dw1, 2)) return fail("linear_dw: dw is null or not aligned to its element size");
+  if (lddw < K) return fail("linear_dw: leading dimension smaller than the row");
+  if ((r = check_sm100())) return r;
+  dc::HGemmParams p = {};
+  p.M = static_cast<int>(N); p.N = static_cast<int>(K);
+  p.out = dw; p.out1 = dw1; p.ldo = lddw; p.bf16 = dtype == DC_DTYPE_BF16;
+  return launch_hgemm<true, true, dc::kEpiLinear>({dz, lddz, N, M}, {dz1, lddz, N, M}, {x, ldx, K, M}, {}, dz1 != nullptr,
+                                                  p, as_stream(stream));
+}
+
+}  // extern "C"
+
+namespace {
+
+// Row blocks of the column sums: enough CTAs for eight per SM, at least 16 rows each.
+int64_t grad_row_blocks(int64_t M, int64_t N) {
+  const int64_t col_blocks = ceil_div(N, dc::kGradCols);
+  return std::max<int64_t>(1, std::min<int64_t>({ceil_div(148 * 8, col_blocks), ceil_div(M, 16), 65535}));
+}
+
+int colsum_finish(const float* p0, const float* p1, int64_t ldp, int64_t P, int64_t N, void* o0, void* o1, int dtype,
+                  cudaStream_t st) {
+  dc::colsum_finish_kernel<<<dim3(static_cast<unsigned>(ceil_div(N, 32)), o1 != nullptr ? 2 : 1), 256, 0, st>>>(
+      p0, p1, ldp, static_cast<int>(P), N, o0, o1, dtype);
+  DC_CHECK_LAUNCH("column sums launch");
+  return DC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_act_grad_workspace(int64_t M, int64_t N, size_t* bytes) {
+  if (M < 0 || N <= 0 || bytes == nullptr) return fail("act_grad: bad shape M=%lld N=%lld", (long long)M, (long long)N);
+  *bytes = static_cast<size_t>(grad_row_blocks(M, N)) * round_up(N, 4) * 2 * sizeof(float);
+  return DC_OK;
+}
+
+int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, int64_t ldz, void* dz, void* dz1,
+                int64_t lddz, void* db, void* db1, void* workspace, size_t workspace_bytes, int dtype, int64_t M,
+                int64_t N, int act, void* stream) {
+  int r;
+  if ((r = check_dims("act_grad", dtype, M, N, 1)) || (r = check_act("act_grad", act))) return r;
+  if (M == 0) return fail("act_grad: no rows (M = 0): every gradient is empty or zero");
+  if (dy == nullptr || !aligned(dy, 2) || lddy < N) return fail("act_grad: dy is null, misaligned or its rows overlap");
+  if (z == nullptr && (z1 != nullptr || dz != nullptr)) return fail("act_grad: dz needs the kept pre-activations");
+  if (z == nullptr && db == nullptr) return fail("act_grad: nothing to compute");
+  if ((r = check_z("act_grad", z, ldz, N)) || (r = check_z("act_grad", z1, ldz, N))) return r;
+  if (z != nullptr) {
+    if ((r = check_operand("act_grad", "dz", dz, lddz, N))) return r;
+    if (z1 != nullptr && (r = check_operand("act_grad", "dz1", dz1, lddz, N))) return r;
+  }
+  if (db1 != nullptr && (z1 == nullptr || db == nullptr)) return fail("act_grad: db1 needs z1 and db");
+  const int64_t blocks = grad_row_blocks(M, N), ldp = round_up(N, 4);
+  if (db != nullptr) {
+    size_t need = 0;
+    dc_act_grad_workspace(M, N, &need);
+    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need)
+      return fail("act_grad: workspace below %zu bytes or misaligned", need);
+    if (!aligned(db, 2) || !aligned(db1, 2)) return fail("act_grad: db must be aligned to its element size");
+  }
+  if ((r = check_sm100())) return r;
+  dc::ActGradParams p = {};
+  p.dy = static_cast<const uint16_t*>(dy); p.lddy = lddy;
+  p.z0 = z; p.z1 = z1; p.ldz = ldz;
+  p.dz0 = static_cast<uint16_t*>(dz); p.dz1 = static_cast<uint16_t*>(dz1); p.lddz = lddz;
+  p.part0 = db != nullptr ? static_cast<float*>(workspace) : nullptr;
+  p.part1 = db != nullptr ? static_cast<float*>(workspace) + blocks * ldp : nullptr;
+  p.ldp = ldp; p.M = M; p.N = N;
+  p.rows_per_block = static_cast<int>(ceil_div(M, blocks));
+  p.act = act; p.bf16 = dtype == DC_DTYPE_BF16;
+  p.dy_vec = aligned(dy, 8) && lddy % 4 == 0;
+  const cudaStream_t st = as_stream(stream);
+  const dim3 grid(static_cast<unsigned>(ceil_div(N, dc::kGradCols)), static_cast<unsigned>(blocks));
+  if (z1 != nullptr) dc::act_grad_kernel<true><<<grid, dc::kGradThreads, 0, st>>>(p);
+  else dc::act_grad_kernel<false><<<grid, dc::kGradThreads, 0, st>>>(p);
+  DC_CHECK_LAUNCH("act_grad launch");
+  if (db != nullptr) return colsum_finish(p.part0, p.part1, ldp, blocks, N, db, db1, dtype, st);
+  return DC_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------ layer norm
+
+namespace {
+
+constexpr int64_t kNormReg = 8192;             // widest row held in registers
+
+int64_t norm_wide_blocks(int64_t M, int64_t D) {
+  return std::max<int64_t>(1, std::min<int64_t>({ceil_div(148 * 8, ceil_div(D, 256)), ceil_div(M, 16), 65535}));
+}
+// CTAs of the persistent backward kernel.
+int64_t norm_bwd_ctas(int64_t M, int64_t D) {
+  if (D > kNormReg) return norm_wide_blocks(M, D);
+  const int64_t rows = D <= 512 ? 8 : 1, per_sm = D <= 512 ? 4 : D <= 2048 ? 6 : 2;
+  return std::min<int64_t>(ceil_div(M, rows), 148 * per_sm);
+}
+
+template <typename T, int E, bool BWD>
+int launch_norm_reg(const dc::NormParams& p, int64_t ctas, cudaStream_t st) {
+  auto go = [&](auto tpr, auto ept) {
+    constexpr int TPR = decltype(tpr)::value, EPT = decltype(ept)::value;
+    if constexpr (BWD)
+      dc::norm_bwd_kernel<T, E, EPT, TPR><<<static_cast<unsigned>(ctas), dc::NormCta<TPR>::kThreads, 0, st>>>(p);
+    else
+      dc::norm_fwd_kernel<T, E, EPT, TPR><<<static_cast<unsigned>(ctas), dc::NormCta<TPR>::kThreads, 0, st>>>(p);
+  };
+  using std::integral_constant;
+  if (p.D <= 256) go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+  else if (p.D <= 512) go(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  else if (p.D <= 1024) go(integral_constant<int, 128>{}, integral_constant<int, 8>{});
+  else if (p.D <= 2048) go(integral_constant<int, 128>{}, integral_constant<int, 16>{});
+  else if (p.D <= 4096) go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+  else go(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+  DC_CHECK_LAUNCH("layer_norm launch");
+  return DC_OK;
+}
+
+template <typename T, bool BWD>
+int launch_norm(const dc::NormParams& p, bool vec, cudaStream_t st) {
+  constexpr int E = 16 / sizeof(T);
+  if (p.D <= kNormReg) {
+    const int64_t ctas = BWD ? norm_bwd_ctas(p.M, p.D) : ceil_div(p.M, p.D <= 512 ? 8 : 1);
+    return vec ? launch_norm_reg<T, E, BWD>(p, ctas, st) : launch_norm_reg<T, 1, BWD>(p, ctas, st);
+  }
+  if constexpr (BWD) {
+    dc::norm_dx_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
+    DC_CHECK_LAUNCH("layer_norm_grad launch");
+    if (p.part_w != nullptr) {
+      const int64_t blocks = norm_wide_blocks(p.M, p.D);
+      dc::norm_dw_wide_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(p.D, 256)), static_cast<unsigned>(blocks)), 256, 0, st>>>(
+          p, static_cast<int>(ceil_div(p.M, blocks)));
+    }
+  } else {
+    dc::norm_fwd_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
+  }
+  DC_CHECK_LAUNCH("layer_norm launch");
+  return DC_OK;
+}
+
+template <bool BWD>
+int dispatch_norm(const dc::NormParams& p, int dtype, bool vec, cudaStream_t st) {
+  switch (dtype) {
+    case DC_DTYPE_F32: return launch_norm<float, BWD>(p, vec, st);
+    case DC_DTYPE_F16: return launch_norm<__half, BWD>(p, vec, st);
+    default: return launch_norm<__nv_bfloat16, BWD>(p, vec, st);
+  }
+}
+
+int check_norm(const char* what, int dtype, int w_dtype, int64_t M, int64_t D) {
+  if (dtype != DC_DTYPE_F32 && dtype != DC_DTYPE_F16 && dtype != DC_DTYPE_BF16) return fail("%s: unsupported dtype %d", what, dtype);
+  if (w_dtype != dtype && w_dtype != DC_DTYPE_F32) return fail("%s: the weight must be in x's type or fp32", what);
+  if (M < 0 || D <= 0 || M > INT32_MAX || D > (1 << 30)) return fail("%s: bad shape M=%lld D=%lld", what, (long long)M, (long long)D);
+  return DC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_layer_norm(const void* x, int64_t ldx, const void* w, const void* b, int w_dtype, void* y, int64_t ldy,
+                  float* mean, float* rstd, int dtype, int64_t M, int64_t D, float eps, void* stream) {
+  int r;
+  if ((r = check_norm("layer_norm", dtype, w_dtype, M, D))) return r;
+  if (M == 0) return DC_OK;
+  const size_t es = elem_size(dtype), ws = elem_size(w_dtype);
+  if (x == nullptr || y == nullptr) return fail("layer_norm: null pointer");
+  if (!aligned(x, es) || !aligned(y, es) || !aligned(w, ws) || !aligned(b, ws) || !aligned(mean, 4) || !aligned(rstd, 4))
+    return fail("layer_norm: pointers must be aligned to their element size");
+  if (ldx < 0 || ldy < D) return fail("layer_norm: leading dimension smaller than the row");
+  if ((mean == nullptr) != (rstd == nullptr)) return fail("layer_norm: mean and rstd go together");
+  if ((r = check_sm100())) return r;
+  dc::NormParams p = {};
+  p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.out = y; p.ldo = ldy; p.mean = mean; p.rstd = rstd;
+  p.M = M; p.D = static_cast<int>(D); p.eps = eps; p.w_f32 = w_dtype == DC_DTYPE_F32;
+  const int64_t e = 16 / static_cast<int64_t>(es);
+  const bool vec = D % e == 0 && ldx % e == 0 && ldy % e == 0 && aligned(x, 16) && aligned(y, 16) && aligned(w, 16) && aligned(b, 16);
+  return dispatch_norm<false>(p, dtype, vec, as_stream(stream));
+}
+
+int dc_layer_norm_grad_workspace(int64_t M, int64_t D, size_t* bytes) {
+  if (M < 0 || D <= 0 || bytes == nullptr) return fail("layer_norm_grad: bad shape M=%lld D=%lld", (long long)M, (long long)D);
+  *bytes = static_cast<size_t>(norm_bwd_ctas(M, D)) * round_up(D, 4) * 2 * sizeof(float);
+  return DC_OK;
+}
+
+int dc_layer_norm_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int w_dtype,
+                       const float* mean, const float* rstd, void* dx, int64_t lddx, void* dw, void* db,
+                       void* workspace, size_t workspace_bytes, int dtype, int64_t M, int64_t D, void* stream) {
+  int r;
+  if ((r = check_norm("layer_norm_grad", dtype, w_dtype, M, D))) return r;
+  if (M == 0) return fail("layer_norm_grad: no rows (M = 0): every gradient is empty or zero");
+  const size_t es = elem_size(dtype), ws = elem_size(w_dtype);
+  if (dy == nullptr || x == nullptr || dx == nullptr || mean == nullptr || rstd == nullptr) return fail("layer_norm_grad: null pointer");
+  if (!aligned(x, es) || !aligned(dy, es) || !aligned(dx, es) || !aligned(w, ws) || !aligned(dw, ws) || !aligned(db, ws) ||
+      !aligned(mean, 4) || !aligned(rstd, 4))
+    return fail("layer_norm_grad: pointers must be aligned to their element size");
+  if (ldx < 0 || lddy < 0 || lddx < D) return fail("layer_norm_grad: leading dimension smaller than the row");
+  if (dw == nullptr && db != nullptr) return fail("layer_norm_grad: db is computed with dw");
+  size_t need = 0;
+  dc_layer_norm_grad_workspace(M, D, &need);
+  if (dw != nullptr && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need))
+    return fail("layer_norm_grad: workspace below %zu bytes or misaligned", need);
+  if ((r = check_sm100())) return r;
+  dc::NormParams p = {};
+  p.x = x; p.ldx = ldx; p.dy = dy; p.lddy = lddy; p.w = w; p.out = dx; p.ldo = lddx;
+  p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
+  p.ldp = round_up(D, 4);
+  const int64_t ctas = norm_bwd_ctas(M, D);
+  if (dw != nullptr) { p.part_w = static_cast<float*>(workspace); p.part_b = p.part_w + ctas * p.ldp; }
+  p.M = M; p.D = static_cast<int>(D); p.w_f32 = w_dtype == DC_DTYPE_F32;
+  const int64_t e = 16 / static_cast<int64_t>(es);
+  const bool vec = D % e == 0 && ldx % e == 0 && lddy % e == 0 && lddx % e == 0 && aligned(x, 16) && aligned(dy, 16) &&
+                   aligned(dx, 16) && aligned(w, 16);
+  const cudaStream_t st = as_stream(stream);
+  if ((r = dispatch_norm<true>(p, dtype, vec, st))) return r;
+  if (dw != nullptr) return colsum_finish(p.part_w, p.part_b, p.ldp, ctas, D, dw, db, w_dtype, st);
+  return DC_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------ embedding
+
+namespace {
+
+int check_embed(const char* what, int dtype, int64_t T, int64_t V, int64_t D) {
+  if (dtype != DC_DTYPE_F32 && dtype != DC_DTYPE_F16 && dtype != DC_DTYPE_BF16) return fail("%s: unsupported dtype %d", what, dtype);
+  if (T < 0 || V <= 0 || D <= 0 || T > INT32_MAX - 4096 || V >= INT32_MAX || D > (1 << 30))
+    return fail("%s: bad shape T=%lld V=%lld D=%lld", what, (long long)T, (long long)V, (long long)D);
+  return DC_OK;
+}
+
+template <typename T, int E>
+int launch_embed_fwd(const dc::EmbedIds& ids, const void* table, int64_t ldt, void* out, int64_t ldo, int64_t D, float scale,
+                     cudaStream_t st) {
+  const int64_t vecs = ceil_div(D, E);
+  unsigned bx = 8;
+  while (bx < 128 && bx < vecs) bx *= 2;
+  const unsigned by = 128 / bx;
+  dc::embed_fwd_kernel<T, E><<<static_cast<unsigned>(ceil_div(ids.T, by)), dim3(bx, by), 0, st>>>(
+      ids, static_cast<const T*>(table), ldt, static_cast<T*>(out), ldo, static_cast<int>(D), scale);
+  DC_CHECK_LAUNCH("embedding launch");
+  return DC_OK;
+}
+
+// Workspace of the gradient: two (key, index) pairs of arrays, the radix histogram, the partials.
+struct EmbedPlan {
+  bool rank;                // counting sort in one launch
+  int passes, bits;         // radix
+  int64_t tiles, chunk, chunks;
+  size_t keys[2], idx[2], hist, part, total;
+};
+
+EmbedPlan embed_plan(int64_t T, int64_t V, int64_t D) {
+  EmbedPlan e = {};
+  e.rank = T <= dc::kRankMax && V < (1 << 19);
+  int nbits = 1;
+  while ((V >> nbits) != 0) ++nbits;             // keys are 0 .. V
+  e.passes = e.rank ? 0 : (nbits + dc::kRadixBits - 1) / dc::kRadixBits;
+  e.bits = e.rank ? 0 : (nbits + e.passes - 1) / e.passes;
+  e.tiles = e.rank ? 0 : ceil_div(T, dc::kRadixTile);
+  const int64_t slabs = ceil_div(D, 8 * dc::kSumThreads);
+  e.chunk = 8;
+  while (e.chunk < dc::kSumChunkMax && ceil_div(T, 2 * e.chunk) * slabs >= 4 * 148) e.chunk *= 2;
+  e.chunks = ceil_div(T, e.chunk);
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t a = at; at += (n + 255) / 256 * 256; return a; };
+  for (int i = 0; i < (e.rank ? 1 : 2); ++i) { e.keys[i] = take(T * 4); e.idx[i] = take(T * 4); }
+  e.hist = take((static_cast<size_t>(e.tiles) << e.bits) * 4);
+  e.part = take(static_cast<size_t>(e.chunks) * 2 * D * 4);
+  e.total = at;
+  return e;
+}
+
+template <typename T, int E>
+int launch_embed_sum(const dc::EmbedSumParams& p, int64_t chunks, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(p.D, E * dc::kSumThreads)));
+  if (grid.y > 65535) return fail("embedding_grad: rows of %d values are too wide", p.D);
+  dc::embed_sum_kernel<T, E><<<grid, dc::kSumThreads, 0, st>>>(p);
+  DC_CHECK_LAUNCH("embedding_grad sum launch");
+  dc::embed_join_kernel<T, E><<<grid, dc::kSumThreads, 0, st>>>(p);
+  DC_CHECK_LAUNCH("embedding_grad join launch");
+  return DC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_embedding(const void* ids, int ids_i64, int64_t T, const void* table, int64_t ldt, int64_t V, int64_t D,
+                 float scale, void* out, int64_t ldo, int dtype, void* stream) {
+  int r;
+  if ((r = check_embed("embedding", dtype, T, V, D))) return r;
+  if (T == 0) return DC_OK;
+  const size_t es = elem_size(dtype);
+  if (ids == nullptr || table == nullptr || out == nullptr) return fail("embedding: null pointer");
+  if (!aligned(ids, ids_i64 ? 8 : 4) || !aligned(table, es) || !aligned(out, es))
+    return fail("embedding: pointers must be aligned to their element size");
+  if (ldt < D || ldo < D) return fail("embedding: leading dimension smaller than the row");
+  if ((r = check_sm100())) return r;
+  const dc::EmbedIds e = {ids, ids_i64 != 0, T, V, -1};
+  const int64_t n = 16 / static_cast<int64_t>(es);
+  const bool vec = D % n == 0 && ldt % n == 0 && ldo % n == 0 && aligned(table, 16) && aligned(out, 16);
+  const cudaStream_t st = as_stream(stream);
+  switch (dtype) {
+    case DC_DTYPE_F32: return vec ? launch_embed_fwd<float, 4>(e, table, ldt, out, ldo, D, scale, st)
+                                  : launch_embed_fwd<float, 1>(e, table, ldt, out, ldo, D, scale, st);
+    case DC_DTYPE_F16: return vec ? launch_embed_fwd<__half, 8>(e, table, ldt, out, ldo, D, scale, st)
+                                  : launch_embed_fwd<__half, 1>(e, table, ldt, out, ldo, D, scale, st);
+    default: return vec ? launch_embed_fwd<__nv_bfloat16, 8>(e, table, ldt, out, ldo, D, scale, st)
+                        : launch_embed_fwd<__nv_bfloat16, 1>(e, table, ldt, out, ldo, D, scale, st);
+  }
+}
+
+int dc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, size_t* bytes) {
+  int r;
+  if ((r = check_embed("embedding_grad", DC_DTYPE_F32, T, V, D))) return r;
+  if (bytes == nullptr) return fail("embedding_grad: null pointer");
+  *bytes = embed_plan(T, V, D).total;
+  return DC_OK;
+}
+
+int dc_embedding_grad(const void* dy, int64_t lddy, const void* ids, int ids_i64, int64_t T, int64_t V, int64_t D,
+                      int64_t padding_idx, float scale, void* dtable, void* workspace, size_t workspace_bytes, int dtype,
+                      void* stream) {
+  int r;
+  if ((r = check_embed("embedding_grad", dtype, T, V, D))) return r;
+  const size_t es = elem_size(dtype);
+  if (dtable == nullptr || !aligned(dtable, es)) return fail("embedding_grad: dtable is null or not aligned to its element size");
+  if (T > 0 && (dy == nullptr || ids == nullptr)) return fail("embedding_grad: null pointer");
+  if (!aligned(ids, ids_i64 ? 8 : 4) || !aligned(dy, es)) return fail("embedding_grad: pointers must be aligned to their element size");
+  if (lddy < 0) return fail("embedding_grad: negative leading dimension");
+  const EmbedPlan plan = embed_plan(T, V, D);
+  if (T > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < plan.total))
+    return fail("embedding_grad: workspace below %zu bytes or misaligned", plan.total);
+  if ((r = check_sm100())) return r;
+  const cudaStream_t st = as_stream(stream);
+  cudaError_t ce = cudaMemsetAsync(dtable, 0, static_cast<size_t>(V) * D * es, st);
+  if (ce != cudaSuccess) return cuda_fail(ce, "embedding_grad zero fill");
+  if (T == 0) return DC_OK;
+
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  auto u32 = [&](size_t off) { return reinterpret_cast<uint32_t*>(ws + off); };
+  const dc::EmbedIds e = {ids, ids_i64 != 0, T, V, padding_idx};
+  int cur = 0;
+  if (plan.rank) {
+    dc::embed_rank_kernel<<<static_cast<unsigned>(ceil_div(T, dc::kRankItems)), 32 * dc::kRankWarps, 0, st>>>(
+        e, u32(plan.keys[0]), u32(plan.idx[0]));
+    DC_CHECK_LAUNCH("embedding_grad sort launch");
+  } else {
+    const unsigned tiles = static_cast<unsigned>(plan.tiles);
+    const unsigned threads = 32 * dc::kRadixWarps;
+    for (int pass = 0; pass < plan.passes; ++pass) {
+      const int shift = pass * plan.bits, out = pass & 1, in = out ^ 1;
+      uint32_t* hist = u32(plan.hist);
+      if (pass == 0) dc::radix_hist_kernel<true><<<tiles, threads, 0, st>>>(e, nullptr, hist, shift, plan.bits);
+      else dc::radix_hist_kernel<false><<<tiles, threads, 0, st>>>(e, u32(plan.keys[in]), hist, shift, plan.bits);
+      dc::radix_scan_kernel<<<1, 1024, 0, st>>>(hist, plan.tiles << plan.bits);
+      if (pass == 0)
+        dc::radix_scatter_kernel<true><<<tiles, threads, 0, st>>>(e, nullptr, nullptr, hist, u32(plan.keys[out]),
+                                                                  u32(plan.idx[out]), shift, plan.bits);
+      else
+        dc::radix_scatter_kernel<false><<<tiles, threads, 0, st>>>(e, u32(plan.keys[in]), u32(plan.idx[in]), hist,
+                                                                   u32(plan.keys[out]), u32(plan.idx[out]), shift, plan.bits);
+      DC_CHECK_LAUNCH("embedding_grad sort launch");
+      cur = out;
+    }
+  }
+  dc::EmbedSumParams p = {};
+  p.skey = u32(plan.keys[cur]); p.sidx = u32(plan.idx[cur]);
+  p.T = T; p.V = V; p.dy = dy; p.lddy = lddy; p.out = dtable; p.part = reinterpret_cast<float*>(ws + plan.part);
+  p.D = static_cast<int>(D); p.chunk = static_cast<int>(plan.chunk); p.scale = scale;
+  const int64_t n = 16 / static_cast<int64_t>(es);
+  const bool vec = D % n == 0 && lddy % n == 0 && aligned(dy, 16) && aligned(dtable, 16);
+  switch (dtype) {
+    case DC_DTYPE_F32: return vec ? launch_embed_sum<float, 4>(p, plan.chunks, st) : launch_embed_sum<float, 1>(p, plan.chunks, st);
+    case DC_DTYPE_F16: return vec ? launch_embed_sum<__half, 8>(p, plan.chunks, st) : launch_embed_sum<__half, 1>(p, plan.chunks, st);
+    default: return vec ? launch_embed_sum<__nv_bfloat16, 8>(p, plan.chunks, st) : launch_embed_sum<__nv_bfloat16, 1>(p, plan.chunks, st);
+  }
+}
+
+}  // extern "C"

@@ -445,3 +445,269 @@ def selftest_exp2(x: torch.Tensor):
     poly, ref = torch.empty_like(x), torch.empty_like(x)
     _lib.check(_lib.load().dc_selftest_exp2(_ptr(x), _ptr(poly), _ptr(ref), x.numel(), _stream(x)))
     return poly, ref
+
+
+# ─── text operators (dc_linear, dc_gated_linear, dc_layer_norm, dc_embedding and gradients) ──
+
+_ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU,
+         "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
+
+
+def _launch(fn, t: torch.Tensor, *args) -> None:
+    """Call a C entry point with the current stream of ``t``'s device as its last argument."""
+    dev = t.device.index
+    if dev == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if status != _lib.DC_OK:
+        _lib.check(status)
+
+
+def _addr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _act_code(act) -> int:
+    if act not in _ACTS:
+        raise ValueError(f"unknown activation {act!r}; choose from {sorted(k for k in _ACTS if k)}")
+    return _ACTS[act]
+
+
+def _check_text(what: str, lead: torch.Tensor, dtypes, /, **others: torch.Tensor | None) -> None:
+    """``lead`` is a CUDA tensor of one of ``dtypes``, the others share its type and device."""
+    _require_cuda(lead)
+    if lead.dtype not in dtypes:
+        raise TypeError(f"{what}: unsupported dtype {lead.dtype}")
+    for name, t in others.items():
+        if t is not None and (t.dtype != lead.dtype or t.device != lead.device):
+            raise TypeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {lead.dtype} on {lead.device}")
+
+
+_HALF = (torch.bfloat16, torch.float16)
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def matrix_operand(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [R, C] itself when its rows are what a TMA tile load takes (unit inner stride, 16-byte
+    aligned rows that do not overlap), else a copy with padded rows."""
+    r, c = t.shape
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (r == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= c)):
+        return t
+    return t.new_empty(r, (c + 7) & ~7)[:, :c].copy_(t)
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Leading dimension of a matrix operand (any multiple of 8 will do for a single row)."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) & ~7
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [R, C] with unit inner stride."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _ld_rows(t: torch.Tensor) -> int:
+    """Row stride of a tensor read or written row by row (one row: its width)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(what: str, name: str, t: torch.Tensor | None, n: int) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what}: {name} must have shape ({n},), got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None,
+           residual: torch.Tensor | None = None, keep_z: bool = False):
+    """``(y, z)``: ``y = act(z) + residual``, ``z = x @ w.T + bias`` for 16-bit ``x`` [M, K] and ``w``
+    [N, K] (``dc_linear``). ``z`` is the fp32 pre-activation (rows padded to 4) when ``keep_z``."""
+    _check_text("linear", x, _HALF, w=w, bias=bias, residual=residual)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"linear: x {tuple(x.shape)} does not match w {tuple(w.shape)}")
+    (M, K), N = x.shape, w.shape[0]
+    code = _act_code(act)
+    bias = _vector("linear", "bias", bias, N)
+    if residual is not None:
+        if residual.shape != (M, N):
+            raise ValueError(f"linear: residual must have shape {(M, N)}, got {tuple(residual.shape)}")
+        residual = _rows(residual)
+    x, w = matrix_operand(x), matrix_operand(w)
+    y = x.new_empty(M, N)
+    z = x.new_empty(M, (N + 3) & ~3, dtype=torch.float32) if keep_z else None
+    _launch(_lib.load().dc_linear, x, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _addr(bias), _addr(residual),
+            0 if residual is None else residual.stride(0), y.data_ptr(), N, _addr(z), 0 if z is None else z.shape[1],
+            _DTYPE[x.dtype], M, N, K, code)
+    return y, z
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
+                 b_up: torch.Tensor | None = None, act: str | None = "silu", keep_z: bool = False):
+    """``(h, z_gate, z_up)``: ``h = act(z_gate) * z_up`` of the two projections of ``x`` [M, K] by
+    ``w_gate``, ``w_up`` [N, K] (``dc_gated_linear``); the fp32 pre-activations when ``keep_z``."""
+    _check_text("gated_linear", x, _HALF, w_gate=w_gate, w_up=w_up, b_gate=b_gate, b_up=b_up)
+    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or x.shape[1] != w_gate.shape[1]:
+        raise ValueError(f"gated_linear: shapes of x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)} and w_up "
+                         f"{tuple(w_up.shape)} do not match")
+    (M, K), N = x.shape, w_gate.shape[0]
+    code = _act_code(act)
+    b_gate, b_up = _vector("gated_linear", "b_gate", b_gate, N), _vector("gated_linear", "b_up", b_up, N)
+    x, w_gate, w_up = matrix_operand(x), matrix_operand(w_gate), matrix_operand(w_up)
+    h = x.new_empty(M, N)
+    ldz = (N + 3) & ~3
+    zg, zu = x.new_empty(2, M, ldz, dtype=torch.float32).unbind(0) if keep_z else (None, None)
+    _launch(_lib.load().dc_gated_linear, x, x.data_ptr(), _ld(x), w_gate.data_ptr(), _ld(w_gate), w_up.data_ptr(),
+            _ld(w_up), _addr(b_gate), _addr(b_up), h.data_ptr(), N, _addr(zg), _addr(zu), ldz, _DTYPE[x.dtype],
+            M, N, K, code)
+    return h, zg, zu
+
+
+def act_grad(dy: torch.Tensor, z: torch.Tensor | None, z1: torch.Tensor | None, act: str | None,
+             bias_grad: bool = False, bias_grad1: bool = False):
+    """``(dz, dz1, db, db1)`` from ``dy`` [M, N] and the kept pre-activations (``dc_act_grad``); with
+    ``z`` None, ``dz`` is ``dy``. The ``dz`` rows are padded to matrix-operand alignment."""
+    M, N = dy.shape
+    if z is None and not bias_grad:
+        return dy, None, None, None
+    dy = _rows(dy)
+    if M > 1 and dy.stride(0) < N:
+        dy = dy.contiguous()
+    lib = _lib.load()
+    dz = dz1 = db = db1 = ws = None
+    lddz = (N + 7) & ~7
+    if z is not None:
+        dz = dy.new_empty(M, lddz)[:, :N]
+        if z1 is not None:
+            dz1 = dy.new_empty(M, lddz)[:, :N]
+    nbytes = ctypes.c_size_t(0)
+    if bias_grad or bias_grad1:
+        db = dy.new_empty(N)
+        db1 = dy.new_empty(N) if bias_grad1 else None
+        _lib.check(lib.dc_act_grad_workspace(M, N, ctypes.byref(nbytes)))
+        ws = torch.empty(nbytes.value, device=dy.device, dtype=torch.uint8)
+    _launch(lib.dc_act_grad, dy, dy.data_ptr(), _ld_rows(dy), _addr(z), _addr(z1), 0 if z is None else z.stride(0),
+            _addr(dz), _addr(dz1), lddz, _addr(db), _addr(db1), _addr(ws), nbytes.value, _DTYPE[dy.dtype], M, N,
+            _act_code(act))
+    return (dy if z is None else dz), dz1, db, db1
+
+
+def linear_dx(dz: torch.Tensor, w: torch.Tensor, dz1: torch.Tensor | None = None,
+              w1: torch.Tensor | None = None) -> torch.Tensor:
+    """``dz @ w`` (``+ dz1 @ w1``) for ``dz`` [M, N], ``w`` [N, K] (``dc_linear_dx``)."""
+    dz, w = matrix_operand(dz), matrix_operand(w)
+    if w1 is not None:
+        w1 = matrix_operand(w1)
+    (M, N), K = dz.shape, w.shape[1]
+    dx = dz.new_empty(M, K)
+    _launch(_lib.load().dc_linear_dx, dz, dz.data_ptr(), _addr(dz1), _ld(dz), w.data_ptr(), _ld(w), _addr(w1),
+            0 if w1 is None else _ld(w1), dx.data_ptr(), K, _DTYPE[dz.dtype], M, N, K)
+    return dx
+
+
+def linear_dw(dz: torch.Tensor, x: torch.Tensor, dz1: torch.Tensor | None = None):
+    """``dz.T @ x`` (and ``dz1.T @ x``) for ``dz`` [M, N], ``x`` [M, K] (``dc_linear_dw``):
+    ``(dw, dw1 or None)``."""
+    dz, x = matrix_operand(dz), matrix_operand(x)
+    (M, N), K = dz.shape, x.shape[1]
+    dw = x.new_empty(N, K)
+    dw1 = x.new_empty(N, K) if dz1 is not None else None
+    _launch(_lib.load().dc_linear_dw, dz, dz.data_ptr(), _addr(dz1), _ld(dz), x.data_ptr(), _ld(x), dw.data_ptr(),
+            _addr(dw1), K, _DTYPE[dz.dtype], M, N, K)
+    return dw, dw1
+
+
+def layer_norm(x: torch.Tensor, w: torch.Tensor | None, b: torch.Tensor | None, eps: float, keep_stats: bool = False):
+    """``(y, mean, rstd)`` of the rows of ``x`` [M, D] (``dc_layer_norm``); ``w`` and ``b`` [D] in x's
+    type or fp32. ``mean`` and ``rstd`` are fp32 [M] when ``keep_stats``."""
+    _check_text("layer_norm", x, _FLOATS)
+    M, D = x.shape
+    w, b, wcode = _norm_affine("layer_norm", x, w, b)
+    x = _rows(x)
+    y = x.new_empty(M, D)
+    stats = x.new_empty(2, M, dtype=torch.float32) if keep_stats else None
+    base = _addr(stats)
+    _launch(_lib.load().dc_layer_norm, x, x.data_ptr(), _ld_rows(x), _addr(w), _addr(b), wcode, y.data_ptr(), D,
+            base, base + 4 * M if base else 0, _DTYPE[x.dtype], M, D, eps)
+    return (y, None, None) if stats is None else (y, stats[0], stats[1])
+
+
+def _norm_affine(what: str, x: torch.Tensor, w, b):
+    """The affine vectors in one type the kernels take, and its code."""
+    D = x.shape[-1]
+    for name, t in (("weight", w), ("bias", b)):
+        if t is not None and (t.device != x.device or t.dtype not in (x.dtype, torch.float32)):
+            raise TypeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {x.dtype} or fp32 on {x.device}")
+    w, b = _vector(what, "weight", w, D), _vector(what, "bias", b, D)
+    kinds = {t.dtype for t in (w, b) if t is not None}
+    if len(kinds) == 2:                      # one in x's type, one in fp32
+        w, b = w.float(), b.float()
+    kind = torch.float32 if torch.float32 in kinds else x.dtype
+    return w, b, _DTYPE[kind]
+
+
+def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor | None, mean: torch.Tensor, rstd: torch.Tensor,
+                    weight_grad: bool = True, bias_grad: bool = True, dtype: torch.dtype | None = None):
+    """``(dx, dw, db)`` of :func:`layer_norm` (``dc_layer_norm_grad``). ``dw`` and ``db`` come in
+    ``dtype`` (x's type or fp32; default: ``w``'s, else x's)."""
+    _check_text("layer_norm_grad", dy, _FLOATS, x=x)
+    M, D = x.shape
+    dtype = dtype or (x.dtype if w is None else w.dtype)
+    if w is not None and w.dtype != dtype:
+        w = w.to(dtype)
+    dy, x = _rows(dy), _rows(x)
+    lib = _lib.load()
+    dx = x.new_empty(M, D)
+    dw = db = ws = None
+    nbytes = ctypes.c_size_t(0)
+    if weight_grad or bias_grad:
+        dw = x.new_empty(D, dtype=dtype)
+        db = x.new_empty(D, dtype=dtype) if bias_grad else None
+        _lib.check(lib.dc_layer_norm_grad_workspace(M, D, ctypes.byref(nbytes)))
+        ws = torch.empty(nbytes.value, device=x.device, dtype=torch.uint8)
+    _launch(lib.dc_layer_norm_grad, x, dy.data_ptr(), _ld_rows(dy), x.data_ptr(), _ld_rows(x), _addr(w),
+            _DTYPE[dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D, _addr(dw), _addr(db), _addr(ws),
+            nbytes.value, _DTYPE[x.dtype], M, D)
+    return dx, dw if weight_grad else None, db
+
+
+def _check_ids(what: str, ids: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32) or ids.device != like.device:
+        raise TypeError(f"{what}: ids must be int64 or int32 on {like.device}, got {ids.dtype} on {ids.device}")
+    return ids.reshape(-1).contiguous()
+
+
+def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``scale * table[ids]`` [T, D] for flat ``ids`` and ``table`` [V, D] (``dc_embedding``)."""
+    _check_text("embedding", table, _FLOATS)
+    ids = _check_ids("embedding", ids, table)
+    V, D = table.shape
+    table = _rows(table)
+    if V > 1 and table.stride(0) < D:
+        table = table.contiguous()
+    T = ids.shape[0]
+    out = table.new_empty(T, D)
+    _launch(_lib.load().dc_embedding, table, ids.data_ptr(), int(ids.dtype == torch.int64), T, table.data_ptr(),
+            _ld_rows(table), V, D, scale, out.data_ptr(), D, _DTYPE[table.dtype])
+    return out
+
+
+def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, V: int, scale: float = 1.0,
+                   padding_idx: int = -1) -> torch.Tensor:
+    """The dense gradient [V, D] of :func:`embedding`'s table (``dc_embedding_grad``)."""
+    _check_text("embedding_grad", dy, _FLOATS)
+    ids = _check_ids("embedding_grad", ids, dy)
+    T, D = dy.shape
+    if ids.shape[0] != T:
+        raise ValueError(f"embedding_grad: {ids.shape[0]} ids for {T} rows")
+    dy = _rows(dy)
+    lib = _lib.load()
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(lib.dc_embedding_grad_workspace(T, V, D, ctypes.byref(nbytes)))
+    ws = torch.empty(nbytes.value, device=dy.device, dtype=torch.uint8)
+    out = dy.new_empty(V, D)
+    _launch(lib.dc_embedding_grad, dy, dy.data_ptr(), _ld_rows(dy), ids.data_ptr(), int(ids.dtype == torch.int64), T,
+            V, D, padding_idx, scale, out.data_ptr(), ws.data_ptr(), nbytes.value, _DTYPE[dy.dtype])
+    return out

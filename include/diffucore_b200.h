@@ -61,7 +61,8 @@ int dc_set_quant_division(int mode);
 int dc_quant_division(void);
 
 /* Read (and optionally clear) the device-global error word that bounded in-kernel waits set
- * when they give up (1 = a wait timed out, 2 = the timeout self-test fired). Synchronous. */
+ * when they give up (1 = a wait timed out, 2 = the timeout self-test fired), and the word an embedding lookup sets for
+ * a token id outside its table (3). Synchronous. */
 int dc_device_error(unsigned int* code, int clear);
 
 /* Per-row symmetric int8 quantization of x [M, K] (row stride ldx elements):
@@ -249,6 +250,78 @@ int dc_selftest_exp2(const float* x, float* poly, float* ref, int64_t n, void* s
  * bounded by limit_cycles. The wait gives up, writes 1 to *status_dev (device int) and sets the
  * device error word to 2. No counterpart in the reference (its kernels have no bounded waits). */
 int dc_selftest_wait_timeout(long long limit_cycles, int* status_dev, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Text operators: the dense and gated projections, layer norm and token embedding of prompt
+ * encoders and trained prompt adapters, with their gradients. 16-bit operands are bf16 or fp16
+ * (one type per call); every sum is fp32 in a fixed order, results are rounded once.
+ *
+ * Matrix operands (x, w, dz) are row-major with a 16-byte aligned base and a leading dimension
+ * that is a multiple of 8 elements; outputs, biases and residuals need element alignment only.
+ * --------------------------------------------------------------------------------------------- */
+
+#define DC_ACT_NONE 0
+#define DC_ACT_RELU 1
+#define DC_ACT_SILU 2
+#define DC_ACT_GELU 3        /* 0.5 z (1 + erf(z / sqrt 2)) */
+#define DC_ACT_GELU_TANH 4   /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+
+/* y[M, N] = act(z) + residual, z = x[M, K] . w[N, K]^T + bias. bias [N] and residual [M, N] (row
+ * stride ldr, 0 for one row shared by all) may be null. `z`, if not null, receives z in fp32 for
+ * the backward pass: 16-byte aligned, ldz a multiple of 4 and at least N rounded up to 4. */
+int dc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+              int64_t ldr, void* y, int64_t ldy, float* z, int64_t ldz, int dtype, int64_t M, int64_t N, int64_t K,
+              int act, void* stream);
+
+/* h[M, N] = act(x . w_gate^T + b_gate) * (x . w_up^T + b_up); z_gate and z_up (both or neither)
+ * receive the two pre-activation values in fp32, as in dc_linear. */
+int dc_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
+                    const void* b_gate, const void* b_up, void* h, int64_t ldh, float* z_gate, float* z_up,
+                    int64_t ldz, int dtype, int64_t M, int64_t N, int64_t K, int act, void* stream);
+
+/* Pointwise backward of the projections and the bias gradients, from dy [M, N]:
+ *   dc_linear (z1 null):         dz = dy act'(z), db = column sums of dz; with z null dz is dy and
+ *                                only db is computed
+ *   dc_gated_linear (z, z1):     dz = dy z1 act'(z), dz1 = dy act(z), db / db1 their column sums
+ * dz and dz1 (row stride lddz) are matrix operands of the two calls below; db and db1 may be null,
+ * else `workspace` (16-byte aligned) holds dc_act_grad_workspace() bytes. */
+int dc_act_grad_workspace(int64_t M, int64_t N, size_t* bytes);
+int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, int64_t ldz, void* dz, void* dz1,
+                int64_t lddz, void* db, void* db1, void* workspace, size_t workspace_bytes, int dtype, int64_t M,
+                int64_t N, int act, void* stream);
+
+/* dx[M, K] = dz[M, N] . w[N, K] (+ dz1 . w1 when they are not null, in the same accumulator). */
+int dc_linear_dx(const void* dz, const void* dz1, int64_t lddz, const void* w, int64_t ldw, const void* w1, int64_t ldw1,
+                 void* dx, int64_t lddx, int dtype, int64_t M, int64_t N, int64_t K, void* stream);
+
+/* dw[N, K] = dz[M, N]^T . x[M, K] (and dw1 = dz1^T . x when they are not null, in one launch). */
+int dc_linear_dw(const void* dz, const void* dz1, int64_t lddz, const void* x, int64_t ldx, void* dw, void* dw1,
+                 int64_t lddw, int dtype, int64_t M, int64_t N, int64_t K, void* stream);
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over the rows of x [M, D] (fp32, fp16 or bf16). w and b
+ * may be null and are in x's type or fp32 (w_dtype). mean and rstd [M] (both or neither) are kept
+ * for the backward pass. */
+int dc_layer_norm(const void* x, int64_t ldx, const void* w, const void* b, int w_dtype, void* y, int64_t ldy,
+                  float* mean, float* rstd, int dtype, int64_t M, int64_t D, float eps, void* stream);
+
+/* dx, and with dw not null dw = sum_rows dy xhat, db = sum_rows dy (db may be null) in w_dtype;
+ * `workspace` (16-byte aligned) then holds dc_layer_norm_grad_workspace() bytes. */
+int dc_layer_norm_grad_workspace(int64_t M, int64_t D, size_t* bytes);
+int dc_layer_norm_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int w_dtype,
+                       const float* mean, const float* rstd, void* dx, int64_t lddx, void* dw, void* db,
+                       void* workspace, size_t workspace_bytes, int dtype, int64_t M, int64_t D, void* stream);
+
+/* out[t] = scale * table[ids[t]] for T ids (int64 or int32) into a table [V, D]. An id outside
+ * [0, V) gives a zero row and sets the device error word (3). */
+int dc_embedding(const void* ids, int ids_i64, int64_t T, const void* table, int64_t ldt, int64_t V, int64_t D,
+                 float scale, void* out, int64_t ldo, int dtype, void* stream);
+
+/* dtable[V, D] (contiguous, every row written) = scale * sum of dy[t] over ids[t] == v, in the
+ * order of t. Ids outside [0, V) and padding_idx (-1: none) get no gradient. */
+int dc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, size_t* bytes);
+int dc_embedding_grad(const void* dy, int64_t lddy, const void* ids, int ids_i64, int64_t T, int64_t V, int64_t D,
+                      int64_t padding_idx, float scale, void* dtable, void* workspace, size_t workspace_bytes, int dtype,
+                      void* stream);
 
 #ifdef __cplusplus
 }
