@@ -8,7 +8,7 @@
 // sums are the same on every call, without float atomics):
 //   sort    up to 8192 tokens: each token's place is the number of smaller (id, t) keys, counted
 //           against all keys in shared memory, one launch; more: least-significant-digit radix
-//           passes of up to 9 bits (histogram per tile, scan, stable scatter)
+//           passes of up to 9 bits (histogram per tile, stable scatter)
 //   sum     a CTA per chunk of sorted places and slab of columns adds up runs of equal ids; runs
 //           inside the chunk go to the table, the first and last may continue in the
 //           neighbouring chunks and leave fp32 partials
@@ -61,6 +61,29 @@ embed_fwd_kernel(const EmbedIds ids, const T* __restrict__ table, int64_t ldt, T
   }
 }
 
+// ------------------------------------------------------------------ zero fill
+
+// The gradient's rows start as zeros. The sorting kernels keep few SMs busy and wait on latency, so
+// each launch of theirs carries extra CTAs that zero a slice of the table.
+struct FillSlice {
+  uint8_t* p;               // 16-byte aligned up to `tail`
+  int64_t bytes;
+  int ctas;                 // CTAs of the launch that fill (the first ones sort)
+};
+
+constexpr int kFillCta = 64 << 10;      // bytes per filling CTA, about
+
+__device__ __forceinline__ void fill_slice(const FillSlice& f, int cta) {
+  const int64_t units = f.bytes >> 4;
+  const int64_t stride = static_cast<int64_t>(f.ctas) * blockDim.x;
+  uint4* q = reinterpret_cast<uint4*>(f.p);
+#pragma unroll 4
+  for (int64_t i = static_cast<int64_t>(cta) * blockDim.x + threadIdx.x; i < units; i += stride) q[i] = make_uint4(0, 0, 0, 0);
+  if (cta == 0) {
+    for (int64_t i = (units << 4) + threadIdx.x; i < f.bytes; i += blockDim.x) f.p[i] = 0;
+  }
+}
+
 // ------------------------------------------------------------------ sort
 
 constexpr int kRankMax = 8192;          // tokens of the counting sort: (id, t) fit 19 + 13 bits
@@ -68,7 +91,12 @@ constexpr int kRankItems = 32;          // tokens per CTA
 constexpr int kRankWarps = 8;
 
 __global__ void __launch_bounds__(32 * kRankWarps)
-embed_rank_kernel(const EmbedIds ids, uint32_t* __restrict__ skey, uint32_t* __restrict__ sidx) {
+embed_rank_kernel(const EmbedIds ids, uint32_t* __restrict__ skey, uint32_t* __restrict__ sidx, int ctas,
+                  const FillSlice fill) {
+  if (static_cast<int>(blockIdx.x) >= ctas) {
+    fill_slice(fill, static_cast<int>(blockIdx.x) - ctas);
+    return;
+  }
   __shared__ __align__(16) uint32_t keys[kRankMax];
   __shared__ int count[kRankWarps][32];
   const int T = static_cast<int>(ids.T);
@@ -97,96 +125,93 @@ embed_rank_kernel(const EmbedIds ids, uint32_t* __restrict__ skey, uint32_t* __r
   }
 }
 
-constexpr int kRadixTile = 2048;
+constexpr int kRadixTile = 1024;
 constexpr int kRadixWarps = 8;
 constexpr int kRadixBits = 9;
 constexpr int kRadixDigits = 1 << kRadixBits;
 
-// Digit counts of each tile: hist[digit * tiles + tile]. The first pass reads the ids.
+// Digit counts of each tile: hist[tile * digits + digit]. The first pass reads the ids.
 template <bool FIRST>
 __global__ void __launch_bounds__(32 * kRadixWarps)
 radix_hist_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, uint32_t* __restrict__ hist, int shift,
-                  int bits) {
+                  int bits, int tiles, const FillSlice fill) {
+  if (static_cast<int>(blockIdx.x) >= tiles) {
+    fill_slice(fill, static_cast<int>(blockIdx.x) - tiles);
+    return;
+  }
   __shared__ uint32_t h[kRadixDigits];
   const int digits = 1 << bits;
   for (int d = threadIdx.x; d < digits; d += blockDim.x) h[d] = 0;
   __syncthreads();
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kRadixTile;
-  for (int i = threadIdx.x; i < kRadixTile; i += blockDim.x) {
-    const int64_t t = base + i;
+#pragma unroll
+  for (int i = 0; i < kRadixTile / (32 * kRadixWarps); ++i) {
+    const int64_t t = base + i * (32 * kRadixWarps) + threadIdx.x;
     if (t < ids.T) atomicAdd(&h[((FIRST ? key_at(ids, t) : keys[t]) >> shift) & (digits - 1)], 1u);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += blockDim.x) hist[static_cast<int64_t>(d) * gridDim.x + blockIdx.x] = h[d];
+  for (int d = threadIdx.x; d < digits; d += blockDim.x) hist[static_cast<int64_t>(blockIdx.x) * digits + d] = h[d];
 }
 
-// Exclusive scan of n counts in place, one CTA; each thread scans a run of 16 per step.
-constexpr int kScanPer = 16;
-__global__ void __launch_bounds__(1024)
-radix_scan_kernel(uint32_t* __restrict__ hist, int64_t n) {
-  __shared__ uint32_t warp_sum[32];
-  __shared__ uint32_t total;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t carry = 0;
-  for (int64_t base = 0; base < n; base += 1024 * kScanPer) {
-    const int64_t at = base + static_cast<int64_t>(threadIdx.x) * kScanPer;
-    uint32_t v[kScanPer], s = 0;
-#pragma unroll
-    for (int i = 0; i < kScanPer; ++i) { v[i] = at + i < n ? hist[at + i] : 0u; }
-#pragma unroll
-    for (int i = 0; i < kScanPer; ++i) { const uint32_t x = v[i]; v[i] = s; s += x; }
-    uint32_t incl = s;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    if (lane == 31) warp_sum[warp] = incl;
-    __syncthreads();
-    if (warp == 0) {
-      const uint32_t own = warp_sum[lane];
-      uint32_t x = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      warp_sum[lane] = x - own;
-      if (lane == 31) total = x;
-    }
-    __syncthreads();
-    const uint32_t off = carry + warp_sum[warp] + incl - s;
-#pragma unroll
-    for (int i = 0; i < kScanPer; ++i)
-      if (at + i < n) hist[at + i] = off + v[i];
-    carry += total;
-    __syncthreads();
-  }
-}
-
-// Stable scatter of a tile. Warp w owns keys [256 w, 256 w + 256) of the tile, 32 at a time; a
-// key's place is the digit's base for the tile + equal digits in earlier warps + in earlier rounds
-// of its warp + in lower lanes.
+// Stable scatter of a tile. Warp w owns keys [32 kRounds w, 32 kRounds (w + 1)) of the tile, 32 at a
+// time; a key's place is the number of smaller digits + equal digits in earlier tiles (both summed
+// here from the tiles' counts) + in earlier warps + in earlier rounds of its warp + in lower lanes.
 template <bool FIRST>
 __global__ void __launch_bounds__(32 * kRadixWarps)
 radix_scatter_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ idx,
-                     const uint32_t* __restrict__ base_of, uint32_t* __restrict__ keys_out,
-                     uint32_t* __restrict__ idx_out, int shift, int bits) {
+                     const uint32_t* __restrict__ hist, uint32_t* __restrict__ keys_out,
+                     uint32_t* __restrict__ idx_out, int shift, int bits, int tiles, const FillSlice fill) {
+  if (static_cast<int>(blockIdx.x) >= tiles) {
+    fill_slice(fill, static_cast<int>(blockIdx.x) - tiles);
+    return;
+  }
   __shared__ uint32_t cnt[kRadixWarps][kRadixDigits];
+  __shared__ uint32_t below[kRadixWarps];
   constexpr int kRounds = kRadixTile / (32 * kRadixWarps);
+  constexpr int kPerThread = kRadixDigits / (32 * kRadixWarps);   // digits per thread
   const int digits = 1 << bits;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kRadixWarps * kRadixDigits; i += blockDim.x) (&cnt[0][0])[i] = 0;
-  __syncthreads();
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kRadixTile + warp * (32 * kRounds);
-  uint32_t key[kRounds], place[kRounds];
+  uint32_t key[kRounds], val[kRounds], place[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const int64_t t = base + r * 32 + lane;
-    const bool in = t < ids.T;
-    key[r] = in ? (FIRST ? key_at(ids, t) : keys[t]) : 0u;
+    key[r] = t < ids.T ? (FIRST ? key_at(ids, t) : keys[t]) : 0u;
+    val[r] = t < ids.T ? (FIRST ? static_cast<uint32_t>(t) : idx[t]) : 0u;
+  }
+  for (int i = threadIdx.x; i < kRadixWarps * kRadixDigits; i += blockDim.x) (&cnt[0][0])[i] = 0;
+  // Digits kPerThread * threadIdx.x, ...: counts of all tiles and of the tiles before this one.
+  uint32_t total[kPerThread], before_tile[kPerThread], mine = 0;
+#pragma unroll
+  for (int j = 0; j < kPerThread; ++j) {
+    const int d = threadIdx.x * kPerThread + j;
+    total[j] = 0; before_tile[j] = 0;
+    if (d < digits) {
+#pragma unroll 8
+      for (int i = 0; i < tiles; ++i) {
+        const uint32_t c = hist[static_cast<int64_t>(i) * digits + d];
+        total[j] += c;
+        if (i < static_cast<int>(blockIdx.x)) before_tile[j] += c;
+      }
+    }
+    mine += total[j];
+  }
+  uint32_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) below[warp] = incl;
+  __syncthreads();                          // cnt is zero, below is complete
+  uint32_t smaller = incl - mine;           // keys with a smaller digit than this thread's first
+#pragma unroll
+  for (int w = 0; w < kRadixWarps; ++w) smaller += w < warp ? below[w] : 0u;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const bool in = base + r * 32 + lane < ids.T;
     const uint32_t d = (key[r] >> shift) & (digits - 1);
-    // lanes past the end form a group of their own (digit count is at most 512)
+    // lanes past the end form a group of their own (digits are below 512)
     const uint32_t peers = __match_any_sync(0xffffffffu, in ? d : 0xFFFFu);
     place[r] = __popc(peers & ((1u << lane) - 1u));
     uint32_t before = 0;
@@ -197,19 +222,23 @@ radix_scatter_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, cons
     place[r] += before;
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += blockDim.x) {
-    uint32_t s = base_of[static_cast<int64_t>(d) * gridDim.x + blockIdx.x];
 #pragma unroll
-    for (int w = 0; w < kRadixWarps; ++w) { const uint32_t c = cnt[w][d]; cnt[w][d] = s; s += c; }
+  for (int j = 0; j < kPerThread; ++j) {
+    const int d = threadIdx.x * kPerThread + j;
+    if (d < digits) {
+      uint32_t s = smaller + before_tile[j];
+#pragma unroll
+      for (int w = 0; w < kRadixWarps; ++w) { const uint32_t c = cnt[w][d]; cnt[w][d] = s; s += c; }
+    }
+    smaller += total[j];
   }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int64_t t = base + r * 32 + lane;
-    if (t < ids.T) {
+    if (base + r * 32 + lane < ids.T) {
       const uint32_t to = cnt[warp][(key[r] >> shift) & (digits - 1)] + place[r];
       keys_out[to] = key[r];
-      idx_out[to] = FIRST ? static_cast<uint32_t>(t) : idx[t];
+      idx_out[to] = val[r];
     }
   }
 }
@@ -287,9 +316,12 @@ embed_sum_kernel(const EmbedSumParams p) {
   }
 }
 
-// The run that starts in this chunk and continues in the next ones, if there is one.
+// The run that starts in this chunk and continues in the next ones, if there is one. Four groups of
+// threads add a quarter of its partial rows each, then the quarters are added in order.
+constexpr int kJoinGroups = 4;
+
 template <typename T, int E>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads * kJoinGroups)
 embed_join_kernel(const EmbedSumParams p) {
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.chunk;
   const int64_t end = begin + p.chunk;
@@ -303,21 +335,37 @@ embed_join_kernel(const EmbedSumParams p) {
     const int64_t mid = (lo + hi) >> 1;
     if (p.skey[mid] == k) lo = mid; else hi = mid;
   }
-  const int64_t last = lo / p.chunk;
-  const int c = (blockIdx.y * kSumThreads + threadIdx.x) * E;
-  if (c >= p.D) return;
+  const int64_t first = blockIdx.x + 1, n = lo / p.chunk - blockIdx.x;      // its other chunks
+  __shared__ float part[kJoinGroups][E][kSumThreads];
+  const int t = threadIdx.x % kSumThreads, g = threadIdx.x / kSumThreads;
+  const int c = (blockIdx.y * kSumThreads + t) * E;
   float acc[E];
-  const float* q = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.D + c;
 #pragma unroll
-  for (int j = 0; j < E; ++j) acc[j] = q[j];
-#pragma unroll 4
-  for (int64_t ch = blockIdx.x + 1; ch <= last; ++ch) {
-    const float* s = p.part + ch * 2 * p.D + c;
+  for (int j = 0; j < E; ++j) acc[j] = 0.f;
+  if (c < p.D) {
+    if (g == 0) {
+      const float* q = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.D + c;
 #pragma unroll
-    for (int j = 0; j < E; ++j) acc[j] += s[j];
+      for (int j = 0; j < E; ++j) acc[j] = q[j];
+    }
+    const int64_t c1 = first + n * (g + 1) / kJoinGroups;
+#pragma unroll 8
+    for (int64_t ch = first + n * g / kJoinGroups; ch < c1; ++ch) {
+      const float* s = p.part + ch * 2 * p.D + c;
+#pragma unroll
+      for (int j = 0; j < E; ++j) acc[j] += s[j];
+    }
   }
 #pragma unroll
-  for (int j = 0; j < E; ++j) acc[j] *= p.scale;
+  for (int j = 0; j < E; ++j) part[g][j][t] = acc[j];
+  __syncthreads();
+  if (g != 0 || c >= p.D) return;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+#pragma unroll
+    for (int i = 1; i < kJoinGroups; ++i) acc[j] += part[i][j][t];
+    acc[j] *= p.scale;
+  }
   store_e<T, E>(static_cast<T*>(p.out) + static_cast<int64_t>(k) * p.D + c, acc);
 }
 

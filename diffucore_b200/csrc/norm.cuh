@@ -2,10 +2,10 @@
 // the backward pass
 //   dx = rstd (a - mean(a) - xhat mean(a xhat)),  a = dy w,  xhat = (x - mean) rstd
 //   dw = sum_rows dy xhat,  db = sum_rows dy.
-// Bound by HBM: forward one read and one write of x, backward two reads and one write. A row is
-// held in the registers of one warp, or of a CTA of 128 or 512 threads, EPT values per thread, so
-// x is read once and the variance is the mean of squared deviations (two passes over registers,
-// no cancellation). Rows wider than 8192 values are read again from cache instead.
+// Bound by HBM: forward one read and one write of x, backward two reads and one write. Every value is
+// read once and held in registers while its row's sums are formed; the variance is the mean of
+// squared deviations from the mean (no cancellation). Only rows beyond the widest register layout
+// are read again from cache.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -81,6 +81,9 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* red, int& t
   return make_float2(a, b);
 }
 
+template <typename T, bool VEC> struct NormUnit { using type = T; };
+template <typename T> struct NormUnit<T, true> { using type = uint4; };
+
 struct NormParams {
   const void* x;
   int64_t ldx;
@@ -99,144 +102,275 @@ struct NormParams {
   int D;
   float eps;
   int w_f32;
+  int stages, slot;         // ring kernel: stages, bytes per row and tensor
 };
 
 template <int TPR> struct NormCta { static constexpr int kThreads = TPR == 32 ? 256 : TPR; };
 
-template <typename T, int E, int EPT, int TPR>
+// Forward, rows in registers: TPR threads per row, NU units each. A unit is 16 bytes (VEC) or one
+// value, kept packed until it is used, so a warp holds a row of 4096 16-bit values in 64 registers
+// per lane: 16 loads in flight per lane and no barrier at all.
+template <typename T, bool VEC, int NU, int TPR>
 __global__ void __launch_bounds__(NormCta<TPR>::kThreads)
 norm_fwd_kernel(const NormParams p) {
-  constexpr int NV = EPT / E;
+  constexpr int E = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
   constexpr int kRows = NormCta<TPR>::kThreads / TPR;
+  using Unit = typename NormUnit<T, VEC>::type;
   __shared__ float2 red[2 * (TPR / 32)];
   int turn = 0;
   const int t = threadIdx.x % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
   if (row >= p.M) return;                      // whole warps (TPR == 32) or the whole CTA
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-  float v[EPT];
+  Unit v[NU];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < NU; ++i) {
     const int c = (i * TPR + t) * E;
-    if (c < p.D) {
-      load_e<T, E>(x + c, v + i * E);
-    } else {
-#pragma unroll
-      for (int j = 0; j < E; ++j) v[i * E + j] = 0.f;
-    }
+    v[i] = Unit{};                             // zero bits: zeros in every type
+    if (c < p.D) v[i] = *reinterpret_cast<const Unit*>(x + c);
   }
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) s += v[i];
+  for (int i = 0; i < NU; ++i) {
+    const T* h = reinterpret_cast<const T*>(&v[i]);
+#pragma unroll
+    for (int j = 0; j < E; ++j) s += to_f(h[j]);
+  }
   const float inv = 1.0f / static_cast<float>(p.D);
   const float mean = row_sum2<TPR>(s, 0.f, red, turn).x * inv;
   s = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < NU; ++i) {
     if ((i * TPR + t) * E < p.D) {
+      const T* h = reinterpret_cast<const T*>(&v[i]);
 #pragma unroll
-      for (int j = 0; j < E; ++j) { const float d = v[i * E + j] - mean; s += d * d; }
+      for (int j = 0; j < E; ++j) { const float d = to_f(h[j]) - mean; s += d * d; }
     }
   }
-  const float var = row_sum2<TPR>(s, 0.f, red, turn).x * inv;
-  const float rstd = 1.0f / sqrtf(var + p.eps);
+  const float rstd = 1.0f / sqrtf(row_sum2<TPR>(s, 0.f, red, turn).x * inv + p.eps);
   if (t == 0 && p.mean != nullptr) { p.mean[row] = mean; p.rstd[row] = rstd; }
   T* y = static_cast<T*>(p.out) + row * p.ldo;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < NU; ++i) {
     const int c = (i * TPR + t) * E;
     if (c < p.D) {
+      const T* h = reinterpret_cast<const T*>(&v[i]);
       float w[E], b[E], o[E];
       if (p.w != nullptr) load_w<T, E>(p.w, c, p.w_f32, w);
       if (p.b != nullptr) load_w<T, E>(p.b, c, p.w_f32, b);
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float h = (v[i * E + j] - mean) * rstd;
-        o[j] = h * (p.w != nullptr ? w[j] : 1.0f) + (p.b != nullptr ? b[j] : 0.0f);
-      }
+      for (int j = 0; j < E; ++j)
+        o[j] = (to_f(h[j]) - mean) * rstd * (p.w != nullptr ? w[j] : 1.0f) + (p.b != nullptr ? b[j] : 0.0f);
       store_e<T, E>(y + c, o);
     }
   }
 }
 
-// Persistent: each CTA takes every gridDim.x-th row (group of rows), its threads keep the dw / db
-// sums of their own columns in registers and write one partial row at the end.
-template <typename T, int E, int EPT, int TPR>
-__global__ void __launch_bounds__(NormCta<TPR>::kThreads)
-norm_bwd_kernel(const NormParams p) {
+// Rows streamed through a ring of shared-memory stages by bulk copies: the backward pass, and the
+// forward pass of rows that no 16-byte access fits. Persistent CTAs of 256 threads (512 for rows
+// above 4096 values) take kRows rows at a time; each thread keeps its columns of w (and of the dw /
+// db sums) in registers for all its rows. The registers that those sums take leave too little room
+// to hide HBM's latency with loads in flight; the ring keeps several rows per CTA on their way
+// whatever the occupancy.
+//
+// A bulk copy starts and ends on 16-byte boundaries. Where rows do not, the copy takes the aligned
+// window around the row; the bytes before and after it belong to the neighbouring rows, and the
+// first and the last row, which lack one, are read in place instead.
+constexpr int kRingMax = 8;
+
+template <int TPR> struct RingCta { static constexpr int kThreads = TPR > 256 ? TPR : 256; };
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+template <typename T, int E, int TPR, bool BWD>
+__global__ void __launch_bounds__(RingCta<TPR>::kThreads, TPR > 256 ? 1 : 2)
+norm_ring_kernel(const NormParams p) {
+  constexpr int EPT = 16;
   constexpr int NV = EPT / E;
-  constexpr int kRows = NormCta<TPR>::kThreads / TPR;
-  __shared__ float2 red[2 * (TPR / 32)];
-  int turn = 0;
+  constexpr int kRows = RingCta<TPR>::kThreads / TPR;
+  constexpr int kTensors = BWD ? 2 : 1;
+  extern __shared__ __align__(16) uint8_t ring[];      // [stage][row][x, dy][slot]
+  __shared__ __align__(8) uint64_t full[kRingMax];
+  __shared__ float2 red[2 * (RingCta<TPR>::kThreads / 32)];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-  float w[EPT], dw[EPT], db[EPT];
+  const int64_t blocks = (p.M + kRows - 1) / kRows;
+  const uint8_t* src[2] = {static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.dy)};
+  const int64_t pitch[2] = {p.ldx * static_cast<int64_t>(sizeof(T)), p.lddy * static_cast<int64_t>(sizeof(T))};
+  const int row_bytes = p.D * static_cast<int>(sizeof(T));
+  const bool edges = E == 1;                            // rows 0 and M - 1 are read in place
+  auto slot = [&](int stage, int r, int which) { return ring + ((stage * kRows + r) * kTensors + which) * p.slot; };
+
+  // Thread 0: the copies of the rows of one block.
+  auto issue = [&](int stage, int64_t block) {
+    uint32_t total = 0;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int r = 0; r < kRows; ++r) {
+        const int64_t row = block * kRows + r;
+        if (row >= p.M || (edges && (row == 0 || row == p.M - 1))) continue;
+#pragma unroll
+        for (int k = 0; k < kTensors; ++k) {
+          const uintptr_t a = reinterpret_cast<uintptr_t>(src[k] + row * pitch[k]);
+          const uintptr_t lo = a & ~uintptr_t(15), hi = (a + row_bytes + 15) & ~uintptr_t(15);
+          if (pass == 0) total += static_cast<uint32_t>(hi - lo);
+          else bulk_load(slot(stage, r, k), reinterpret_cast<const void*>(lo), static_cast<uint32_t>(hi - lo), &full[stage]);
+        }
+      }
+      if (pass == 0) {
+        if (total > 0) mbar_arrive_expect_tx(&full[stage], total);
+        else mbar_arrive(&full[stage]);
+      }
+    }
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+    for (int s = 0; s < p.stages; ++s) {
+      const int64_t block = blockIdx.x + static_cast<int64_t>(s) * gridDim.x;
+      if (block < blocks) issue(s, block);
+    }
+  }
+  float w[EPT], sw[EPT], sb[EPT];                       // forward: sb is b
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + t) * E;
 #pragma unroll
-    for (int j = 0; j < E; ++j) { w[i * E + j] = c < p.D ? 1.0f : 0.f; dw[i * E + j] = 0.f; db[i * E + j] = 0.f; }
+    for (int j = 0; j < E; ++j) { w[i * E + j] = c < p.D ? 1.0f : 0.f; sw[i * E + j] = 0.f; sb[i * E + j] = 0.f; }
     if (c < p.D && p.w != nullptr) load_w<T, E>(p.w, c, p.w_f32, w + i * E);
+    if (!BWD && c < p.D && p.b != nullptr) load_w<T, E>(p.b, c, p.w_f32, sb + i * E);
   }
+  __syncthreads();
   const float inv = 1.0f / static_cast<float>(p.D);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub; row < p.M;
-       row += static_cast<int64_t>(gridDim.x) * kRows) {
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
-    const float mean = p.mean[row], rstd = p.rstd[row];
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  // Sums over a row's threads; every thread of the CTA takes part, and when it returns every thread
+  // has read its values of the stage.
+  auto row_sums = [&](float a, float b) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    float2* sl = red + turn * (RingCta<TPR>::kThreads / 32);
+    turn ^= 1;
+    if (TPR > 32 && (threadIdx.x & 31) == 0) sl[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    if (TPR > 32) {
+      a = 0.f; b = 0.f;
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) { const float2 f = sl[sub * (TPR / 32) + i]; a += f.x; b += f.y; }
+    }
+    return make_float2(a, b);
+  };
+
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const int64_t row = block * kRows + sub;
+    const bool live = row < p.M;
+    float mean = 0.f, rstd = 0.f;
+    if (BWD && live) { mean = p.mean[row]; rstd = p.rstd[row]; }
+    mbar_wait(&full[stage], phase, nullptr);
+    __syncwarp();
+    const T* px = nullptr;
+    const T* pd = nullptr;
+    if (live) {
+      const uint8_t* a[2];
+#pragma unroll
+      for (int k = 0; k < kTensors; ++k) {
+        const uint8_t* g = src[k] + row * pitch[k];
+        a[k] = edges && (row == 0 || row == p.M - 1) ? g : slot(stage, sub, k) + (reinterpret_cast<uintptr_t>(g) & 15);
+      }
+      px = reinterpret_cast<const T*>(a[0]);
+      if (BWD) pd = reinterpret_cast<const T*>(a[1]);
+    }
     float h[EPT], d[EPT];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * E;
-      if (c < p.D) {
-        load_e<T, E>(x + c, h + i * E);
-        load_e<T, E>(dy + c, d + i * E);
+      if (live && c < p.D) {
+        load_e<T, E>(px + c, h + i * E);
+        if (BWD) load_e<T, E>(pd + c, d + i * E);
       } else {
 #pragma unroll
         for (int j = 0; j < E; ++j) { h[i * E + j] = mean; d[i * E + j] = 0.f; }
       }
     }
-    float sa = 0.f, sh = 0.f;
+    float2 s;
+    if (BWD) {
+      float sa = 0.f, sh = 0.f;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      h[i] = (h[i] - mean) * rstd;
-      dw[i] += d[i] * h[i];
-      db[i] += d[i];
-      d[i] *= w[i];
-      sa += d[i];
-      sh += d[i] * h[i];
+      for (int i = 0; i < EPT; ++i) {
+        h[i] = (h[i] - mean) * rstd;
+        sw[i] += d[i] * h[i];
+        sb[i] += d[i];
+        d[i] = __fmul_rn(d[i], w[i]);       // the same value in the sum and in dx: a one-value row gives 0
+        sa += d[i];
+        sh += d[i] * h[i];
+      }
+      s = row_sums(sa, sh);
+    } else {
+      float sa = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) sa += h[i];          // 0 past the row
+      s = row_sums(sa, 0.f);
     }
-    const float2 s = row_sum2<TPR>(sa, sh, red, turn);
-    const float ma = s.x * inv, mh = s.y * inv;
-    T* dx = static_cast<T*>(p.out) + row * p.ldo;
+    if (threadIdx.x == 0) {
+      const int64_t next = block + static_cast<int64_t>(p.stages) * gridDim.x;
+      if (next < blocks) issue(stage, next);
+    }
+    if (++stage == p.stages) { stage = 0; phase ^= 1; }
+    if (!BWD) {
+      mean = s.x * inv;
+      float sq = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * E;
-      if (c < p.D) {
-        float o[E];
+      for (int i = 0; i < NV; ++i)
+        if ((i * TPR + t) * E < p.D) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] = rstd * (d[i * E + j] - ma - h[i * E + j] * mh);
-        store_e<T, E>(dx + c, o);
+          for (int j = 0; j < E; ++j) { h[i * E + j] -= mean; sq += h[i * E + j] * h[i * E + j]; }
+        }
+      rstd = 1.0f / sqrtf(row_sums(sq, 0.f).x * inv + p.eps);
+      if (live && t == 0 && p.mean != nullptr) { p.mean[row] = mean; p.rstd[row] = rstd; }
+    }
+    if (live) {
+      T* out = static_cast<T*>(p.out) + row * p.ldo;
+      const float ma = s.x * inv, mh = s.y * inv;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * E;
+        if (c < p.D) {
+          float o[E];
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const int k = i * E + j;
+            o[j] = BWD ? rstd * (d[k] - ma - h[k] * mh) : h[k] * rstd * w[k] + sb[k];
+          }
+          store_e<T, E>(out + c, o);
+        }
       }
     }
   }
-  if (p.part_w == nullptr) return;
-  if (TPR == 32) {
-    // The warps of the CTA hold sums of the same columns: added in warp order.
-    __shared__ float acc[TPR == 32 ? 2 * 32 * EPT : 1];
-    for (int s = 0; s < kRows; ++s) {
-      if (sub == s) {
+  if (!BWD || p.part_w == nullptr) return;
+  if (kRows > 1) {
+    // The CTA's row groups hold sums of the same columns: added in the order of the groups.
+    float* acc = reinterpret_cast<float*>(ring);         // no copy is under way any more
+    __syncthreads();
+    for (int g = 0; g < kRows; ++g) {
+      if (sub == g) {
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
-          const int k = i * 32 + t;
-          acc[k] = s == 0 ? dw[i] : acc[k] + dw[i];
-          acc[32 * EPT + k] = s == 0 ? db[i] : acc[32 * EPT + k] + db[i];
+          const int k = i * TPR + t;
+          acc[k] = g == 0 ? sw[i] : acc[k] + sw[i];
+          acc[TPR * EPT + k] = g == 0 ? sb[i] : acc[TPR * EPT + k] + sb[i];
         }
       }
       __syncthreads();
     }
     if (sub != 0) return;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) { dw[i] = acc[i * 32 + t]; db[i] = acc[32 * EPT + i * 32 + t]; }
+    for (int i = 0; i < EPT; ++i) { sw[i] = acc[i * TPR + t]; sb[i] = acc[TPR * EPT + i * TPR + t]; }
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -244,8 +378,8 @@ norm_bwd_kernel(const NormParams p) {
     if (c < p.D) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        p.part_w[blockIdx.x * p.ldp + c + j] = dw[i * E + j];
-        p.part_b[blockIdx.x * p.ldp + c + j] = db[i * E + j];
+        p.part_w[blockIdx.x * p.ldp + c + j] = sw[i * E + j];
+        p.part_b[blockIdx.x * p.ldp + c + j] = sb[i * E + j];
       }
     }
   }
@@ -292,7 +426,7 @@ norm_dx_wide_kernel(const NormParams p) {
   for (int c = threadIdx.x; c < p.D; c += kNormWide) {
     float w = 1.f;
     if (p.w != nullptr) load_w<T, 1>(p.w, c, p.w_f32, &w);
-    const float a = to_f(dy[c]) * w;
+    const float a = __fmul_rn(to_f(dy[c]), w);
     sa += a;
     sh += a * ((to_f(x[c]) - mean) * rstd);
   }
@@ -301,7 +435,7 @@ norm_dx_wide_kernel(const NormParams p) {
   for (int c = threadIdx.x; c < p.D; c += kNormWide) {
     float w = 1.f;
     if (p.w != nullptr) load_w<T, 1>(p.w, c, p.w_f32, &w);
-    const float a = to_f(dy[c]) * w;
+    const float a = __fmul_rn(to_f(dy[c]), w);
     dx[c] = from_f<T>(rstd * (a - s.x * inv - (to_f(x[c]) - mean) * rstd * (s.y * inv)));
   }
 }

@@ -9,6 +9,7 @@
 #include "host.cuh"
 #include "sm100.cuh"
 #include "hgemm.cuh"
+#include "rowdot.cuh"
 #include "textgrad.cuh"
 #include "norm.cuh"
 #include "embed.cuh"
@@ -76,19 +77,34 @@ int pair_override() {
   return env[0] - '0';
 }
 
+// Tile width of the pair kernel: the one with the fewest waves over the `pairs` CTA pairs times a
+// tile's cost. A tile is bound by what it reads from L2, 256 rows of A and bn rows of B per k
+// (measured: 512 x 20480 x 4096 in three waves, 72.0 us with 192 columns and 82.9 with 256).
+int choose_pair_bn(int64_t m_tiles, int64_t cols, int pairs) {
+  if (const char* env = getenv("DC_HGEMM_BN")) return atoi(env);
+  int best = 256;
+  int64_t best_cost = INT64_MAX;
+  for (int bn = 256; bn >= 128; bn -= 32) {
+    const int64_t cost = ceil_div(m_tiles * ceil_div(cols, bn), pairs) * (256 + bn);
+    if (cost < best_cost) { best = bn; best_cost = cost; }
+  }
+  return best;
+}
+
 // One contraction: A rows x B rows, over one or two segments of k (a0 . b0 + a1 . b1), or, with
 // `stacked`, two A operands of equal shape whose rows follow one another (their products go to
 // p.out and p.out1).
 template <bool AMN, bool BMN, int EPI>
 int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const Operand& b1, bool stacked,
                  dc::HGemmParams p, cudaStream_t st) {
-  const int n_out = EPI == dc::kEpiGated ? 2 * p.N : p.N;       // accumulator columns
   const int sms = sm_count();
-  const int64_t pair_tiles = ceil_div(p.M, 256) * (stacked ? 2 : 1) * ceil_div(n_out, dc::kPairBN);
+  const int64_t m_tiles = ceil_div(p.M, 256) * (stacked ? 2 : 1);
+  p.bn = choose_pair_bn(m_tiles, EPI == dc::kEpiGated ? 2 * static_cast<int64_t>(p.N) : p.N, sms / 2);
+  const int64_t pair_tiles = m_tiles * ceil_div(EPI == dc::kEpiGated ? 2 * static_cast<int64_t>(p.N) : p.N, p.bn);
   const int forced = pair_override();
   const bool pair = forced >= 0 ? forced == 1 : p.M > 256 && pair_tiles * 4 >= sms;
   const int tile_m = pair ? 256 : 128;
-  const int tile_n = (pair ? dc::kPairBN : dc::kClBN) / (EPI == dc::kEpiGated ? 2 : 1);
+  const int tile_n = (pair ? p.bn : dc::kClBN) / (EPI == dc::kEpiGated ? 2 : 1);
   const int bk = pair ? dc::kPairAtoms * dc::kHBK : dc::kHBK;
   const int half_m = static_cast<int>(ceil_div(p.M, tile_m));
   p.tiles_m = half_m * (stacked ? 2 : 1);
@@ -104,7 +120,7 @@ int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const 
   p.out_vec = aligned(p.out, 16) && (p.out1 == nullptr || aligned(p.out1, 16)) && p.ldo % 8 == 0;
   p.res_vec = p.residual != nullptr && aligned(p.residual, 16) && p.ldr % 8 == 0;
   const int box_a = pair ? 128 : p.a_rows;
-  const int box_b = EPI == dc::kEpiGated && !pair ? dc::kClBN / 2 : 128;
+  const int box_b = pair ? p.bn / 2 : EPI == dc::kEpiGated ? dc::kClBN / 2 : dc::kClBN;
   CUtensorMap ma0, ma1, mb0, mb1;
   int r;
   if ((r = operand_map(&ma0, a0, AMN, box_a))) return r;
@@ -136,6 +152,7 @@ int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const 
     if ((r = set_smem(kernel, dc::kClSmem))) return r;
     p.splits = 1;
     while (p.splits < 8 && 2 * p.splits * tiles <= 2 * sms && (p.kb0 + p.kb1) / (2 * p.splits) >= 4) p.splits *= 2;
+    if (const char* env = getenv("DC_HGEMM_SPLITS")) p.splits = atoi(env);
     attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
     cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits));
     cfg.dynamicSmemBytes = dc::kClSmem;
@@ -144,6 +161,56 @@ int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const 
   if (e != cudaSuccess) return cuda_fail(e, "projection launch");
   DC_CHECK_LAUNCH("projection launch");
   return DC_OK;
+}
+
+template <int NT, bool GATED, int AHEAD>
+void launch_rowdot_rows(const dc::RowDotParams& p, bool vec, bool bf16, unsigned ctas, unsigned threads, cudaStream_t st) {
+  const size_t smem = threads / 32 * 16 * 8 * NT * sizeof(float);     // at most 16 KB
+  if (vec) {
+    if (bf16) dc::rowdot_kernel<NT, GATED, true, true, AHEAD><<<ctas, threads, smem, st>>>(p);
+    else dc::rowdot_kernel<NT, GATED, true, false, AHEAD><<<ctas, threads, smem, st>>>(p);
+  } else {
+    if (bf16) dc::rowdot_kernel<NT, GATED, false, true, 4><<<ctas, threads, smem, st>>>(p);
+    else dc::rowdot_kernel<NT, GATED, false, false, 4><<<ctas, threads, smem, st>>>(p);
+  }
+}
+
+template <bool GATED>
+int launch_rowdot(dc::RowDotParams p, bool bf16, cudaStream_t st) {
+  const bool vec = aligned(p.x, 16) && aligned(p.w0, 16) && (p.N == 1 || p.ldw0 % 8 == 0) && (p.M == 1 || p.ldx % 8 == 0) &&
+                   (!GATED || (aligned(p.w1, 16) && (p.N == 1 || p.ldw1 % 8 == 0)));
+  // Eight warps divide the k of a column group, 16 where one group per SM is all there is, fewer for
+  // a short k. Measured, 8 rows: 4096 x 4096 14.2 / 11.6 / 12.4 us with 4 / 8 / 16 warps, gated
+  // 2 x 512 x 4096 12.4 / 8.3 / 7.8, 640 x 640 4.9 / 5.0 / 5.9.
+  const int64_t groups = ceil_div(p.N, GATED ? 8 : 16), steps = ceil_div(p.K, 32);
+  p.ks = groups <= 148 && steps >= 64 ? 16 : 8;
+  while (p.ks > 1 && steps < 2 * p.ks) p.ks /= 2;
+  const int warps = std::max(p.ks, dc::kRowDotWarps);
+  const unsigned ctas = static_cast<unsigned>(ceil_div(groups, warps / p.ks)), threads = 32 * warps;
+  // Up to two CTAs per SM there are registers for eight steps in flight instead of four: 10.2 us
+  // against 11.6 at 4096 x 4096; with more CTAs they cost occupancy (gated 2 x 10240 x 4096: 34.8
+  // against 29.9).
+  if (p.M > 8) launch_rowdot_rows<2, GATED, 4>(p, vec, bf16, ctas, threads, st);
+  else if (ctas <= 2 * 148) launch_rowdot_rows<1, GATED, 8>(p, vec, bf16, ctas, threads, st);
+  else launch_rowdot_rows<1, GATED, 4>(p, vec, bf16, ctas, threads, st);
+  DC_CHECK_LAUNCH("projection launch");
+  return DC_OK;
+}
+
+// Operands of the few-row path: any rows with element alignment.
+int check_few_rows(const char* what, const char* name, const void* p, int64_t ld, int64_t cols) {
+  if (p == nullptr) return fail("%s: %s is null", what, name);
+  if (!aligned(p, 2)) return fail("%s: %s must be aligned to its element size", what, name);
+  if (ld < cols) return fail("%s: leading dimension of %s smaller than its row", what, name);
+  return DC_OK;
+}
+
+// Which projections take the few-row kernel (DC_HGEMM_PAIR picks among the tiled kernels only).
+// Up to 8 rows it reads x once per step and weights always dominate: 4096 x 4096 11.6 us against 14.4
+// for the cluster kernel, gated 2 x 10240 x 4096 29.9 against 38.8. At 9 to 16 rows the second
+// block of x costs as many L1 accesses as the weights: 12.4 against 14.4, but 45 against 40 us.
+bool few_rows(int64_t M, int64_t weights) {
+  return (M <= 8 || (M <= dc::kRowDotMax && weights <= (32 << 20))) && pair_override() < 0;
 }
 
 int check_z(const char* what, const float* z, int64_t ldz, int64_t N) {
@@ -163,11 +230,23 @@ int dc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void
   int r;
   if ((r = check_dims("linear", dtype, M, N, K)) || (r = check_act("linear", act))) return r;
   if (M == 0) return DC_OK;
-  if ((r = check_operand("linear", "x", x, ldx, K)) || (r = check_operand("linear", "w", w, ldw, K))) return r;
+  const bool few = few_rows(M, N * K);
+  const auto check = few ? check_few_rows : check_operand;
+  if ((r = check("linear", "x", x, ldx, K)) || (r = check("linear", "w", w, ldw, K))) return r;
   if (y == nullptr) return fail("linear: y is null");
   if (!aligned(y, 2) || !aligned(bias, 2) || !aligned(residual, 2)) return fail("linear: pointers must be aligned to their element size");
   if (ldy < N || (residual != nullptr && ldr < 0)) return fail("linear: leading dimension smaller than the row");
   if ((r = check_z("linear", z, ldz, N)) || (r = check_sm100())) return r;
+  if (few) {
+    dc::RowDotParams d = {};
+    d.x = static_cast<const uint16_t*>(x); d.ldx = ldx;
+    d.w0 = static_cast<const uint16_t*>(w); d.ldw0 = ldw;
+    d.bias0 = static_cast<const uint16_t*>(bias);
+    d.residual = static_cast<const uint16_t*>(residual); d.ldr = ldr;
+    d.out = static_cast<uint16_t*>(y); d.ldo = ldy; d.z0 = z; d.ldz = ldz;
+    d.M = static_cast<int>(M); d.N = static_cast<int>(N); d.K = static_cast<int>(K); d.act = act;
+    return launch_rowdot<false>(d, dtype == DC_DTYPE_BF16, as_stream(stream));
+  }
   dc::HGemmParams p = {};
   p.M = static_cast<int>(M); p.N = static_cast<int>(N);
   p.out = y; p.ldo = ldy; p.bias = bias; p.residual = residual; p.ldr = ldr;
@@ -181,14 +260,26 @@ int dc_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg
   int r;
   if ((r = check_dims("gated_linear", dtype, M, N, K)) || (r = check_act("gated_linear", act))) return r;
   if (M == 0) return DC_OK;
-  if ((r = check_operand("gated_linear", "x", x, ldx, K)) || (r = check_operand("gated_linear", "w_gate", w_gate, ldwg, K)) ||
-      (r = check_operand("gated_linear", "w_up", w_up, ldwu, K)))
+  const bool few = few_rows(M, 2 * N * K);
+  const auto check = few ? check_few_rows : check_operand;
+  if ((r = check("gated_linear", "x", x, ldx, K)) || (r = check("gated_linear", "w_gate", w_gate, ldwg, K)) ||
+      (r = check("gated_linear", "w_up", w_up, ldwu, K)))
     return r;
   if (h == nullptr) return fail("gated_linear: h is null");
   if (!aligned(h, 2) || !aligned(b_gate, 2) || !aligned(b_up, 2)) return fail("gated_linear: pointers must be aligned to their element size");
   if (ldh < N) return fail("gated_linear: leading dimension smaller than the row");
   if ((z_gate == nullptr) != (z_up == nullptr)) return fail("gated_linear: z_gate and z_up go together");
   if ((r = check_z("gated_linear", z_gate, ldz, N)) || (r = check_z("gated_linear", z_up, ldz, N)) || (r = check_sm100())) return r;
+  if (few) {
+    dc::RowDotParams d = {};
+    d.x = static_cast<const uint16_t*>(x); d.ldx = ldx;
+    d.w0 = static_cast<const uint16_t*>(w_gate); d.ldw0 = ldwg;
+    d.w1 = static_cast<const uint16_t*>(w_up); d.ldw1 = ldwu;
+    d.bias0 = static_cast<const uint16_t*>(b_gate); d.bias1 = static_cast<const uint16_t*>(b_up);
+    d.out = static_cast<uint16_t*>(h); d.ldo = ldh; d.z0 = z_gate; d.z1 = z_up; d.ldz = ldz;
+    d.M = static_cast<int>(M); d.N = static_cast<int>(N); d.K = static_cast<int>(K); d.act = act;
+    return launch_rowdot<true>(d, dtype == DC_DTYPE_BF16, as_stream(stream));
+  }
   dc::HGemmParams p = {};
   p.M = static_cast<int>(M); p.N = static_cast<int>(N);
   p.out = h; p.ldo = ldh; p.bias = b_gate; p.bias1 = b_up;
@@ -310,55 +401,102 @@ int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, i
 
 namespace {
 
-constexpr int64_t kNormReg = 8192;             // widest row held in registers
+constexpr int64_t kNormRing = 8192;            // widest row of the ring kernel
 
 int64_t norm_wide_blocks(int64_t M, int64_t D) {
   return std::max<int64_t>(1, std::min<int64_t>({ceil_div(148 * 8, ceil_div(D, 256)), ceil_div(M, 16), 65535}));
 }
-// CTAs of the persistent backward kernel.
+int ring_threads_per_row(int64_t D) { return D <= 512 ? 32 : D <= 2048 ? 128 : D <= 4096 ? 256 : 512; }
+// CTAs of the backward pass: persistent ring CTAs, two per SM (one of 512 threads).
 int64_t norm_bwd_ctas(int64_t M, int64_t D) {
-  if (D > kNormReg) return norm_wide_blocks(M, D);
-  const int64_t rows = D <= 512 ? 8 : 1, per_sm = D <= 512 ? 4 : D <= 2048 ? 6 : 2;
-  return std::min<int64_t>(ceil_div(M, rows), 148 * per_sm);
+  if (D > kNormRing) return norm_wide_blocks(M, D);
+  const int tpr = ring_threads_per_row(D);
+  return std::min<int64_t>(ceil_div(M, std::max(256, tpr) / tpr), tpr > 256 ? 148 : 2 * 148);
+}
+
+template <typename T, int E, int TPR, bool BWD>
+int launch_ring(dc::NormParams p, int64_t ctas, cudaStream_t st) {
+  constexpr int kThreads = dc::RingCta<TPR>::kThreads, kRows = kThreads / TPR;
+  // A slot holds a row's aligned window. Stages: up to 96 KB of rows per CTA (two fit an SM).
+  p.slot = static_cast<int>(round_up(p.D * static_cast<int64_t>(sizeof(T)), 16)) + (E == 1 ? 16 : 0);
+  const int stage = kRows * (BWD ? 2 : 1) * p.slot;
+  p.stages = std::max(2, std::min(dc::kRingMax, (96 << 10) / stage));
+  const int sums = kRows > 1 ? 2 * TPR * 16 * static_cast<int>(sizeof(float)) : 0;
+  const int smem = std::max(p.stages * stage, sums);
+  auto kernel = dc::norm_ring_kernel<T, E, TPR, BWD>;
+  if (int r = set_smem(kernel, smem)) return r;
+  kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(p);
+  DC_CHECK_LAUNCH("layer_norm launch");
+  return DC_OK;
 }
 
 template <typename T, int E, bool BWD>
-int launch_norm_reg(const dc::NormParams& p, int64_t ctas, cudaStream_t st) {
-  auto go = [&](auto tpr, auto ept) {
-    constexpr int TPR = decltype(tpr)::value, EPT = decltype(ept)::value;
-    if constexpr (BWD)
-      dc::norm_bwd_kernel<T, E, EPT, TPR><<<static_cast<unsigned>(ctas), dc::NormCta<TPR>::kThreads, 0, st>>>(p);
-    else
-      dc::norm_fwd_kernel<T, E, EPT, TPR><<<static_cast<unsigned>(ctas), dc::NormCta<TPR>::kThreads, 0, st>>>(p);
+int launch_ring_rows(const dc::NormParams& p, cudaStream_t st) {
+  const int64_t ctas = norm_bwd_ctas(p.M, p.D);
+  switch (ring_threads_per_row(p.D)) {
+    case 32: return launch_ring<T, E, 32, BWD>(p, ctas, st);
+    case 128: return launch_ring<T, E, 128, BWD>(p, ctas, st);
+    case 256: return launch_ring<T, E, 256, BWD>(p, ctas, st);
+    default: return launch_ring<T, E, 512, BWD>(p, ctas, st);
+  }
+}
+
+// The forward register kernel: with many rows a warp per row as long as it holds the row (no
+// barriers), with few rows more threads per row (latency). False: the row is too wide.
+template <typename T, bool VEC>
+bool launch_norm_reg(const dc::NormParams& p, cudaStream_t st) {
+  constexpr int E = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  const bool many = p.M >= 148 * 16;
+  const int64_t units = ceil_div(p.D, E);
+  const int most = VEC ? (many ? 16 : 2) : (many ? 32 : 8), top = VEC ? 16 : 32;
+  const int tpr = units <= 32 * most ? 32 : units <= 128 * most ? 128 : 512;
+  const int nu = static_cast<int>(ceil_div(units, tpr));
+  if (nu > top) return false;
+  const unsigned ctas = static_cast<unsigned>(ceil_div(p.M, tpr == 32 ? 8 : 1));
+  auto go = [&](auto t, auto n) {
+    constexpr int TPR = decltype(t)::value, NU = decltype(n)::value;
+    dc::norm_fwd_kernel<T, VEC, NU, TPR><<<ctas, dc::NormCta<TPR>::kThreads, 0, st>>>(p);
   };
-  using std::integral_constant;
-  if (p.D <= 256) go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-  else if (p.D <= 512) go(integral_constant<int, 32>{}, integral_constant<int, 16>{});
-  else if (p.D <= 1024) go(integral_constant<int, 128>{}, integral_constant<int, 8>{});
-  else if (p.D <= 2048) go(integral_constant<int, 128>{}, integral_constant<int, 16>{});
-  else if (p.D <= 4096) go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
-  else go(integral_constant<int, 512>{}, integral_constant<int, 16>{});
-  DC_CHECK_LAUNCH("layer_norm launch");
-  return DC_OK;
+  auto units_per_thread = [&](auto t) {
+    using std::integral_constant;
+    if constexpr (VEC) {
+      if (nu <= 1) go(t, integral_constant<int, 1>{});
+      else if (nu <= 2) go(t, integral_constant<int, 2>{});
+      else if (nu <= 4) go(t, integral_constant<int, 4>{});
+      else if (nu <= 8) go(t, integral_constant<int, 8>{});
+      else go(t, integral_constant<int, 16>{});
+    } else {
+      if (nu <= 8) go(t, integral_constant<int, 8>{});
+      else go(t, integral_constant<int, 32>{});
+    }
+  };
+  if (tpr == 32) units_per_thread(std::integral_constant<int, 32>{});
+  else if (tpr == 128) units_per_thread(std::integral_constant<int, 128>{});
+  else units_per_thread(std::integral_constant<int, 512>{});
+  return true;
 }
 
 template <typename T, bool BWD>
 int launch_norm(const dc::NormParams& p, bool vec, cudaStream_t st) {
   constexpr int E = 16 / sizeof(T);
-  if (p.D <= kNormReg) {
-    const int64_t ctas = BWD ? norm_bwd_ctas(p.M, p.D) : ceil_div(p.M, p.D <= 512 ? 8 : 1);
-    return vec ? launch_norm_reg<T, E, BWD>(p, ctas, st) : launch_norm_reg<T, 1, BWD>(p, ctas, st);
-  }
   if constexpr (BWD) {
+    // The window of an unaligned row must lie inside its neighbours.
+    const bool apart = p.ldx >= p.D && p.lddy >= p.D && p.D * sizeof(T) >= 16;
+    if (p.D <= kNormRing && (vec || apart)) return vec ? launch_ring_rows<T, E, true>(p, st) : launch_ring_rows<T, 1, true>(p, st);
     dc::norm_dx_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
     DC_CHECK_LAUNCH("layer_norm_grad launch");
     if (p.part_w != nullptr) {
-      const int64_t blocks = norm_wide_blocks(p.M, p.D);
+      const int64_t blocks = norm_bwd_ctas(p.M, p.D);
       dc::norm_dw_wide_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(p.D, 256)), static_cast<unsigned>(blocks)), 256, 0, st>>>(
           p, static_cast<int>(ceil_div(p.M, blocks)));
     }
   } else {
-    dc::norm_fwd_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
+    const bool apart = p.ldx >= p.D && p.D * sizeof(T) >= 16;
+    const bool many = p.D <= kNormRing && p.M >= 148 * 8;
+    if (many && vec && getenv("DC_NORM_RING")) return launch_ring_rows<T, E, false>(p, st);
+    if (many && !vec && apart) return launch_ring_rows<T, 1, false>(p, st);
+    if (!(vec ? launch_norm_reg<T, true>(p, st) : launch_norm_reg<T, false>(p, st)))
+      dc::norm_fwd_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
   }
   DC_CHECK_LAUNCH("layer_norm launch");
   return DC_OK;
@@ -488,7 +626,7 @@ EmbedPlan embed_plan(int64_t T, int64_t V, int64_t D) {
   e.tiles = e.rank ? 0 : ceil_div(T, dc::kRadixTile);
   const int64_t slabs = ceil_div(D, 8 * dc::kSumThreads);
   e.chunk = 8;
-  while (e.chunk < dc::kSumChunkMax && ceil_div(T, 2 * e.chunk) * slabs >= 4 * 148) e.chunk *= 2;
+  while (e.chunk < dc::kSumChunkMax && ceil_div(T, 2 * e.chunk) * slabs >= 16 * 148) e.chunk *= 2;
   e.chunks = ceil_div(T, e.chunk);
   size_t at = 0;
   auto take = [&](size_t n) { const size_t a = at; at += (n + 255) / 256 * 256; return a; };
@@ -505,7 +643,7 @@ int launch_embed_sum(const dc::EmbedSumParams& p, int64_t chunks, cudaStream_t s
   if (grid.y > 65535) return fail("embedding_grad: rows of %d values are too wide", p.D);
   dc::embed_sum_kernel<T, E><<<grid, dc::kSumThreads, 0, st>>>(p);
   DC_CHECK_LAUNCH("embedding_grad sum launch");
-  dc::embed_join_kernel<T, E><<<grid, dc::kSumThreads, 0, st>>>(p);
+  dc::embed_join_kernel<T, E><<<grid, dc::kSumThreads * dc::kJoinGroups, 0, st>>>(p);
   DC_CHECK_LAUNCH("embedding_grad join launch");
   return DC_OK;
 }
@@ -562,33 +700,52 @@ int dc_embedding_grad(const void* dy, int64_t lddy, const void* ids, int ids_i64
     return fail("embedding_grad: workspace below %zu bytes or misaligned", plan.total);
   if ((r = check_sm100())) return r;
   const cudaStream_t st = as_stream(stream);
-  cudaError_t ce = cudaMemsetAsync(dtable, 0, static_cast<size_t>(V) * D * es, st);
-  if (ce != cudaSuccess) return cuda_fail(ce, "embedding_grad zero fill");
+  uint8_t* const table = static_cast<uint8_t*>(dtable);
+  const int64_t table_bytes = V * D * static_cast<int64_t>(es);
+  // Up to the first 16-byte boundary of an unaligned table, or all of it when there are no tokens.
+  const int64_t head = T == 0 ? table_bytes : std::min<int64_t>(table_bytes, (16 - reinterpret_cast<uintptr_t>(table) % 16) % 16);
+  if (head > 0) {
+    cudaError_t ce = cudaMemsetAsync(table, 0, static_cast<size_t>(head), st);
+    if (ce != cudaSuccess) return cuda_fail(ce, "embedding_grad zero fill");
+  }
   if (T == 0) return DC_OK;
 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   auto u32 = [&](size_t off) { return reinterpret_cast<uint32_t*>(ws + off); };
   const dc::EmbedIds e = {ids, ids_i64 != 0, T, V, padding_idx};
+  // Slice `i` of the launches that share the zero fill.
+  const int launches = plan.rank ? 1 : 2 * plan.passes;
+  const int64_t slice_bytes = round_up(ceil_div(table_bytes - head, launches), 16);
+  auto slice = [&](int i) {
+    const int64_t lo = std::min(table_bytes, head + i * slice_bytes), hi = std::min(table_bytes, lo + slice_bytes);
+    dc::FillSlice f = {table + lo, hi - lo, 0};
+    f.ctas = static_cast<int>(std::min<int64_t>(4 * 148, ceil_div(hi - lo, dc::kFillCta)));
+    return f;
+  };
   int cur = 0;
   if (plan.rank) {
-    dc::embed_rank_kernel<<<static_cast<unsigned>(ceil_div(T, dc::kRankItems)), 32 * dc::kRankWarps, 0, st>>>(
-        e, u32(plan.keys[0]), u32(plan.idx[0]));
+    const dc::FillSlice fill = slice(0);
+    const int ctas = static_cast<int>(ceil_div(T, dc::kRankItems));
+    dc::embed_rank_kernel<<<ctas + fill.ctas, 32 * dc::kRankWarps, 0, st>>>(e, u32(plan.keys[0]), u32(plan.idx[0]), ctas, fill);
     DC_CHECK_LAUNCH("embedding_grad sort launch");
   } else {
-    const unsigned tiles = static_cast<unsigned>(plan.tiles);
+    const int tiles = static_cast<int>(plan.tiles);
     const unsigned threads = 32 * dc::kRadixWarps;
     for (int pass = 0; pass < plan.passes; ++pass) {
       const int shift = pass * plan.bits, out = pass & 1, in = out ^ 1;
       uint32_t* hist = u32(plan.hist);
-      if (pass == 0) dc::radix_hist_kernel<true><<<tiles, threads, 0, st>>>(e, nullptr, hist, shift, plan.bits);
-      else dc::radix_hist_kernel<false><<<tiles, threads, 0, st>>>(e, u32(plan.keys[in]), hist, shift, plan.bits);
-      dc::radix_scan_kernel<<<1, 1024, 0, st>>>(hist, plan.tiles << plan.bits);
-      if (pass == 0)
-        dc::radix_scatter_kernel<true><<<tiles, threads, 0, st>>>(e, nullptr, nullptr, hist, u32(plan.keys[out]),
-                                                                  u32(plan.idx[out]), shift, plan.bits);
-      else
-        dc::radix_scatter_kernel<false><<<tiles, threads, 0, st>>>(e, u32(plan.keys[in]), u32(plan.idx[in]), hist,
-                                                                   u32(plan.keys[out]), u32(plan.idx[out]), shift, plan.bits);
+      const dc::FillSlice f0 = slice(2 * pass), f1 = slice(2 * pass + 1);
+      const unsigned g0 = tiles + f0.ctas, g1 = tiles + f1.ctas;
+      if (pass == 0) {
+        dc::radix_hist_kernel<true><<<g0, threads, 0, st>>>(e, nullptr, hist, shift, plan.bits, tiles, f0);
+        dc::radix_scatter_kernel<true><<<g1, threads, 0, st>>>(e, nullptr, nullptr, hist, u32(plan.keys[out]),
+                                                               u32(plan.idx[out]), shift, plan.bits, tiles, f1);
+      } else {
+        dc::radix_hist_kernel<false><<<g0, threads, 0, st>>>(e, u32(plan.keys[in]), hist, shift, plan.bits, tiles, f0);
+        dc::radix_scatter_kernel<false><<<g1, threads, 0, st>>>(e, u32(plan.keys[in]), u32(plan.idx[in]), hist,
+                                                                u32(plan.keys[out]), u32(plan.idx[out]), shift, plan.bits,
+                                                                tiles, f1);
+      }
       DC_CHECK_LAUNCH("embedding_grad sort launch");
       cur = out;
     }

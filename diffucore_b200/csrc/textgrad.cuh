@@ -40,37 +40,49 @@ act_grad_kernel(const ActGradParams p) {
   const int64_t r0 = static_cast<int64_t>(blockIdx.y) * p.rows_per_block;
   const int64_t r1 = min(p.M, r0 + p.rows_per_block);
   float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int64_t r = r0; r < r1; ++r) {
-    const float4 d4 = load4(p.dy + r * p.lddy + col, n, p.dy_vec, p.bf16);
-    float d[4] = {d4.x, d4.y, d4.z, d4.w};
-    if (p.z0 != nullptr) {
-      const float4 z4 = *reinterpret_cast<const float4*>(p.z0 + r * p.ldz + col);
-      const float z[4] = {z4.x, z4.y, z4.z, z4.w};
-      float e[4];
-      if (GATED) {
-        const float4 u4 = *reinterpret_cast<const float4*>(p.z1 + r * p.ldz + col);
-        const float u[4] = {u4.x, u4.y, u4.z, u4.w};
+  constexpr int kAhead = 4;                 // rows whose loads are in flight at once
+  for (int64_t rb = r0; rb < r1; rb += kAhead) {
+    float4 d4[kAhead], z4[kAhead], u4[kAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 a = act_value_grad(z[j], p.act);
-          e[j] = d[j] * a.x;
-          d[j] *= u[j] * a.y;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] *= act_value_grad(z[j], p.act).y;
-      }
-      // rows of dz are padded to 8 values, so a whole unit may be written
-      *reinterpret_cast<uint2*>(p.dz0 + r * p.lddz + col) = make_uint2(pack_h2(d[0], d[1], p.bf16), pack_h2(d[2], d[3], p.bf16));
-      if (GATED) {
-        *reinterpret_cast<uint2*>(p.dz1 + r * p.lddz + col) = make_uint2(pack_h2(e[0], e[1], p.bf16), pack_h2(e[2], e[3], p.bf16));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s1[j] += e[j];
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t r = rb + k;
+      if (r < r1) {
+        d4[k] = load4(p.dy + r * p.lddy + col, n, p.dy_vec, p.bf16);
+        if (p.z0 != nullptr) z4[k] = *reinterpret_cast<const float4*>(p.z0 + r * p.ldz + col);
+        if (GATED) u4[k] = *reinterpret_cast<const float4*>(p.z1 + r * p.ldz + col);
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s0[j] += d[j];
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t r = rb + k;
+      if (r >= r1) break;
+      float d[4] = {d4[k].x, d4[k].y, d4[k].z, d4[k].w};
+      if (p.z0 != nullptr) {
+        const float z[4] = {z4[k].x, z4[k].y, z4[k].z, z4[k].w};
+        float e[4];
+        if (GATED) {
+          const float u[4] = {u4[k].x, u4[k].y, u4[k].z, u4[k].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 a = act_value_grad(z[j], p.act);
+            e[j] = d[j] * a.x;
+            d[j] *= u[j] * a.y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[j] *= act_value_grad(z[j], p.act).y;
+        }
+        // rows of dz are padded to 8 values, so a whole unit may be written
+        *reinterpret_cast<uint2*>(p.dz0 + r * p.lddz + col) = make_uint2(pack_h2(d[0], d[1], p.bf16), pack_h2(d[2], d[3], p.bf16));
+        if (GATED) {
+          *reinterpret_cast<uint2*>(p.dz1 + r * p.lddz + col) = make_uint2(pack_h2(e[0], e[1], p.bf16), pack_h2(e[2], e[3], p.bf16));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s1[j] += e[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s0[j] += d[j];
+    }
   }
   if (p.part0 != nullptr) {
     *reinterpret_cast<float4*>(p.part0 + blockIdx.y * p.ldp + col) = make_float4(s0[0], s0[1], s0[2], s0[3]);

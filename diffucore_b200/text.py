@@ -26,11 +26,15 @@ from . import kernels
 
 
 def _flat(t: torch.Tensor | None, width: int) -> torch.Tensor | None:
-    return None if t is None else t.reshape(math.prod(t.shape[:-1]), width)
+    return t if t is None or t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), width)
 
 
 def _wants_grad(*ts: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _check_width(what: str, x: torch.Tensor, width: int) -> None:
@@ -204,7 +208,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0,
         if not -V <= padding_idx < V:
             raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {V} rows")
         padding_idx %= V
-    flat = ids.reshape(-1)
+    flat = ids if ids.dim() == 1 else ids.reshape(-1)
     if _wants_grad(table):
         y = _Embedding.apply(flat, table, scale, -1 if padding_idx is None else padding_idx)
     else:

@@ -257,7 +257,8 @@ int dc_selftest_wait_timeout(long long limit_cycles, int* status_dev, void* stre
  * (one type per call); every sum is fp32 in a fixed order, results are rounded once.
  *
  * Matrix operands (x, w, dz) are row-major with a 16-byte aligned base and a leading dimension
- * that is a multiple of 8 elements; outputs, biases and residuals need element alignment only.
+ * that is a multiple of 8 elements; outputs, biases and residuals need element alignment only. For up
+ * to 8 rows (M <= 8) x and w of the forward calls need element alignment only, too.
  * --------------------------------------------------------------------------------------------- */
 
 #define DC_ACT_NONE 0

@@ -24,7 +24,7 @@ def refused(status: int, why: bytes) -> None:
 def test_projection_arguments():
     lib = _lib.load()
 
-    def linear(x=A, ldx=64, w=A, ldw=64, bias=None, res=None, ldr=0, y=A, ldy=32, z=None, ldz=0, dtype=BF16, M=4,
+    def linear(x=A, ldx=64, w=A, ldw=64, bias=None, res=None, ldr=0, y=A, ldy=32, z=None, ldz=0, dtype=BF16, M=40,
                N=32, K=64, act=0):
         return lib.dc_linear(x, ldx, w, ldw, bias, res, ldr, y, ldy, z, ldz, dtype, M, N, K, act, None)
 
@@ -42,6 +42,8 @@ def test_projection_arguments():
     refused(linear(z=A, ldz=30), b"pre-activations")
     refused(linear(z=A + 4, ldz=32), b"pre-activations")
     assert linear(M=0, x=None) == 0
+    refused(linear(M=4, x=A + 1), b"aligned")               # few rows: element alignment only
+    refused(linear(M=4, ldw=63), b"smaller than its row")
     refused(linear(), b"")                                  # no device here
     refused(lib.dc_gated_linear(A, 64, A, 64, A, 64, None, None, A, 32, A, None, 32, BF16, 4, 32, 64, 2, None),
             b"go together")
