@@ -9,10 +9,9 @@
 //   sort    up to 8192 tokens: each token's place is the number of smaller (id, t) keys, counted
 //           against all keys in shared memory, one launch; more: least-significant-digit radix
 //           passes of up to 9 bits (histogram per tile, stable scatter)
-//   sum     a CTA per chunk of sorted places and slab of columns adds up runs of equal ids; runs
-//           inside the chunk go to the table, the first and last may continue in the
-//           neighbouring chunks and leave fp32 partials
-//   join    the chunk in which such a run starts adds its partials in order
+//   sum     a CTA per chunk of sorted places and slab of columns adds up the runs of equal ids that
+//           start in its chunk; a run that covers a whole chunk leaves fp32 partials per chunk
+//   join    adds the partials of those runs in order
 // Chunks of equal length keep a frequent token from falling to one CTA.
 #pragma once
 #include <cuda_bf16.h>
@@ -245,8 +244,11 @@ radix_scatter_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, cons
 
 // ------------------------------------------------------------------ sums over sorted tokens
 
+// A run of equal keys that covers no whole chunk is summed by the CTA of the chunk it starts in, at
+// most one chunk past its end. A longer run leaves one partial row per chunk (its first chunk in slot
+// 1, the others in slot 0) for the join.
 constexpr int kSumThreads = 128;
-constexpr int kSumChunkMax = 128;
+constexpr int kSumChunkMax = 64;
 
 struct EmbedSumParams {
   const uint32_t* skey;
@@ -265,40 +267,52 @@ struct EmbedSumParams {
 template <typename T, int E>
 __global__ void __launch_bounds__(kSumThreads)
 embed_sum_kernel(const EmbedSumParams p) {
-  __shared__ uint32_t key[kSumChunkMax + 2];
-  __shared__ uint32_t idx[kSumChunkMax];
+  constexpr uint32_t kNone = 0xFFFFFFFFu;       // never a key
+  __shared__ uint32_t key[2 * kSumChunkMax + 2];
+  __shared__ uint32_t idx[2 * kSumChunkMax];
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.chunk;
-  const int n = static_cast<int>(min(static_cast<int64_t>(p.chunk), p.T - begin));
-  const uint32_t none = 0xFFFFFFFFu;      // never a key
-  for (int i = threadIdx.x; i < n + 2; i += kSumThreads) {
+  const int chunk = p.chunk;
+  // places of this chunk and the next one, and one on either side
+  for (int i = threadIdx.x; i < 2 * chunk + 2; i += kSumThreads) {
     const int64_t t = begin + i - 1;
-    key[i] = t >= 0 && t < p.T ? p.skey[t] : none;
-    if (i < n) idx[i] = p.sidx[begin + i];
+    key[i] = t >= 0 && t < p.T ? p.skey[t] : kNone;
+    if (i < 2 * chunk && begin + i < p.T) idx[i] = p.sidx[begin + i];
   }
+  const uint32_t before_chunk = begin - chunk - 1 >= 0 ? p.skey[begin - chunk - 1] : kNone;
   __syncthreads();
+  const int n = static_cast<int>(min(static_cast<int64_t>(chunk), p.T - begin));
+  const uint32_t first = key[1], last = key[n];
+  const int i_own = static_cast<int>(threadIdx.x);
+  const int lead = __syncthreads_count(i_own < n && key[i_own + 1] == first);
+  const int tail = __syncthreads_count(i_own < chunk && n == chunk && key[n + i_own + 1] == last);
+  // A leading run that began in the previous chunk and covers neither chunk belongs to that one.
+  const int s0 = key[0] == first && before_chunk != first && key[chunk + 1] != first ? lead : 0;
+  // The last run goes on into the next chunk: to its end, unless it covers that chunk (or this one).
+  const int e0 = n == chunk && s0 < n && key[2 * chunk + 1] != last && !(first == last && key[0] == last) ? n + tail : n;
   const int c = (blockIdx.y * kSumThreads + threadIdx.x) * E;
-  if (c >= p.D || key[1] == static_cast<uint32_t>(p.V)) return;
+  if (c >= p.D || s0 >= e0) return;
   const T* dy = static_cast<const T*>(p.dy) + c;
   float acc[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) acc[j] = 0.f;
-  bool from_before = key[0] == key[1];
+  bool from_before = s0 == 0 && key[0] == key[1];
   constexpr int kAhead = 8;
-  for (int i0 = 0; i0 < n; i0 += kAhead) {
+  for (int i0 = s0; i0 < e0; i0 += kAhead) {
+    if (key[i0 + 1] == static_cast<uint32_t>(p.V)) return;         // sorted last: nothing follows
     float v[kAhead][E];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (i0 + u < n) load_e<T, E>(dy + static_cast<int64_t>(idx[i0 + u]) * p.lddy, v[u]);
+      if (i0 + u < e0) load_e<T, E>(dy + static_cast<int64_t>(idx[i0 + u]) * p.lddy, v[u]);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u;
-      if (i >= n) break;
+      if (i >= e0) break;
       const uint32_t k = key[i + 1];
       if (k == static_cast<uint32_t>(p.V)) return;
 #pragma unroll
       for (int j = 0; j < E; ++j) acc[j] += v[u][j];
       const bool ends = key[i + 2] != k;
-      if (ends || i == n - 1) {
+      if (ends || i == e0 - 1) {
         if (ends && !from_before) {
 #pragma unroll
           for (int j = 0; j < E; ++j) acc[j] *= p.scale;
@@ -316,57 +330,80 @@ embed_sum_kernel(const EmbedSumParams p) {
   }
 }
 
-// The run that starts in this chunk and continues in the next ones, if there is one. Four groups of
-// threads add a quarter of its partial rows each, then the quarters are added in order.
+// Runs that cover a whole chunk. A CTA looks at 8 chunks for one that such a run starts in, and adds
+// the run's partial rows: four groups of threads take a quarter of them each, then the quarters are
+// added in order.
 constexpr int kJoinGroups = 4;
+constexpr int kJoinChunks = 8;
 
 template <typename T, int E>
 __global__ void __launch_bounds__(kSumThreads * kJoinGroups)
 embed_join_kernel(const EmbedSumParams p) {
-  const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.chunk;
-  const int64_t end = begin + p.chunk;
-  if (end >= p.T) return;
-  const uint32_t k = p.skey[end - 1];
-  if (k == static_cast<uint32_t>(p.V) || p.skey[end] != k) return;
-  if (p.skey[begin] == k && begin > 0 && p.skey[begin - 1] == k) return;    // it started before
-  // last place of the run: keys are sorted
-  int64_t lo = end, hi = p.T;               // skey[lo] == k, skey[hi] > k (or hi == T)
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (p.skey[mid] == k) lo = mid; else hi = mid;
-  }
-  const int64_t first = blockIdx.x + 1, n = lo / p.chunk - blockIdx.x;      // its other chunks
   __shared__ float part[kJoinGroups][E][kSumThreads];
+  __shared__ uint32_t found;
+  if (threadIdx.x < 32) {
+    const int64_t ch = static_cast<int64_t>(blockIdx.x) * kJoinChunks + threadIdx.x;
+    const int64_t begin = ch * p.chunk, end = begin + p.chunk;
+    bool starts = false;
+    if (threadIdx.x < kJoinChunks && end + p.chunk < p.T) {
+      const uint32_t k = p.skey[end - 1];
+      // covers the next chunk whole, and began in this one
+      starts = k != static_cast<uint32_t>(p.V) && p.skey[end + p.chunk] == k &&
+               !(p.skey[begin] == k && begin > 0 && p.skey[begin - 1] == k);
+    }
+    const uint32_t m = __ballot_sync(0xffffffffu, starts);
+    if (threadIdx.x == 0) found = m;
+  }
+  __syncthreads();
   const int t = threadIdx.x % kSumThreads, g = threadIdx.x / kSumThreads;
   const int c = (blockIdx.y * kSumThreads + t) * E;
-  float acc[E];
-#pragma unroll
-  for (int j = 0; j < E; ++j) acc[j] = 0.f;
-  if (c < p.D) {
-    if (g == 0) {
-      const float* q = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.D + c;
-#pragma unroll
-      for (int j = 0; j < E; ++j) acc[j] = q[j];
+  for (uint32_t m = found; m != 0; m &= m - 1) {
+    const int which = __ffs(m) - 1;
+    const int64_t ch0 = static_cast<int64_t>(blockIdx.x) * kJoinChunks + which;
+    // The run's last place: keys are sorted, all threads narrow its range together.
+    const uint32_t k = p.skey[(ch0 + 1) * p.chunk];
+    // The first round looks at single places, so only runs beyond 512 more take a second.
+    constexpr int64_t kProbes = kSumThreads * kJoinGroups;
+    int64_t lo = (ch0 + 2) * p.chunk, hi = p.T, step = 1; // skey[lo] == k, skey[hi] > k (or hi == T)
+    while (hi - lo > 1) {
+      const int64_t at = lo + (static_cast<int64_t>(threadIdx.x) + 1) * step;
+      const int64_t below = __syncthreads_count(at < hi && p.skey[at] == k);
+      lo += below * step;
+      if (below < kProbes) hi = min(hi, lo + step);
+      step = (hi - lo + kProbes - 1) / kProbes;
     }
-    const int64_t c1 = first + n * (g + 1) / kJoinGroups;
+    const int64_t n = lo / p.chunk - ch0;                 // its chunks after the first
+    float acc[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) acc[j] = 0.f;
+    if (c < p.D) {
+      if (g == 0) {
+        const float* q = p.part + (ch0 * 2 + 1) * p.D + c;
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[j] = q[j];
+      }
+      const int64_t c1 = ch0 + 1 + n * (g + 1) / kJoinGroups;
 #pragma unroll 8
-    for (int64_t ch = first + n * g / kJoinGroups; ch < c1; ++ch) {
-      const float* s = p.part + ch * 2 * p.D + c;
+      for (int64_t ch = ch0 + 1 + n * g / kJoinGroups; ch < c1; ++ch) {
+        const float* q = p.part + ch * 2 * p.D + c;
 #pragma unroll
-      for (int j = 0; j < E; ++j) acc[j] += s[j];
+        for (int j = 0; j < E; ++j) acc[j] += q[j];
+      }
     }
+#pragma unroll
+    for (int j = 0; j < E; ++j) part[g][j][t] = acc[j];
+    __syncthreads();
+    if (g == 0 && c < p.D) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+#pragma unroll
+        for (int i = 1; i < kJoinGroups; ++i) acc[j] += part[i][j][t];
+        acc[j] *= p.scale;
+      }
+      store_e<T, E>(static_cast<T*>(p.out) + static_cast<int64_t>(k) * p.D + c, acc);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int j = 0; j < E; ++j) part[g][j][t] = acc[j];
-  __syncthreads();
-  if (g != 0 || c >= p.D) return;
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-#pragma unroll
-    for (int i = 1; i < kJoinGroups; ++i) acc[j] += part[i][j][t];
-    acc[j] *= p.scale;
-  }
-  store_e<T, E>(static_cast<T*>(p.out) + static_cast<int64_t>(k) * p.D + c, acc);
 }
 
 }  // namespace dc

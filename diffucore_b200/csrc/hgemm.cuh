@@ -134,6 +134,23 @@ __device__ __forceinline__ float2 act_value_grad(float z, int act) {
   }
 }
 
+// f(j, activation, derivative) for every value of a block.
+template <int N, int ACT, typename F>
+__device__ __forceinline__ void each_grad(const float (&z)[N], F f) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) { const float2 a = act_value_grad(z[j], ACT); f(j, a.x, a.y); }
+}
+template <int N, typename F>
+__device__ __forceinline__ void act_grads(const float (&z)[N], int act, F f) {
+  switch (act) {
+    case kActRelu: each_grad<N, kActRelu>(z, f); break;
+    case kActSilu: each_grad<N, kActSilu>(z, f); break;
+    case kActGelu: each_grad<N, kActGelu>(z, f); break;
+    case kActGeluTanh: each_grad<N, kActGeluTanh>(z, f); break;
+    default: each_grad<N, kActNone>(z, f); break;
+  }
+}
+
 // ------------------------------------------------------------------ operand tiles
 
 // TMA loads of one 64-deep atom. K-major: one box of 64 k x `rows` rows at (k, row). MN-major:

@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 #include "hgemm.cuh"
 #include "textgrad.cuh"
 
@@ -38,14 +39,14 @@ __device__ __forceinline__ void load_e(const T* p, float* f) {
 }
 template <typename T, int E>
 __device__ __forceinline__ void store_e(T* p, const float* f) {
-  if (E == 1) {
+  if constexpr (E == 1) {
     *p = from_f<T>(f[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
   } else {
-    uint4 u;
-    T* h = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int i = 0; i < E; ++i) h[i] = from_f<T>(f[i]);
-    *reinterpret_cast<uint4*>(p) = u;
+    constexpr int bf16 = std::is_same<T, __nv_bfloat16>::value;
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_h2(f[0], f[1], bf16), pack_h2(f[2], f[3], bf16),
+                                              pack_h2(f[4], f[5], bf16), pack_h2(f[6], f[7], bf16));
   }
 }
 // E values of the weight or bias, in x's type or in fp32.
@@ -57,6 +58,70 @@ __device__ __forceinline__ void load_w(const void* w, int64_t i, bool f32, float
   } else {
     load_e<T, E>(static_cast<const T*>(w) + i, f);
   }
+}
+
+// Two floats in one 64-bit register pair: the packed fp32 instructions of sm_100 do two operations per
+// issue slot, and issue slots are what bounds the 16-bit rows.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// A 16-byte unit of x's type as pairs of floats, and back.
+template <typename T>
+__device__ __forceinline__ void unit_pairs(const uint4& u, Pair (&f)[8 / sizeof(T)]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (sizeof(T) == 4) {
+    f[0] = pair(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    f[1] = pair(__uint_as_float(w[2]), __uint_as_float(w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+      } else {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[i] = pair(v.x, v.y);
+      }
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pairs_unit(const Pair (&f)[8 / sizeof(T)]) {
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 4) {
+    const float2 a = split(f[0]), b = split(f[1]);
+    w[0] = __float_as_uint(a.x); w[1] = __float_as_uint(a.y); w[2] = __float_as_uint(b.x); w[3] = __float_as_uint(b.y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = split(f[i]);
+      w[i] = pack_h2(v.x, v.y, std::is_same<T, __nv_bfloat16>::value);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Sums of two values over the TPR threads of a row. A CTA holds one row when TPR > 32; `red` is
@@ -95,9 +160,10 @@ struct NormParams {
   int64_t ldo;
   float* mean;              // [M]; forward: null when not kept
   float* rstd;
-  float* part_w;            // backward: [gridDim.x, ldp] partial column sums, or null
+  float* part_w;            // backward: [parts, ldp] partial column sums, or null
   float* part_b;
   int64_t ldp;
+  int parts;                // partial rows
   int64_t M;
   int D;
   float eps;
@@ -147,7 +213,7 @@ norm_fwd_kernel(const NormParams p) {
       for (int j = 0; j < E; ++j) { const float d = to_f(h[j]) - mean; s += d * d; }
     }
   }
-  const float rstd = 1.0f / sqrtf(row_sum2<TPR>(s, 0.f, red, turn).x * inv + p.eps);
+  const float rstd = rsqrtf(row_sum2<TPR>(s, 0.f, red, turn).x * inv + p.eps);
   if (t == 0 && p.mean != nullptr) { p.mean[row] = mean; p.rstd[row] = rstd; }
   T* y = static_cast<T*>(p.out) + row * p.ldo;
 #pragma unroll
@@ -167,210 +233,273 @@ norm_fwd_kernel(const NormParams p) {
 }
 
 // Rows streamed through a ring of shared-memory stages by bulk copies: the backward pass, and the
-// forward pass of rows that no 16-byte access fits. Persistent CTAs of 256 threads (512 for rows
-// above 4096 values) take kRows rows at a time; each thread keeps its columns of w (and of the dw /
-// db sums) in registers for all its rows. The registers that those sums take leave too little room
-// to hide HBM's latency with loads in flight; the ring keeps several rows per CTA on their way
-// whatever the occupancy.
+// forward pass of many rows. Persistent CTAs of 128 threads (more for wide rows) take kRows rows at
+// a time, TPR threads and EPT values per thread for each; warp 0 also issues the copies,
+// into the stage that the previous step emptied (a warp of its own for them would cost the others a
+// quarter of their registers). A thread keeps its columns of w (and of the dw / db sums) in registers for all its rows.
+// Those registers leave too little occupancy to hide HBM's latency with loads in flight; the ring keeps
+// several rows per CTA on their way whatever the occupancy.
 //
-// A bulk copy starts and ends on 16-byte boundaries. Where rows do not, the copy takes the aligned
-// window around the row; the bytes before and after it belong to the neighbouring rows, and the
-// first and the last row, which lack one, are read in place instead.
+// A bulk copy starts and ends on 16-byte boundaries. Where rows do not (E == 1), the copy takes the
+// aligned window around the row; the bytes before and after it belong to the neighbouring rows, and
+// the first and the last row, which lack one, are read in place instead.
 constexpr int kRingMax = 8;
 
-template <int TPR> struct RingCta { static constexpr int kThreads = TPR > 256 ? TPR : 256; };
+template <int TPR, int EPT, bool BWD> struct RingCta {
+  static constexpr int kThreads = TPR > 128 ? TPR : 128;
+  static constexpr int kSmThreads = EPT > 16 ? (BWD ? 256 : 512) : (BWD ? 512 : 768);   // resident per SM
+  static constexpr int kPerSm = kSmThreads > kThreads ? kSmThreads / kThreads : 1;
+};
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-template <typename T, int E, int TPR, bool BWD>
-__global__ void __launch_bounds__(RingCta<TPR>::kThreads, TPR > 256 ? 1 : 2)
+template <typename T, int E, int EPT, int TPR, bool BWD>
+__global__ void __launch_bounds__(RingCta<TPR, EPT, BWD>::kThreads, RingCta<TPR, EPT, BWD>::kPerSm)
 norm_ring_kernel(const NormParams p) {
-  constexpr int EPT = 16;
   constexpr int NV = EPT / E;
-  constexpr int kRows = RingCta<TPR>::kThreads / TPR;
+  constexpr int kThreads = RingCta<TPR, EPT, BWD>::kThreads;
+  constexpr int kWarps = kThreads / 32;
+  constexpr int kRows = kThreads / TPR;
   constexpr int kTensors = BWD ? 2 : 1;
   extern __shared__ __align__(16) uint8_t ring[];      // [stage][row][x, dy][slot]
   __shared__ __align__(8) uint64_t full[kRingMax];
-  __shared__ float2 red[2 * (RingCta<TPR>::kThreads / 32)];
-  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  __shared__ __align__(8) uint64_t empty[kRingMax];
+  __shared__ float2 red[2 * kWarps];
+  const int warp = warp_id(), lane = lane_id();
   const int64_t blocks = (p.M + kRows - 1) / kRows;
   const uint8_t* src[2] = {static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.dy)};
   const int64_t pitch[2] = {p.ldx * static_cast<int64_t>(sizeof(T)), p.lddy * static_cast<int64_t>(sizeof(T))};
   const int row_bytes = p.D * static_cast<int>(sizeof(T));
-  const bool edges = E == 1;                            // rows 0 and M - 1 are read in place
+  auto in_place = [&](int64_t row) { return E == 1 && (row == 0 || row == p.M - 1); };
   auto slot = [&](int stage, int r, int which) { return ring + ((stage * kRows + r) * kTensors + which) * p.slot; };
 
-  // Thread 0: the copies of the rows of one block.
-  auto issue = [&](int stage, int64_t block) {
-    uint32_t total = 0;
-#pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      for (int r = 0; r < kRows; ++r) {
-        const int64_t row = block * kRows + r;
-        if (row >= p.M || (edges && (row == 0 || row == p.M - 1))) continue;
-#pragma unroll
-        for (int k = 0; k < kTensors; ++k) {
-          const uintptr_t a = reinterpret_cast<uintptr_t>(src[k] + row * pitch[k]);
-          const uintptr_t lo = a & ~uintptr_t(15), hi = (a + row_bytes + 15) & ~uintptr_t(15);
-          if (pass == 0) total += static_cast<uint32_t>(hi - lo);
-          else bulk_load(slot(stage, r, k), reinterpret_cast<const void*>(lo), static_cast<uint32_t>(hi - lo), &full[stage]);
-        }
-      }
-      if (pass == 0) {
-        if (total > 0) mbar_arrive_expect_tx(&full[stage], total);
-        else mbar_arrive(&full[stage]);
-      }
-    }
-  };
-
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], kWarps); }
     fence_barrier_init();
+  }
+  __syncthreads();
+
+  // Warp 0: the copies of a block's rows into a stage, lane r row r.
+  auto issue = [&](int stage, int64_t block) {
+    const int64_t row = block * kRows + lane;
+    const bool copies = lane < kRows && row < p.M && !in_place(row);
+    uintptr_t lo[kTensors];
+    uint32_t n[kTensors], total = 0;
+#pragma unroll
+    for (int k = 0; k < kTensors; ++k) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(src[k] + row * pitch[k]);
+      lo[k] = at & ~uintptr_t(15);
+      n[k] = static_cast<uint32_t>(((at + row_bytes + 15) & ~uintptr_t(15)) - lo[k]);
+      if (copies) total += n[k];
+    }
+    if constexpr (kRows > 1) {
+#pragma unroll
+      for (int o = 1; o < kRows; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);    // rows are in the first lanes
+    }
+    if (lane == 0) {
+      if (total > 0) mbar_arrive_expect_tx(&full[stage], total);
+      else mbar_arrive(&full[stage]);
+    }
+    __syncwarp();
+    if (copies) {
+#pragma unroll
+      for (int k = 0; k < kTensors; ++k) bulk_load(slot(stage, lane, k), reinterpret_cast<const void*>(lo[k]), n[k], &full[stage]);
+    }
+    __syncwarp();
+  };
+  if (warp == 0) {
     for (int s = 0; s < p.stages; ++s) {
       const int64_t block = blockIdx.x + static_cast<int64_t>(s) * gridDim.x;
       if (block < blocks) issue(s, block);
     }
   }
-  float w[EPT], sw[EPT], sb[EPT];                       // forward: sb is b
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * E;
-#pragma unroll
-    for (int j = 0; j < E; ++j) { w[i * E + j] = c < p.D ? 1.0f : 0.f; sw[i * E + j] = 0.f; sb[i * E + j] = 0.f; }
-    if (c < p.D && p.w != nullptr) load_w<T, E>(p.w, c, p.w_f32, w + i * E);
-    if (!BWD && c < p.D && p.b != nullptr) load_w<T, E>(p.b, c, p.w_f32, sb + i * E);
-  }
-  __syncthreads();
-  const float inv = 1.0f / static_cast<float>(p.D);
-  int stage = 0, turn = 0;
-  uint32_t phase = 0;
-  // Sums over a row's threads; every thread of the CTA takes part, and when it returns every thread
-  // has read its values of the stage.
-  auto row_sums = [&](float a, float b) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    float2* sl = red + turn * (RingCta<TPR>::kThreads / 32);
-    turn ^= 1;
-    if (TPR > 32 && (threadIdx.x & 31) == 0) sl[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    if (TPR > 32) {
-      a = 0.f; b = 0.f;
-#pragma unroll
-      for (int i = 0; i < TPR / 32; ++i) { const float2 f = sl[sub * (TPR / 32) + i]; a += f.x; b += f.y; }
-    }
-    return make_float2(a, b);
-  };
 
-  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-    const int64_t row = block * kRows + sub;
-    const bool live = row < p.M;
-    float mean = 0.f, rstd = 0.f;
-    if (BWD && live) { mean = p.mean[row]; rstd = p.rstd[row]; }
-    mbar_wait(&full[stage], phase, nullptr);
-    __syncwarp();
-    const T* px = nullptr;
-    const T* pd = nullptr;
-    if (live) {
-      const uint8_t* a[2];
-#pragma unroll
-      for (int k = 0; k < kTensors; ++k) {
-        const uint8_t* g = src[k] + row * pitch[k];
-        a[k] = edges && (row == 0 || row == p.M - 1) ? g : slot(stage, sub, k) + (reinterpret_cast<uintptr_t>(g) & 15);
-      }
-      px = reinterpret_cast<const T*>(a[0]);
-      if (BWD) pd = reinterpret_cast<const T*>(a[1]);
-    }
-    float h[EPT], d[EPT];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  constexpr int kPairs = EPT / 2;
+  Pair w[kPairs], sw[kPairs], sb[kPairs];               // forward: sb is b
+  {
+    float wf[EPT], bf[EPT];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * E;
-      if (live && c < p.D) {
-        load_e<T, E>(px + c, h + i * E);
-        if (BWD) load_e<T, E>(pd + c, d + i * E);
-      } else {
 #pragma unroll
-        for (int j = 0; j < E; ++j) { h[i * E + j] = mean; d[i * E + j] = 0.f; }
+      for (int j = 0; j < E; ++j) { wf[i * E + j] = c < p.D ? 1.0f : 0.f; bf[i * E + j] = 0.f; }
+      if (c < p.D && p.w != nullptr) load_w<T, E>(p.w, c, p.w_f32, wf + i * E);
+      if (!BWD && c < p.D && p.b != nullptr) load_w<T, E>(p.b, c, p.w_f32, bf + i * E);
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      w[i] = pair(wf[2 * i], wf[2 * i + 1]);
+      sb[i] = pair(bf[2 * i], bf[2 * i + 1]);
+      sw[i] = pair(0.f, 0.f);
+    }
+  }
+  const float inv = 1.0f / static_cast<float>(p.D);
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  // Sums over a row's threads, two halves of `red` in turn so that one barrier per sum is enough.
+  auto row_sums = [&](float2 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      if (BWD) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if constexpr (TPR > 32) {
+      constexpr int kParts = TPR / 32;
+      float2* sl = red + turn * kWarps;
+      turn ^= 1;
+      if (lane == 0) sl[warp] = v;
+      named_barrier_sync(1 + sub, TPR);
+      v = sl[sub * kParts + lane % kParts];
+#pragma unroll
+      for (int o = kParts / 2; o > 0; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        if (BWD) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
       }
     }
-    float2 s;
-    if (BWD) {
-      float sa = 0.f, sh = 0.f;
-#pragma unroll
-      for (int i = 0; i < EPT; ++i) {
-        h[i] = (h[i] - mean) * rstd;
-        sw[i] += d[i] * h[i];
-        sb[i] += d[i];
-        d[i] = __fmul_rn(d[i], w[i]);       // the same value in the sum and in dx: a one-value row gives 0
-        sa += d[i];
-        sh += d[i] * h[i];
-      }
-      s = row_sums(sa, sh);
-    } else {
-      float sa = 0.f;
-#pragma unroll
-      for (int i = 0; i < EPT; ++i) sa += h[i];          // 0 past the row
-      s = row_sums(sa, 0.f);
-    }
-    if (threadIdx.x == 0) {
-      const int64_t next = block + static_cast<int64_t>(p.stages) * gridDim.x;
-      if (next < blocks) issue(stage, next);
-    }
-    if (++stage == p.stages) { stage = 0; phase ^= 1; }
-    if (!BWD) {
-      mean = s.x * inv;
-      float sq = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if ((i * TPR + t) * E < p.D) {
-#pragma unroll
-          for (int j = 0; j < E; ++j) { h[i * E + j] -= mean; sq += h[i * E + j] * h[i * E + j]; }
-        }
-      rstd = 1.0f / sqrtf(row_sums(sq, 0.f).x * inv + p.eps);
-      if (live && t == 0 && p.mean != nullptr) { p.mean[row] = mean; p.rstd[row] = rstd; }
-    }
+    return v;
+  };
+  float mean = 0.f, rstd = 0.f;                         // backward: of the next row, loaded a row ahead
+  auto load_stats = [&](int64_t block) {
+    const int64_t row = block * kRows + sub;
+    mean = row < p.M ? p.mean[row] : 0.f;
+    rstd = row < p.M ? p.rstd[row] : 0.f;
+  };
+  if (BWD && blockIdx.x < blocks) load_stats(blockIdx.x);
+
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const int64_t row = block * kRows + sub;
+    const bool live = kRows == 1 || row < p.M;
+    float mu = mean, rs = rstd;
+    if (BWD && block + gridDim.x < blocks) load_stats(block + gridDim.x);
+    mbar_wait(&full[stage], phase, nullptr);
+    __syncwarp();
+    const uint8_t* a[2] = {nullptr, nullptr};
     if (live) {
-      T* out = static_cast<T*>(p.out) + row * p.ldo;
-      const float ma = s.x * inv, mh = s.y * inv;
+#pragma unroll
+      for (int k = 0; k < kTensors; ++k) {
+        const uint8_t* g = src[k] + row * pitch[k];
+        a[k] = in_place(row) ? g : slot(stage, sub, k) + (reinterpret_cast<uintptr_t>(g) & 15);
+      }
+    }
+    // Values past the row read as the mean: their deviation is 0 backward, and they add 0 forward.
+    Pair h[kPairs], d[BWD ? kPairs : 1];
+    {
+      float hf[EPT], df[EPT];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + t) * E;
-        if (c < p.D) {
-          float o[E];
+        if (live && c < p.D) {
+          load_e<T, E>(reinterpret_cast<const T*>(a[0]) + c, hf + i * E);
+          if (BWD) load_e<T, E>(reinterpret_cast<const T*>(a[1]) + c, df + i * E);
+        } else {
 #pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const int k = i * E + j;
-            o[j] = BWD ? rstd * (d[k] - ma - h[k] * mh) : h[k] * rstd * w[k] + sb[k];
-          }
-          store_e<T, E>(out + c, o);
+          for (int j = 0; j < E; ++j) { hf[i * E + j] = mu; df[i * E + j] = 0.f; }
         }
+      }
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        h[i] = pair(hf[2 * i], hf[2 * i + 1]);
+        if (BWD) d[i] = pair(df[2 * i], df[2 * i + 1]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[stage]);          // this warp's values are in registers
+    // Refill the stage of the step before: the other warps are past it or nearly so.
+    if (warp == 0 && block != blockIdx.x) {
+      const int prev = stage == 0 ? p.stages - 1 : stage - 1;
+      const int64_t next = block + static_cast<int64_t>(p.stages - 1) * gridDim.x;
+      if (next < blocks) {
+        const bool ok = mbar_wait(&empty[prev], stage == 0 ? phase ^ 1 : phase, nullptr);
+        if (__all_sync(0xffffffffu, ok)) issue(prev, next);
+      }
+    }
+    if (++stage == p.stages) { stage = 0; phase ^= 1; }
+    float2 s = make_float2(0.f, 0.f);
+    if (BWD) {
+      const Pair nm = pair(-mu, -mu), rr = pair(rs, rs);
+      Pair sa = pair(0.f, 0.f), sh = sa;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        h[i] = (h[i] + nm) * rr;
+        sw[i] = fma(d[i], h[i], sw[i]);
+        sb[i] = sb[i] + d[i];
+        d[i] = d[i] * w[i];
+        sa = sa + d[i];
+        sh = fma(d[i], h[i], sh);
+      }
+      const float2 fa = split(sa), fh = split(sh);
+      s = row_sums(make_float2(fa.x + fa.y, fh.x + fh.y));
+    } else {
+      Pair sa = pair(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) sa = sa + h[i];
+      float2 f = split(sa);
+      mu = row_sums(make_float2(f.x + f.y, 0.f)).x * inv;
+      const Pair nm = pair(-mu, -mu);
+      sa = pair(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        h[i] = h[i] + nm;
+        // the pair's two values are E-neighbours or, one value per unit, TPR columns apart
+        const int c0 = E == 1 ? 2 * i * TPR + t : (2 * i / E * TPR + t) * E, c1 = E == 1 ? c0 + TPR : c0;
+        if (c1 < p.D) {
+          sa = fma(h[i], h[i], sa);
+        } else if (E == 1 && c0 < p.D) {
+          const Pair one = pair(split(h[i]).x, 0.f);
+          sa = fma(one, one, sa);
+        }
+      }
+      f = split(sa);
+      rs = rsqrtf(row_sums(make_float2(f.x + f.y, 0.f)).x * inv + p.eps);
+      if (live && t == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = rs; }
+    }
+    if (live) {
+      T* out = static_cast<T*>(p.out) + row * p.ldo;
+      const Pair rr = pair(rs, rs), nma = pair(-s.x * inv, -s.x * inv), nmh = pair(-s.y * inv, -s.y * inv);
+      float o[EPT];
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const float2 f = split(BWD ? (fma(h[i], nmh, d[BWD ? i : 0]) + nma) * rr : fma(h[i] * rr, w[i], sb[i]));
+        o[2 * i] = f.x;
+        o[2 * i + 1] = f.y;
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * E;
+        if (c < p.D) store_e<T, E>(out + c, o + i * E);
       }
     }
   }
   if (!BWD || p.part_w == nullptr) return;
+  float fw[EPT], fb[EPT];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const float2 x = split(sw[i]), y = split(sb[i]);
+    fw[2 * i] = x.x; fw[2 * i + 1] = x.y;
+    fb[2 * i] = y.x; fb[2 * i + 1] = y.y;
+  }
   if (kRows > 1) {
     // The CTA's row groups hold sums of the same columns: added in the order of the groups.
     float* acc = reinterpret_cast<float*>(ring);         // no copy is under way any more
-    __syncthreads();
     for (int g = 0; g < kRows; ++g) {
+      __syncthreads();
       if (sub == g) {
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
           const int k = i * TPR + t;
-          acc[k] = g == 0 ? sw[i] : acc[k] + sw[i];
-          acc[TPR * EPT + k] = g == 0 ? sb[i] : acc[TPR * EPT + k] + sb[i];
+          acc[k] = g == 0 ? fw[i] : acc[k] + fw[i];
+          acc[TPR * EPT + k] = g == 0 ? fb[i] : acc[TPR * EPT + k] + fb[i];
         }
       }
-      __syncthreads();
     }
+    __syncthreads();
     if (sub != 0) return;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) { sw[i] = acc[i * TPR + t]; sb[i] = acc[TPR * EPT + i * TPR + t]; }
+    for (int i = 0; i < EPT; ++i) { fw[i] = acc[i * TPR + t]; fb[i] = acc[TPR * EPT + i * TPR + t]; }
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -378,8 +507,187 @@ norm_ring_kernel(const NormParams p) {
     if (c < p.D) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        p.part_w[blockIdx.x * p.ldp + c + j] = sw[i * E + j];
-        p.part_b[blockIdx.x * p.ldp + c + j] = sb[i * E + j];
+        p.part_w[blockIdx.x * p.ldp + c + j] = fw[i * E + j];
+        p.part_b[blockIdx.x * p.ldp + c + j] = fb[i * E + j];
+      }
+    }
+  }
+}
+
+// The affine vector of 16-byte units of a row in shared memory: units in x's type, or, for fp32
+// vectors beside 16-bit rows (W32), E / 4 planes of four floats per unit, so that a warp's loads are
+// consecutive. A null vector reads as `fill`.
+template <typename T, bool W32>
+struct AffineStage {
+  static constexpr int E = 16 / static_cast<int>(sizeof(T));
+  static constexpr int kPlanes = W32 ? E / 4 : 1;
+
+  __device__ static void store(uint4* dst, const void* w, int units, float fill) {
+    for (int i = threadIdx.x; i < units * kPlanes; i += blockDim.x) {
+      uint4 v;
+      if (w != nullptr) {
+        v = W32 ? static_cast<const uint4*>(w)[(i % units) * kPlanes + i / units] : static_cast<const uint4*>(w)[i];
+      } else if (W32) {
+        const uint32_t f = __float_as_uint(fill);
+        v = make_uint4(f, f, f, f);
+      } else {
+        T* h = reinterpret_cast<T*>(&v);
+#pragma unroll
+        for (int j = 0; j < E; ++j) h[j] = from_f<T>(fill);
+      }
+      dst[i] = v;
+    }
+  }
+  __device__ static void load(const uint4* src, int units, int unit, Pair (&f)[E / 2]) {
+    if (W32) {
+#pragma unroll
+      for (int q = 0; q < kPlanes; ++q) {
+        const float4 v = reinterpret_cast<const float4*>(src)[q * units + unit];
+        f[2 * q] = pair(v.x, v.y);
+        f[2 * q + 1] = pair(v.z, v.w);
+      }
+    } else {
+      unit_pairs<T>(src[unit], f);
+    }
+  }
+};
+
+// Backward of aligned rows of 8193 to 16384 values: a persistent CTA of 512 threads per row, 32 values
+// per thread. The dw / db sums take 64 of the 128 registers that a thread can have, so x and dy stay
+// in the ring's stage and are read twice, before and after the row's two sums, and w is staged in
+// shared memory: 8000 x 16384 bf16 rows in 231 us, 298 in the kernels for any width.
+constexpr int kBwdThreads = 512;
+constexpr int kBwdValues = 32;
+
+template <typename T, bool W32>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+norm_bwd_kernel(const NormParams p) {
+  using Affine = AffineStage<T, W32>;
+  constexpr int E = Affine::E, NU = kBwdValues / E, kPairs = E / 2, kWarps = kBwdThreads / 32;
+  extern __shared__ __align__(16) uint4 smem[];          // w, then [stage][x, dy][units]
+  __shared__ __align__(8) uint64_t full[kRingMax];
+  __shared__ __align__(8) uint64_t empty[kRingMax];
+  __shared__ float2 red[2 * kWarps];
+  const int warp = warp_id(), lane = lane_id();
+  const int t = threadIdx.x;
+  const int units = p.D / E;
+  const uint32_t row_bytes = static_cast<uint32_t>(units) * 16;
+  uint4* const ring = smem + units * Affine::kPlanes;
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], kWarps); }
+    fence_barrier_init();
+  }
+  Affine::store(smem, p.w, units, 1.0f);
+  __syncthreads();
+  auto issue = [&](int stage, int64_t row) {              // thread 0
+    uint4* dst = ring + static_cast<int64_t>(stage) * 2 * units;
+    mbar_arrive_expect_tx(&full[stage], 2 * row_bytes);
+    bulk_load(dst, x + row * p.ldx, row_bytes, &full[stage]);
+    bulk_load(dst + units, dy + row * p.lddy, row_bytes, &full[stage]);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      const int64_t row = blockIdx.x + static_cast<int64_t>(s) * gridDim.x;
+      if (row < p.M) issue(s, row);
+    }
+  }
+  Pair sw[NU][kPairs], sb[NU][kPairs];
+#pragma unroll
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) { sw[i][j] = pair(0.f, 0.f); sb[i][j] = sw[i][j]; }
+  const float inv = 1.0f / static_cast<float>(p.D);
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  float next_mean = 0.f, next_rstd = 0.f;                // loaded a row ahead
+  auto load_stats = [&](int64_t row) {
+    next_mean = p.mean[row];
+    next_rstd = p.rstd[row];
+  };
+  if (blockIdx.x < p.M) load_stats(blockIdx.x);
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    const Pair nm = pair(-next_mean, -next_mean), rr = pair(next_rstd, next_rstd);
+    if (row + gridDim.x < p.M) load_stats(row + gridDim.x);
+    mbar_wait(&full[stage], phase, nullptr);
+    __syncwarp();
+    const uint4* xs = ring + static_cast<int64_t>(stage) * 2 * units;
+    const uint4* ds = xs + units;
+    Pair sa[2] = {pair(0.f, 0.f), pair(0.f, 0.f)}, sh[2] = {sa[0], sa[0]};
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int u = i * kBwdThreads + t;
+      if (u < units) {
+        Pair h[kPairs], d[kPairs], w[kPairs];
+        unit_pairs<T>(xs[u], h);
+        unit_pairs<T>(ds[u], d);
+        Affine::load(smem, units, u, w);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const Pair c = (h[j] + nm) * rr;
+          sw[i][j] = fma(d[j], c, sw[i][j]);
+          sb[i][j] = sb[i][j] + d[j];
+          const Pair a = d[j] * w[j];
+          sa[j % 2] = sa[j % 2] + a;
+          sh[j % 2] = fma(a, c, sh[j % 2]);
+        }
+      }
+    }
+    const float2 fa = split(sa[0] + sa[1]), fh = split(sh[0] + sh[1]);
+    float2 s = make_float2(fa.x + fa.y, fh.x + fh.y);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+    }
+    float2* sl = red + turn * kWarps;                    // two halves in turn: one barrier per row
+    turn ^= 1;
+    if (lane == 0) sl[warp] = s;
+    __syncthreads();
+    s = sl[lane % kWarps];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+    }
+    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.ldo);
+    const Pair nma = pair(-s.x * inv, -s.x * inv), nmh = pair(-s.y * inv, -s.y * inv);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int u = i * kBwdThreads + t;
+      if (u < units) {
+        Pair h[kPairs], d[kPairs], w[kPairs];
+        unit_pairs<T>(xs[u], h);
+        unit_pairs<T>(ds[u], d);
+        Affine::load(smem, units, u, w);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) d[j] = (fma((h[j] + nm) * rr, nmh, d[j] * w[j]) + nma) * rr;
+        out[u] = pairs_unit<T>(d);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[stage]);
+    // Refill the stage of the step before: the other warps are past it or nearly so.
+    if (threadIdx.x == 0 && row != blockIdx.x) {
+      const int prev = stage == 0 ? p.stages - 1 : stage - 1;
+      const int64_t next = row + static_cast<int64_t>(p.stages - 1) * gridDim.x;
+      if (next < p.M && mbar_wait(&empty[prev], stage == 0 ? phase ^ 1 : phase, nullptr)) issue(prev, next);
+    }
+    __syncwarp();
+    if (++stage == p.stages) { stage = 0; phase ^= 1; }
+  }
+  if (p.part_w == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    const int c = (i * kBwdThreads + t) * E;
+    if (c < p.D) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        const int64_t at = static_cast<int64_t>(blockIdx.x) * p.ldp + c + 2 * j;     // ldp is even
+        *reinterpret_cast<float2*>(p.part_w + at) = split(sw[i][j]);
+        *reinterpret_cast<float2*>(p.part_b + at) = split(sb[i][j]);
       }
     }
   }
@@ -401,7 +709,7 @@ norm_fwd_wide_kernel(const NormParams p) {
   const float mean = row_sum2<kNormWide>(s, 0.f, red, turn).x * inv;
   s = 0.f;
   for (int c = threadIdx.x; c < p.D; c += kNormWide) { const float d = to_f(x[c]) - mean; s += d * d; }
-  const float rstd = 1.0f / sqrtf(row_sum2<kNormWide>(s, 0.f, red, turn).x * inv + p.eps);
+  const float rstd = rsqrtf(row_sum2<kNormWide>(s, 0.f, red, turn).x * inv + p.eps);
   if (threadIdx.x == 0 && p.mean != nullptr) { p.mean[row] = mean; p.rstd[row] = rstd; }
   T* y = static_cast<T*>(p.out) + row * p.ldo;
   for (int c = threadIdx.x; c < p.D; c += kNormWide) {
@@ -412,7 +720,7 @@ norm_fwd_wide_kernel(const NormParams p) {
   }
 }
 
-template <typename T>
+template <typename T, int E>
 __global__ void __launch_bounds__(kNormWide)
 norm_dx_wide_kernel(const NormParams p) {
   __shared__ float2 red[2 * (kNormWide / 32)];
@@ -423,41 +731,57 @@ norm_dx_wide_kernel(const NormParams p) {
   const float mean = p.mean[row], rstd = p.rstd[row];
   const float inv = 1.0f / static_cast<float>(p.D);
   float sa = 0.f, sh = 0.f;
-  for (int c = threadIdx.x; c < p.D; c += kNormWide) {
-    float w = 1.f;
-    if (p.w != nullptr) load_w<T, 1>(p.w, c, p.w_f32, &w);
-    const float a = __fmul_rn(to_f(dy[c]), w);
-    sa += a;
-    sh += a * ((to_f(x[c]) - mean) * rstd);
+#pragma unroll 4
+  for (int c = threadIdx.x * E; c < p.D; c += kNormWide * E) {
+    float xv[E], a[E], w[E];
+    load_e<T, E>(x + c, xv);
+    load_e<T, E>(dy + c, a);
+    if (p.w != nullptr) load_w<T, E>(p.w, c, p.w_f32, w);
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float v = __fmul_rn(a[j], p.w != nullptr ? w[j] : 1.f);
+      sa += v;
+      sh += v * ((xv[j] - mean) * rstd);
+    }
   }
   const float2 s = row_sum2<kNormWide>(sa, sh, red, turn);
+  const float ma = s.x * inv, mh = s.y * inv;
   T* dx = static_cast<T*>(p.out) + row * p.ldo;
-  for (int c = threadIdx.x; c < p.D; c += kNormWide) {
-    float w = 1.f;
-    if (p.w != nullptr) load_w<T, 1>(p.w, c, p.w_f32, &w);
-    const float a = __fmul_rn(to_f(dy[c]), w);
-    dx[c] = from_f<T>(rstd * (a - s.x * inv - (to_f(x[c]) - mean) * rstd * (s.y * inv)));
+#pragma unroll 4
+  for (int c = threadIdx.x * E; c < p.D; c += kNormWide * E) {
+    float xv[E], a[E], w[E], o[E];
+    load_e<T, E>(x + c, xv);
+    load_e<T, E>(dy + c, a);
+    if (p.w != nullptr) load_w<T, E>(p.w, c, p.w_f32, w);
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      o[j] = rstd * (__fmul_rn(a[j], p.w != nullptr ? w[j] : 1.f) - ma - (xv[j] - mean) * rstd * mh);
+    store_e<T, E>(dx + c, o);
   }
 }
 
-// Partial dw / db of a row block: one thread per column.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// Partial dw / db of a row block: one thread per E columns.
+template <typename T, int E>
+__global__ void __launch_bounds__(128)
 norm_dw_wide_kernel(const NormParams p, int rows_per_block) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int c = (blockIdx.x * 128 + threadIdx.x) * E;
   if (c >= p.D) return;
   const int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows_per_block;
   const int64_t r1 = min(p.M, r0 + rows_per_block);
-  float sw = 0.f, sb = 0.f;
+  float sw[E], sb[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) { sw[j] = 0.f; sb[j] = 0.f; }
 #pragma unroll 4
   for (int64_t r = r0; r < r1; ++r) {
-    const float d = to_f(static_cast<const T*>(p.dy)[r * p.lddy + c]);
-    const float h = (to_f(static_cast<const T*>(p.x)[r * p.ldx + c]) - p.mean[r]) * p.rstd[r];
-    sw += d * h;
-    sb += d;
+    float d[E], xv[E];
+    load_e<T, E>(static_cast<const T*>(p.dy) + r * p.lddy + c, d);
+    load_e<T, E>(static_cast<const T*>(p.x) + r * p.ldx + c, xv);
+    const float mean = p.mean[r], rstd = p.rstd[r];
+#pragma unroll
+    for (int j = 0; j < E; ++j) { sw[j] += d[j] * ((xv[j] - mean) * rstd); sb[j] += d[j]; }
   }
-  p.part_w[blockIdx.y * p.ldp + c] = sw;
-  p.part_b[blockIdx.y * p.ldp + c] = sb;
+#pragma unroll
+  for (int j = 0; j < E; ++j) { p.part_w[blockIdx.y * p.ldp + c + j] = sw[j]; p.part_b[blockIdx.y * p.ldp + c + j] = sb[j]; }
 }
 
 }  // namespace dc

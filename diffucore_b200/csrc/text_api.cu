@@ -328,10 +328,10 @@ int dc_linear_dw(const void* dz, const void* dz1, int64_t lddz, const void* x, i
 
 namespace {
 
-// Row blocks of the column sums: enough CTAs for eight per SM, at least 16 rows each.
+// Row blocks of the column sums: about eight CTAs per SM, at least 16 rows each.
 int64_t grad_row_blocks(int64_t M, int64_t N) {
   const int64_t col_blocks = ceil_div(N, dc::kGradCols);
-  return std::max<int64_t>(1, std::min<int64_t>({ceil_div(148 * 8, col_blocks), ceil_div(M, 16), 65535}));
+  return std::max<int64_t>(1, std::min<int64_t>({148 * 8 / col_blocks, ceil_div(M, 16), 65535}));
 }
 
 int colsum_finish(const float* p0, const float* p1, int64_t ldp, int64_t P, int64_t N, void* o0, void* o1, int dtype,
@@ -348,7 +348,7 @@ extern "C" {
 
 int dc_act_grad_workspace(int64_t M, int64_t N, size_t* bytes) {
   if (M < 0 || N <= 0 || bytes == nullptr) return fail("act_grad: bad shape M=%lld N=%lld", (long long)M, (long long)N);
-  *bytes = static_cast<size_t>(grad_row_blocks(M, N)) * round_up(N, 4) * 2 * sizeof(float);
+  *bytes = static_cast<size_t>(grad_row_blocks(M, N)) * round_up(N, 8) * 2 * sizeof(float);
   return DC_OK;
 }
 
@@ -367,7 +367,7 @@ int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, i
     if (z1 != nullptr && (r = check_operand("act_grad", "dz1", dz1, lddz, N))) return r;
   }
   if (db1 != nullptr && (z1 == nullptr || db == nullptr)) return fail("act_grad: db1 needs z1 and db");
-  const int64_t blocks = grad_row_blocks(M, N), ldp = round_up(N, 4);
+  const int64_t blocks = grad_row_blocks(M, N), ldp = round_up(N, 8);
   if (db != nullptr) {
     size_t need = 0;
     dc_act_grad_workspace(M, N, &need);
@@ -385,11 +385,13 @@ int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, i
   p.ldp = ldp; p.M = M; p.N = N;
   p.rows_per_block = static_cast<int>(ceil_div(M, blocks));
   p.act = act; p.bf16 = dtype == DC_DTYPE_BF16;
-  p.dy_vec = aligned(dy, 8) && lddy % 4 == 0;
+  p.dy_vec = aligned(dy, 16) && lddy % 8 == 0;
   const cudaStream_t st = as_stream(stream);
   const dim3 grid(static_cast<unsigned>(ceil_div(N, dc::kGradCols)), static_cast<unsigned>(blocks));
-  if (z1 != nullptr) dc::act_grad_kernel<true><<<grid, dc::kGradThreads, 0, st>>>(p);
-  else dc::act_grad_kernel<false><<<grid, dc::kGradThreads, 0, st>>>(p);
+  const dim3 block(dc::kGradX, dc::kGradY);
+  if (z1 != nullptr) dc::act_grad_kernel<2><<<grid, block, 0, st>>>(p);
+  else if (z != nullptr) dc::act_grad_kernel<1><<<grid, block, 0, st>>>(p);
+  else dc::act_grad_kernel<0><<<grid, block, 0, st>>>(p);
   DC_CHECK_LAUNCH("act_grad launch");
   if (db != nullptr) return colsum_finish(p.part0, p.part1, ldp, blocks, N, db, db1, dtype, st);
   return DC_OK;
@@ -401,54 +403,114 @@ int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, i
 
 namespace {
 
-constexpr int64_t kNormRing = 8192;            // widest row of the ring kernel
-
 int64_t norm_wide_blocks(int64_t M, int64_t D) {
-  return std::max<int64_t>(1, std::min<int64_t>({ceil_div(148 * 8, ceil_div(D, 256)), ceil_div(M, 16), 65535}));
+  return std::max<int64_t>(1, std::min<int64_t>({ceil_div(148 * 16, ceil_div(D, 512)), ceil_div(M, 16), 65535}));
 }
-int ring_threads_per_row(int64_t D) { return D <= 512 ? 32 : D <= 2048 ? 128 : D <= 4096 ? 256 : 512; }
-// CTAs of the backward pass: persistent ring CTAs, two per SM (one of 512 threads).
-int64_t norm_bwd_ctas(int64_t M, int64_t D) {
-  if (D > kNormRing) return norm_wide_blocks(M, D);
-  const int tpr = ring_threads_per_row(D);
-  return std::min<int64_t>(ceil_div(M, std::max(256, tpr) / tpr), tpr > 256 ? 148 : 2 * 148);
+// The ring kernel's launch shape: threads per row, values per thread, stages and persistent CTAs, as
+// many per SM as its registers and 200 KB of shared memory allow with at least two stages each; no
+// shape (ctas 0) where the row is too wide for it.
+struct RingPlan { int tpr, ept, slot, stages, smem; int64_t ctas; };
+
+RingPlan ring_plan(int64_t M, int64_t D, size_t es, bool vec, bool bwd) {
+  // 32 values per thread: the sums over a row cost each warp as much as 16 values' arithmetic
+  // (32768 x 4096 bf16: 96 us forward against 117 with 16 values, 167 against 171 backward). Rows read
+  // by single values need more threads' loads in flight at 2048 (10007 x 2047: 39 against 45 us).
+  RingPlan n = {};
+  n.tpr = D <= 1024 ? 32 : D <= 2048 ? 64 : D <= 4096 ? 128 : D <= 8192 ? 256 : 512;
+  n.ept = D <= 256 ? 8 : D <= 512 ? 16 : 32;
+  if (!vec && n.tpr == 64) { n.tpr = 128; n.ept = 16; }
+  if (D > 16384 || (bwd && D > 8192)) return n;
+  const int threads = std::max(128, n.tpr), rows = threads / n.tpr;
+  const int sm_threads = n.ept > 16 ? (bwd ? 256 : 512) : (bwd ? 512 : 768);
+  n.slot = static_cast<int>(round_up(D * static_cast<int64_t>(es), 16)) + (vec ? 0 : 16);
+  const int64_t stage = static_cast<int64_t>(rows) * (bwd ? 2 : 1) * n.slot;
+  constexpr int64_t kSm = 200 << 10;
+  int per_sm = std::max(1, sm_threads / threads);
+  while (per_sm > 0 && 2 * stage * per_sm > kSm) --per_sm;
+  if (per_sm == 0) return n;
+  n.stages = static_cast<int>(std::min<int64_t>(dc::kRingMax, kSm / per_sm / stage));
+  const int64_t sums = rows > 1 ? 2 * n.tpr * n.ept * 4 : 0;
+  n.smem = static_cast<int>(std::max(n.stages * stage, sums));
+  n.ctas = std::min<int64_t>(ceil_div(M, rows), 148 * per_sm);
+  return n;
 }
 
-template <typename T, int E, int TPR, bool BWD>
-int launch_ring(dc::NormParams p, int64_t ctas, cudaStream_t st) {
-  constexpr int kThreads = dc::RingCta<TPR>::kThreads, kRows = kThreads / TPR;
-  // A slot holds a row's aligned window. Stages: up to 96 KB of rows per CTA (two fit an SM).
-  p.slot = static_cast<int>(round_up(p.D * static_cast<int64_t>(sizeof(T)), 16)) + (E == 1 ? 16 : 0);
-  const int stage = kRows * (BWD ? 2 : 1) * p.slot;
-  p.stages = std::max(2, std::min(dc::kRingMax, (96 << 10) / stage));
-  const int sums = kRows > 1 ? 2 * TPR * 16 * static_cast<int>(sizeof(float)) : 0;
-  const int smem = std::max(p.stages * stage, sums);
-  auto kernel = dc::norm_ring_kernel<T, E, TPR, BWD>;
-  if (int r = set_smem(kernel, smem)) return r;
-  kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(p);
+// norm_bwd_kernel's stages and shared memory; no shape (stages 0) where fewer than two stages fit.
+struct NormBwdPlan { int stages, smem; };
+
+NormBwdPlan norm_bwd_plan(int64_t D, size_t es, bool w32) {
+  NormBwdPlan n = {};
+  if (D > dc::kBwdThreads * dc::kBwdValues) return n;
+  const int64_t w = D * static_cast<int64_t>(w32 ? 4 : es), stage = 2 * D * static_cast<int64_t>(es);
+  constexpr int64_t kSm = 200 << 10;
+  n.stages = static_cast<int>(std::min<int64_t>(dc::kRingMax, (kSm - w) / stage));
+  if (n.stages < 2) n.stages = 0;
+  n.smem = static_cast<int>(w + n.stages * stage);
+  return n;
+}
+
+template <typename T>
+int launch_norm_bwd(dc::NormParams p, const NormBwdPlan& n, cudaStream_t st) {
+  p.stages = n.stages;
+  auto go = [&](auto kernel) {
+    if (int r = set_smem(kernel, n.smem)) return r;
+    kernel<<<static_cast<unsigned>(p.parts), dc::kBwdThreads, n.smem, st>>>(p);
+    DC_CHECK_LAUNCH("layer_norm_grad launch");
+    return DC_OK;
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (p.w_f32) return go(dc::norm_bwd_kernel<T, true>);
+  }
+  return go(dc::norm_bwd_kernel<T, false>);
+}
+
+template <typename T, int E, int EPT, int TPR, bool BWD>
+int launch_ring(dc::NormParams p, const RingPlan& n, cudaStream_t st) {
+  p.slot = n.slot;
+  p.stages = n.stages;
+  auto kernel = dc::norm_ring_kernel<T, E, EPT, TPR, BWD>;
+  if (int r = set_smem(kernel, n.smem)) return r;
+  kernel<<<static_cast<unsigned>(n.ctas), dc::RingCta<TPR, EPT, BWD>::kThreads, n.smem, st>>>(p);
   DC_CHECK_LAUNCH("layer_norm launch");
   return DC_OK;
 }
 
 template <typename T, int E, bool BWD>
-int launch_ring_rows(const dc::NormParams& p, cudaStream_t st) {
-  const int64_t ctas = norm_bwd_ctas(p.M, p.D);
-  switch (ring_threads_per_row(p.D)) {
-    case 32: return launch_ring<T, E, 32, BWD>(p, ctas, st);
-    case 128: return launch_ring<T, E, 128, BWD>(p, ctas, st);
-    case 256: return launch_ring<T, E, 256, BWD>(p, ctas, st);
-    default: return launch_ring<T, E, 512, BWD>(p, ctas, st);
+int launch_ring_rows(const dc::NormParams& p, const RingPlan& n, cudaStream_t st) {
+  switch (n.tpr * 100 + n.ept) {
+    case 3208: return launch_ring<T, E, 8, 32, BWD>(p, n, st);
+    case 3216: return launch_ring<T, E, 16, 32, BWD>(p, n, st);
+    case 3232: return launch_ring<T, E, 32, 32, BWD>(p, n, st);
+    case 12832: return launch_ring<T, E, 32, 128, BWD>(p, n, st);
+    case 25632: return launch_ring<T, E, 32, 256, BWD>(p, n, st);
   }
+  if constexpr (E == 1) {
+    if (n.tpr == 128) return launch_ring<T, E, 16, 128, BWD>(p, n, st);
+  } else {
+    if (n.tpr == 64) return launch_ring<T, E, 32, 64, BWD>(p, n, st);
+  }
+  if constexpr (!BWD) return launch_ring<T, E, 32, 512, BWD>(p, n, st);
+  return fail("layer_norm: no kernel for rows of %d values", p.D);
 }
 
-// The forward register kernel: with many rows a warp per row as long as it holds the row (no
-// barriers), with few rows more threads per row (latency). False: the row is too wide.
+template <typename T, int E>
+int launch_norm_grad_wide(const dc::NormParams& p, cudaStream_t st) {
+  dc::norm_dx_wide_kernel<T, E><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
+  DC_CHECK_LAUNCH("layer_norm_grad launch");
+  if (p.part_w == nullptr) return DC_OK;
+  dc::norm_dw_wide_kernel<T, E><<<dim3(static_cast<unsigned>(ceil_div(p.D, 128 * E)), static_cast<unsigned>(p.parts)), 128, 0, st>>>(
+      p, static_cast<int>(ceil_div(p.M, p.parts)));
+  DC_CHECK_LAUNCH("layer_norm_grad launch");
+  return DC_OK;
+}
+
+// The forward register kernel, for few rows and narrow ones: the fewest threads per row that hold it
+// in two units (eight single values) each, up to 512 threads and eight units. False: too wide.
 template <typename T, bool VEC>
 bool launch_norm_reg(const dc::NormParams& p, cudaStream_t st) {
   constexpr int E = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
-  const bool many = p.M >= 148 * 16;
   const int64_t units = ceil_div(p.D, E);
-  const int most = VEC ? (many ? 16 : 2) : (many ? 32 : 8), top = VEC ? 16 : 32;
+  constexpr int most = VEC ? 2 : 8, top = VEC ? 8 : 32;
   const int tpr = units <= 32 * most ? 32 : units <= 128 * most ? 128 : 512;
   const int nu = static_cast<int>(ceil_div(units, tpr));
   if (nu > top) return false;
@@ -457,49 +519,52 @@ bool launch_norm_reg(const dc::NormParams& p, cudaStream_t st) {
     constexpr int TPR = decltype(t)::value, NU = decltype(n)::value;
     dc::norm_fwd_kernel<T, VEC, NU, TPR><<<ctas, dc::NormCta<TPR>::kThreads, 0, st>>>(p);
   };
-  auto units_per_thread = [&](auto t) {
-    using std::integral_constant;
-    if constexpr (VEC) {
-      if (nu <= 1) go(t, integral_constant<int, 1>{});
-      else if (nu <= 2) go(t, integral_constant<int, 2>{});
-      else if (nu <= 4) go(t, integral_constant<int, 4>{});
-      else if (nu <= 8) go(t, integral_constant<int, 8>{});
-      else go(t, integral_constant<int, 16>{});
-    } else {
-      if (nu <= 8) go(t, integral_constant<int, 8>{});
-      else go(t, integral_constant<int, 32>{});
-    }
-  };
-  if (tpr == 32) units_per_thread(std::integral_constant<int, 32>{});
-  else if (tpr == 128) units_per_thread(std::integral_constant<int, 128>{});
-  else units_per_thread(std::integral_constant<int, 512>{});
+  using std::integral_constant;
+  using I32 = integral_constant<int, 32>;
+  using I128 = integral_constant<int, 128>;
+  using I512 = integral_constant<int, 512>;
+  if (tpr == 32) go(I32{}, integral_constant<int, most>{});
+  else if (tpr == 128) go(I128{}, integral_constant<int, most>{});
+  else if (nu <= most) go(I512{}, integral_constant<int, most>{});
+  else go(I512{}, integral_constant<int, top>{});
   return true;
+}
+
+// Which kernel a gradient runs in, and its partial rows: the ring, for unaligned rows where the window
+// of a row lies inside its neighbours; the kernel for wide aligned rows; else the ones for any width.
+enum NormGradPath { kNormGradRing, kNormGradLong, kNormGradWide };
+NormGradPath norm_grad_path(const dc::NormParams& p, bool vec, size_t es, int64_t* parts) {
+  const RingPlan r = ring_plan(p.M, p.D, es, vec, true);
+  if (r.ctas > 0 && (vec || (p.ldx >= p.D && p.lddy >= p.D && p.D * es >= 16))) { *parts = r.ctas; return kNormGradRing; }
+  if (vec && norm_bwd_plan(p.D, es, p.w_f32).stages > 0) { *parts = std::min<int64_t>(p.M, 148); return kNormGradLong; }
+  *parts = norm_wide_blocks(p.M, p.D);
+  return kNormGradWide;
 }
 
 template <typename T, bool BWD>
 int launch_norm(const dc::NormParams& p, bool vec, cudaStream_t st) {
   constexpr int E = 16 / sizeof(T);
+  const RingPlan n = ring_plan(p.M, p.D, sizeof(T), vec, BWD);
   if constexpr (BWD) {
-    // The window of an unaligned row must lie inside its neighbours.
-    const bool apart = p.ldx >= p.D && p.lddy >= p.D && p.D * sizeof(T) >= 16;
-    if (p.D <= kNormRing && (vec || apart)) return vec ? launch_ring_rows<T, E, true>(p, st) : launch_ring_rows<T, 1, true>(p, st);
-    dc::norm_dx_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
-    DC_CHECK_LAUNCH("layer_norm_grad launch");
-    if (p.part_w != nullptr) {
-      const int64_t blocks = norm_bwd_ctas(p.M, p.D);
-      dc::norm_dw_wide_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(p.D, 256)), static_cast<unsigned>(blocks)), 256, 0, st>>>(
-          p, static_cast<int>(ceil_div(p.M, blocks)));
+    int64_t parts;
+    switch (norm_grad_path(p, vec, sizeof(T), &parts)) {
+      case kNormGradRing: return vec ? launch_ring_rows<T, E, true>(p, n, st) : launch_ring_rows<T, 1, true>(p, n, st);
+      case kNormGradLong: return launch_norm_bwd<T>(p, norm_bwd_plan(p.D, sizeof(T), p.w_f32), st);
+      default: return vec ? launch_norm_grad_wide<T, E>(p, st) : launch_norm_grad_wide<T, 1>(p, st);
     }
   } else {
+    // Many rows of more than 256 values (or unaligned ones) through the ring: 30000 x 2048 bf16 53 us
+    // against 66 in the register kernel; 100000 x 256 39 against 33.
     const bool apart = p.ldx >= p.D && p.D * sizeof(T) >= 16;
-    const bool many = p.D <= kNormRing && p.M >= 148 * 8;
-    if (many && vec && getenv("DC_NORM_RING")) return launch_ring_rows<T, E, false>(p, st);
-    if (many && !vec && apart) return launch_ring_rows<T, 1, false>(p, st);
+    if (p.M >= 148 * 8 && n.ctas > 0) {
+      if (vec && p.D > 256) return launch_ring_rows<T, E, false>(p, n, st);
+      if (!vec && apart) return launch_ring_rows<T, 1, false>(p, n, st);
+    }
     if (!(vec ? launch_norm_reg<T, true>(p, st) : launch_norm_reg<T, false>(p, st)))
       dc::norm_fwd_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
+    DC_CHECK_LAUNCH("layer_norm launch");
+    return DC_OK;
   }
-  DC_CHECK_LAUNCH("layer_norm launch");
-  return DC_OK;
 }
 
 template <bool BWD>
@@ -544,7 +609,9 @@ int dc_layer_norm(const void* x, int64_t ldx, const void* w, const void* b, int 
 
 int dc_layer_norm_grad_workspace(int64_t M, int64_t D, size_t* bytes) {
   if (M < 0 || D <= 0 || bytes == nullptr) return fail("layer_norm_grad: bad shape M=%lld D=%lld", (long long)M, (long long)D);
-  *bytes = static_cast<size_t>(norm_bwd_ctas(M, D)) * round_up(D, 4) * 2 * sizeof(float);
+  // Enough for every path: up to six persistent CTAs per SM, or the wide kernel's row blocks.
+  *bytes = static_cast<size_t>(std::max<int64_t>(norm_wide_blocks(M, D), std::min<int64_t>(M, 6 * 148))) * round_up(D, 4) * 2 *
+           sizeof(float);
   return DC_OK;
 }
 
@@ -570,15 +637,17 @@ int dc_layer_norm_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx,
   p.x = x; p.ldx = ldx; p.dy = dy; p.lddy = lddy; p.w = w; p.out = dx; p.ldo = lddx;
   p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
   p.ldp = round_up(D, 4);
-  const int64_t ctas = norm_bwd_ctas(M, D);
-  if (dw != nullptr) { p.part_w = static_cast<float*>(workspace); p.part_b = p.part_w + ctas * p.ldp; }
   p.M = M; p.D = static_cast<int>(D); p.w_f32 = w_dtype == DC_DTYPE_F32;
   const int64_t e = 16 / static_cast<int64_t>(es);
   const bool vec = D % e == 0 && ldx % e == 0 && lddy % e == 0 && lddx % e == 0 && aligned(x, 16) && aligned(dy, 16) &&
                    aligned(dx, 16) && aligned(w, 16);
+  int64_t parts;
+  norm_grad_path(p, vec, es, &parts);
+  p.parts = static_cast<int>(parts);
+  if (dw != nullptr) { p.part_w = static_cast<float*>(workspace); p.part_b = p.part_w + p.parts * p.ldp; }
   const cudaStream_t st = as_stream(stream);
   if ((r = dispatch_norm<true>(p, dtype, vec, st))) return r;
-  if (dw != nullptr) return colsum_finish(p.part_w, p.part_b, p.ldp, ctas, D, dw, db, w_dtype, st);
+  if (dw != nullptr) return colsum_finish(p.part_w, p.part_b, p.ldp, p.parts, D, dw, db, w_dtype, st);
   return DC_OK;
 }
 
@@ -643,7 +712,9 @@ int launch_embed_sum(const dc::EmbedSumParams& p, int64_t chunks, cudaStream_t s
   if (grid.y > 65535) return fail("embedding_grad: rows of %d values are too wide", p.D);
   dc::embed_sum_kernel<T, E><<<grid, dc::kSumThreads, 0, st>>>(p);
   DC_CHECK_LAUNCH("embedding_grad sum launch");
-  dc::embed_join_kernel<T, E><<<grid, dc::kSumThreads * dc::kJoinGroups, 0, st>>>(p);
+  if (chunks <= 2) return DC_OK;             // no run can go on behind the chunk after its first
+  const dim3 join(static_cast<unsigned>(ceil_div(chunks, dc::kJoinChunks)), grid.y);
+  dc::embed_join_kernel<T, E><<<join, dc::kSumThreads * dc::kJoinGroups, 0, st>>>(p);
   DC_CHECK_LAUNCH("embedding_grad join launch");
   return DC_OK;
 }

@@ -9,8 +9,9 @@
 
 namespace dc {
 
-constexpr int kGradThreads = 128;
-constexpr int kGradCols = 4 * kGradThreads;     // columns per block
+constexpr int kGradX = 64;                      // threads across the columns of a CTA, 8 columns each
+constexpr int kGradY = 4;                       // row groups of a CTA
+constexpr int kGradCols = 8 * kGradX;
 
 struct ActGradParams {
   const uint16_t* dy;       // [M, N], row stride lddy
@@ -23,70 +24,108 @@ struct ActGradParams {
   int64_t lddz;
   float* part0;             // [row blocks, ldp] column sums of dz before rounding, or null
   float* part1;
-  int64_t ldp;
+  int64_t ldp;              // a multiple of 8
   int64_t M, N;
   int rows_per_block;
   int act, bf16, dy_vec;
 };
 
-// dz = dy act'(z); gated: dg = dy u act'(g), du = dy act(g). One thread per 4 columns, a row
-// block per CTA. Bound by HBM: 2 B (dy) + 4 or 8 B (z) read and 2 or 4 B written per element.
-template <bool GATED>
-__global__ void __launch_bounds__(kGradThreads)
+// Eight 16-bit values (one vector access when `vec`), zero past `n` of them.
+__device__ __forceinline__ uint4 load8_bits(const uint16_t* src, int n, bool vec) {
+  if (vec && n >= 8) return __ldg(reinterpret_cast<const uint4*>(src));
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = i < n ? __ldg(src + i) : 0u;
+  return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+}
+__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8], int bf16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = h_to_f(w[i] & 0xFFFFu, bf16); f[2 * i + 1] = h_to_f(w[i] >> 16, bf16); }
+}
+__device__ __forceinline__ uint4 pack8(const float (&f)[8], int bf16) {
+  return make_uint4(pack_h2(f[0], f[1], bf16), pack_h2(f[2], f[3], bf16), pack_h2(f[4], f[5], bf16), pack_h2(f[6], f[7], bf16));
+}
+
+// FORM 0: column sums of dy alone; 1: dz = dy act'(z); 2 (gated): dg = dy u act'(g), du = dy act(g).
+// A thread owns 8 columns, a CTA 512 columns of a row block, its four row groups every fourth row.
+// Bound by HBM: 2 B (dy) + 4 or 8 B (z) read and 2 or 4 B written per element; kAhead rows per thread
+// are loaded ahead of their arithmetic.
+template <int FORM>
+__global__ void __launch_bounds__(kGradX * kGradY)
 act_grad_kernel(const ActGradParams p) {
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kGradCols + threadIdx.x * 4;
-  const int n = static_cast<int>(min(static_cast<int64_t>(4), p.N - col));
-  if (n <= 0) return;
+  constexpr int kAhead = FORM == 0 ? 8 : FORM == 1 ? 3 : 2;
+  __shared__ float red[FORM == 2 ? 2 : 1][kGradY][kGradCols];
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kGradCols + threadIdx.x * 8;
+  const int n = static_cast<int>(min(static_cast<int64_t>(8), p.N - col));      // may be <= 0
+  const bool z_hi = n > 4;                  // z rows are padded to 4 values
   const int64_t r0 = static_cast<int64_t>(blockIdx.y) * p.rows_per_block;
   const int64_t r1 = min(p.M, r0 + p.rows_per_block);
-  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-  constexpr int kAhead = 4;                 // rows whose loads are in flight at once
-  for (int64_t rb = r0; rb < r1; rb += kAhead) {
-    float4 d4[kAhead], z4[kAhead], u4[kAhead];
+  float s0[8], s1[8];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int64_t r = rb + k;
-      if (r < r1) {
-        d4[k] = load4(p.dy + r * p.lddy + col, n, p.dy_vec, p.bf16);
-        if (p.z0 != nullptr) z4[k] = *reinterpret_cast<const float4*>(p.z0 + r * p.ldz + col);
-        if (GATED) u4[k] = *reinterpret_cast<const float4*>(p.z1 + r * p.ldz + col);
-      }
-    }
+  for (int j = 0; j < 8; ++j) { s0[j] = 0.f; s1[j] = 0.f; }
+  if (n > 0) {
+    for (int64_t rb = r0 + threadIdx.y; rb < r1; rb += kGradY * kAhead) {
+      uint4 dv[kAhead];
+      float z[kAhead][8], u[kAhead][8];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int64_t r = rb + k;
-      if (r >= r1) break;
-      float d[4] = {d4[k].x, d4[k].y, d4[k].z, d4[k].w};
-      if (p.z0 != nullptr) {
-        const float z[4] = {z4[k].x, z4[k].y, z4[k].z, z4[k].w};
-        float e[4];
-        if (GATED) {
-          const float u[4] = {u4[k].x, u4[k].y, u4[k].z, u4[k].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 a = act_value_grad(z[j], p.act);
-            e[j] = d[j] * a.x;
-            d[j] *= u[j] * a.y;
+      for (int k = 0; k < kAhead; ++k) {
+        const int64_t r = rb + k * kGradY;
+        if (r < r1) {
+          dv[k] = load8_bits(p.dy + r * p.lddy + col, n, p.dy_vec);
+          if (FORM >= 1) {
+            const float4* q = reinterpret_cast<const float4*>(p.z0 + r * p.ldz + col);
+            const float4 a = q[0], b = z_hi ? q[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+            z[k][0] = a.x; z[k][1] = a.y; z[k][2] = a.z; z[k][3] = a.w; z[k][4] = b.x; z[k][5] = b.y; z[k][6] = b.z; z[k][7] = b.w;
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) d[j] *= act_value_grad(z[j], p.act).y;
-        }
-        // rows of dz are padded to 8 values, so a whole unit may be written
-        *reinterpret_cast<uint2*>(p.dz0 + r * p.lddz + col) = make_uint2(pack_h2(d[0], d[1], p.bf16), pack_h2(d[2], d[3], p.bf16));
-        if (GATED) {
-          *reinterpret_cast<uint2*>(p.dz1 + r * p.lddz + col) = make_uint2(pack_h2(e[0], e[1], p.bf16), pack_h2(e[2], e[3], p.bf16));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s1[j] += e[j];
+          if (FORM == 2) {
+            const float4* q = reinterpret_cast<const float4*>(p.z1 + r * p.ldz + col);
+            const float4 a = q[0], b = z_hi ? q[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+            u[k][0] = a.x; u[k][1] = a.y; u[k][2] = a.z; u[k][3] = a.w; u[k][4] = b.x; u[k][5] = b.y; u[k][6] = b.z; u[k][7] = b.w;
+          }
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s0[j] += d[j];
+      for (int k = 0; k < kAhead; ++k) {
+        const int64_t r = rb + k * kGradY;
+        if (r >= r1) break;
+        float d[8];
+        unpack8(dv[k], d, p.bf16);
+        if (FORM == 1) {
+          act_grads(z[k], p.act, [&](int j, float, float da) { d[j] *= da; });
+          *reinterpret_cast<uint4*>(p.dz0 + r * p.lddz + col) = pack8(d, p.bf16);     // rows are padded to 8
+        }
+        if (FORM == 2) {
+          float e[8];
+          act_grads(z[k], p.act, [&](int j, float a, float da) { e[j] = d[j] * a; d[j] *= u[k][j] * da; });
+          *reinterpret_cast<uint4*>(p.dz0 + r * p.lddz + col) = pack8(d, p.bf16);
+          *reinterpret_cast<uint4*>(p.dz1 + r * p.lddz + col) = pack8(e, p.bf16);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s1[j] += e[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s0[j] += d[j];
+      }
     }
   }
-  if (p.part0 != nullptr) {
-    *reinterpret_cast<float4*>(p.part0 + blockIdx.y * p.ldp + col) = make_float4(s0[0], s0[1], s0[2], s0[3]);
-    if (GATED) *reinterpret_cast<float4*>(p.part1 + blockIdx.y * p.ldp + col) = make_float4(s1[0], s1[1], s1[2], s1[3]);
+  if (p.part0 == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    red[0][threadIdx.y][threadIdx.x * 8 + j] = s0[j];
+    if (FORM == 2) red[FORM == 2][threadIdx.y][threadIdx.x * 8 + j] = s1[j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.y * kGradX + threadIdx.x; i < kGradCols; i += kGradX * kGradY) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * kGradCols + i;
+    if (c >= p.N) continue;
+    float a = red[0][0][i], b = FORM == 2 ? red[FORM == 2][0][i] : 0.f;
+#pragma unroll
+    for (int y = 1; y < kGradY; ++y) {
+      a += red[0][y][i];
+      if (FORM == 2) b += red[FORM == 2][y][i];
+    }
+    p.part0[blockIdx.y * p.ldp + c] = a;
+    if (FORM == 2) p.part1[blockIdx.y * p.ldp + c] = b;
   }
 }
 
