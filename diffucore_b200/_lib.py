@@ -133,6 +133,25 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+_ext = None
+
+
+def text_ext():
+    """The torch binding of the text operators (``_text_ext.so``, loaded once per process)."""
+    global _ext
+    if _ext is None:
+        load()
+        try:
+            import torch  # noqa: F401  its libraries first
+
+            from . import _text_ext
+        except ImportError as e:
+            raise NativeLibraryError("_text_ext.so is not built or does not fit this torch; run "
+                                     f"`python -m diffucore_b200.build` ({e})") from e
+        _ext = _text_ext
+    return _ext
+
+
 def check(status: int) -> None:
     if status != DC_OK:
         msg = load().dc_last_error().decode(errors="replace")

@@ -1,5 +1,8 @@
 """Builds the sm_100a shared library ``libdiffucore_b200.so`` in-tree with nvcc.
 
+Two files: ``libdiffucore_b200.so``, the C-ABI library, and ``_text_ext.so``, the torch binding of its
+text operators (g++ against the installed torch's headers).
+
 The library has one translation unit per group of entry points (``csrc/dc_api.cu``: the W8A8 and
 INT8 attention path, ``csrc/text_api.cu``: the text operators; each includes its kernel headers),
 compiled side by side for ``sm_100a`` only and linked with the CUDA runtime statically, so the
@@ -21,6 +24,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "libdiffucore_b200.so"
+EXT = PKG / "_text_ext.so"
 OBJECTS = PKG / "_build"
 
 NVCC_FLAGS = [
@@ -96,6 +100,38 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
+def build_ext(force: bool = False, verbose: bool = False) -> Path:
+    """Compile ``csrc/text_ext.cpp`` against the installed torch into ``_text_ext.so``, linked to the
+    library beside it, unless it is up to date."""
+    src = CSRC / "text_ext.cpp"
+    if not force and EXT.exists():
+        built = EXT.stat().st_mtime
+        if all(p.stat().st_mtime <= built for p in _includes(src.resolve(), set())):
+            return EXT
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    lib_dir = Path(torch.__file__).resolve().parent / "lib"
+    cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    includes = [*cpp_extension.include_paths(), str(cuda / "include"), sysconfig.get_paths()["include"]]
+    tmp = EXT.with_suffix(".so.tmp")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *(f"-isystem{p}" for p in includes), str(src), "-o", str(tmp),
+          f"-L{PKG}", "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN", f"-L{lib_dir}", f"-Wl,-rpath,{lib_dir}",
+          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"], verbose)
+    os.replace(tmp, EXT)
+    return EXT
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Everything native: the library, then the binding that links to it."""
+    lib = build_library(force, verbose)
+    build_ext(force, verbose)
+    return lib
+
+
 if __name__ == "__main__":
     force = "--force" in sys.argv
-    print(build_library(force=force, verbose=True))
+    print(build(force=force, verbose=True))

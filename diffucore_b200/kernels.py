@@ -8,7 +8,6 @@ on sm_100 CUDA tensors only and raise for anything else; there is no CPU impleme
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 
 import torch
@@ -449,321 +448,78 @@ def selftest_exp2(x: torch.Tensor):
 
 
 # ─── text operators (dc_linear, dc_gated_linear, dc_layer_norm, dc_embedding and gradients) ──
+#
+# The single steps of diffucore_b200.text on flat tensors, through its native binding.
 
-_ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU,
-         "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
-
-
-# The current stream's handle without building a Stream object (1.3 us of a 10 us call).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+ACTIVATIONS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU,
+               "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
 
 
-def _launch(fn, dev: int, *args) -> None:
-    """Call a C entry point on device ``dev`` with its current stream as the last argument."""
-    if dev == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev))
-    if status:
-        _lib.check(status)
-
-
-def _addr(t: torch.Tensor | None) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
-def _act_code(act) -> int:
+def act_code(act: str | None) -> int:
     try:
-        return _ACTS[act]
+        return ACTIVATIONS[act]
     except KeyError:
-        raise ValueError(f"unknown activation {act!r}; choose from {sorted(k for k in _ACTS if k)}") from None
-
-
-_HALF = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
-
-
-def _check_text(what: str, dtypes, lead: torch.Tensor, *others: tuple) -> tuple[int, int]:
-    """(dtype code, device index) of ``lead``, a CUDA tensor of one of ``dtypes``; the ``others``, pairs
-    of a name and a tensor or None, must share both."""
-    dt, dev = lead.dtype, lead.get_device()
-    code = dtypes.get(dt)
-    if dev < 0 or code is None:
-        _require_cuda(lead)
-        raise TypeError(f"{what}: unsupported dtype {dt}")
-    for name, t in others:
-        if t is not None and (t.dtype is not dt or t.get_device() != dev):
-            raise TypeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {dt} on {lead.device}")
-    return code, dev
-
-
-def _tile_loadable(t: torch.Tensor) -> bool:
-    """Whether a TMA tile load takes the rows of ``t`` [R, C]: unit inner stride, 16-byte aligned rows
-    that do not overlap."""
-    (r, c), (s0, s1) = t.shape, t.stride()
-    return s1 == 1 and t.data_ptr() % 16 == 0 and (r == 1 or (s0 % 8 == 0 and s0 >= c))
+        raise ValueError(f"unknown activation {act!r}; choose from {sorted(k for k in ACTIVATIONS if k)}") from None
 
 
 def matrix_operand(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [R, C] itself when :func:`_tile_loadable`, else a copy with padded rows."""
-    if _tile_loadable(t):
-        return t
-    r, c = t.shape
-    return t.new_empty(r, (c + 7) & ~7)[:, :c].copy_(t)
-
-
-ROWDOT_MAX = 8      # rows of x up to which the few-row kernel always runs
-
-
-def _projection_operand(t: torch.Tensor, rows: int) -> torch.Tensor:
-    """A forward operand for ``rows`` rows of x: few rows go to a kernel that reads any layout
-    in place; DC_HGEMM_PAIR forces the tensor-core kernels."""
-    if _tile_loadable(t):
-        return t
-    (r, c), (s0, s1) = t.shape, t.stride()
-    if rows <= ROWDOT_MAX and s1 == 1 and (r == 1 or s0 >= c) and os.environ.get("DC_HGEMM_PAIR") not in ("0", "1"):
-        return t
-    return matrix_operand(t)
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Leading dimension of a matrix operand (any multiple of 8 will do for a single row)."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) & ~7
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [R, C] with unit inner stride."""
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-
-
-def _ld_rows(t: torch.Tensor) -> int:
-    """Row stride of a tensor read or written row by row (one row: its width)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _vector(what: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
-    if t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{what}: {name} must have shape ({n},), got {tuple(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
+    """``t`` [R, C] itself when a TMA tile load takes its rows (unit inner stride, 16-byte aligned rows
+    that do not overlap), else a copy with padded rows."""
+    return _lib.text_ext().matrix_operand(t)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None,
            residual: torch.Tensor | None = None, keep_z: bool = False):
     """``(y, z)``: ``y = act(z) + residual``, ``z = x @ w.T + bias`` for 16-bit ``x`` [M, K] and ``w``
     [N, K] (``dc_linear``). ``z`` is the fp32 pre-activation (rows padded to 4) when ``keep_z``."""
-    dt, dev = _check_text("linear", _HALF, x, ("w", w), ("bias", bias), ("residual", residual))
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
-        raise ValueError(f"linear: x {tuple(x.shape)} does not match w {tuple(w.shape)}")
-    (M, K), N = x.shape, w.shape[0]
-    code = _act_code(act)
-    bp = rp = ldr = zp = ldz = 0
-    if bias is not None:
-        bias = _vector("linear", "bias", bias, N)
-        bp = bias.data_ptr()
-    if residual is not None:
-        if residual.shape != (M, N):
-            raise ValueError(f"linear: residual must have shape {(M, N)}, got {tuple(residual.shape)}")
-        residual = _rows(residual)
-        rp, ldr = residual.data_ptr(), residual.stride(0)
-    x, w = _projection_operand(x, M), _projection_operand(w, M)
-    y = x.new_empty((M, N))
-    z = None
-    if keep_z:
-        ldz = (N + 3) & ~3
-        z = x.new_empty((M, ldz), dtype=torch.float32)
-        zp = z.data_ptr()
-    _launch(_lib.load().dc_linear, dev, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), bp, rp, ldr, y.data_ptr(), N, zp,
-            ldz, dt, M, N, K, code)
-    return y, z
+    return _lib.text_ext().linear_raw(x, w, bias, act_code(act), residual, keep_z)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
                  b_up: torch.Tensor | None = None, act: str | None = "silu", keep_z: bool = False):
     """``(h, z_gate, z_up)``: ``h = act(z_gate) * z_up`` of the two projections of ``x`` [M, K] by
     ``w_gate``, ``w_up`` [N, K] (``dc_gated_linear``); the fp32 pre-activations when ``keep_z``."""
-    dt, dev = _check_text("gated_linear", _HALF, x, ("w_gate", w_gate), ("w_up", w_up), ("b_gate", b_gate),
-                          ("b_up", b_up))
-    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or x.shape[1] != w_gate.shape[1]:
-        raise ValueError(f"gated_linear: shapes of x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)} and w_up "
-                         f"{tuple(w_up.shape)} do not match")
-    (M, K), N = x.shape, w_gate.shape[0]
-    code = _act_code(act)
-    if b_gate is not None:
-        b_gate = _vector("gated_linear", "b_gate", b_gate, N)
-    if b_up is not None:
-        b_up = _vector("gated_linear", "b_up", b_up, N)
-    x, w_gate, w_up = (_projection_operand(t, M) for t in (x, w_gate, w_up))
-    h = x.new_empty((M, N))
-    ldz = (N + 3) & ~3
-    zg, zu = x.new_empty((2, M, ldz), dtype=torch.float32).unbind(0) if keep_z else (None, None)
-    _launch(_lib.load().dc_gated_linear, dev, x.data_ptr(), _ld(x), w_gate.data_ptr(), _ld(w_gate), w_up.data_ptr(),
-            _ld(w_up), _addr(b_gate), _addr(b_up), h.data_ptr(), N, _addr(zg), _addr(zu), ldz, dt, M, N, K, code)
-    return h, zg, zu
-
-
-@functools.lru_cache(maxsize=512)
-def _workspace_bytes(entry: str, *shape: int) -> int:
-    """Workspace size of a gradient (a function of the shape alone)."""
-    n = ctypes.c_size_t(0)
-    _lib.check(getattr(_lib.load(), entry)(*shape, ctypes.byref(n)))
-    return n.value
-
-
-def _workspace(t: torch.Tensor, nbytes: int) -> torch.Tensor:
-    return t.new_empty((nbytes,), dtype=torch.uint8)
+    return _lib.text_ext().gated_linear_raw(x, w_gate, w_up, b_gate, b_up, act_code(act), keep_z)
 
 
 def act_grad(dy: torch.Tensor, z: torch.Tensor | None, z1: torch.Tensor | None, act: str | None,
              bias_grad: bool = False, bias_grad1: bool = False):
     """``(dz, dz1, db, db1)`` from ``dy`` [M, N] and the kept pre-activations (``dc_act_grad``); with
     ``z`` None, ``dz`` is ``dy``. The ``dz`` rows are padded to matrix-operand alignment."""
-    M, N = dy.shape
-    if z is None and not bias_grad:
-        return dy, None, None, None
-    dy = _rows(dy)
-    if M > 1 and dy.stride(0) < N:
-        dy = dy.contiguous()
-    dz = dz1 = db = db1 = ws = None
-    nbytes = 0
-    lddz = (N + 7) & ~7
-    if z is not None:
-        dz = dy.new_empty(M, lddz)[:, :N]
-        if z1 is not None:
-            dz1 = dy.new_empty(M, lddz)[:, :N]
-    if bias_grad or bias_grad1:
-        db = dy.new_empty(N)
-        db1 = dy.new_empty(N) if bias_grad1 else None
-        nbytes = _workspace_bytes("dc_act_grad_workspace", M, N)
-        ws = _workspace(dy, nbytes)
-    _launch(_lib.load().dc_act_grad, dy.get_device(), dy.data_ptr(), _ld_rows(dy), _addr(z), _addr(z1),
-            0 if z is None else z.stride(0), _addr(dz), _addr(dz1), lddz, _addr(db), _addr(db1), _addr(ws), nbytes,
-            _HALF[dy.dtype], M, N, _act_code(act))
-    return (dy if z is None else dz), dz1, db, db1
+    return _lib.text_ext().act_grad_raw(dy, z, z1, act_code(act), bias_grad, bias_grad1)
 
 
 def linear_dx(dz: torch.Tensor, w: torch.Tensor, dz1: torch.Tensor | None = None,
               w1: torch.Tensor | None = None) -> torch.Tensor:
     """``dz @ w`` (``+ dz1 @ w1``) for ``dz`` [M, N], ``w`` [N, K] (``dc_linear_dx``)."""
-    dz, w = matrix_operand(dz), matrix_operand(w)
-    if w1 is not None:
-        w1 = matrix_operand(w1)
-    (M, N), K = dz.shape, w.shape[1]
-    dx = dz.new_empty(M, K)
-    _launch(_lib.load().dc_linear_dx, dz.get_device(), dz.data_ptr(), _addr(dz1), _ld(dz), w.data_ptr(), _ld(w),
-            _addr(w1), 0 if w1 is None else _ld(w1), dx.data_ptr(), K, _DTYPE[dz.dtype], M, N, K)
-    return dx
+    return _lib.text_ext().linear_dx_raw(dz, w, dz1, w1)
 
 
 def linear_dw(dz: torch.Tensor, x: torch.Tensor, dz1: torch.Tensor | None = None):
-    """``dz.T @ x`` (and ``dz1.T @ x``) for ``dz`` [M, N], ``x`` [M, K] (``dc_linear_dw``):
-    ``(dw, dw1 or None)``."""
-    dz, x = matrix_operand(dz), matrix_operand(x)
-    (M, N), K = dz.shape, x.shape[1]
-    dw = x.new_empty(N, K)
-    dw1 = x.new_empty(N, K) if dz1 is not None else None
-    _launch(_lib.load().dc_linear_dw, dz.get_device(), dz.data_ptr(), _addr(dz1), _ld(dz), x.data_ptr(), _ld(x),
-            dw.data_ptr(), _addr(dw1), K, _DTYPE[dz.dtype], M, N, K)
-    return dw, dw1
+    """``(dz.T @ x, dz1.T @ x or None)`` for ``dz`` [M, N], ``x`` [M, K] (``dc_linear_dw``)."""
+    return _lib.text_ext().linear_dw_raw(dz, x, dz1)
 
 
 def layer_norm(x: torch.Tensor, w: torch.Tensor | None, b: torch.Tensor | None, eps: float, keep_stats: bool = False):
     """``(y, mean, rstd)`` of the rows of ``x`` [M, D] (``dc_layer_norm``); ``w`` and ``b`` [D] in x's
-    type or fp32. ``mean`` and ``rstd`` are fp32 [M] when ``keep_stats``."""
-    dt, dev = _check_text("layer_norm", _DTYPE, x)
-    M, D = x.shape
-    w, b, wcode = _norm_affine("layer_norm", x, w, b)
-    x = _rows(x)
-    y = x.new_empty((M, D))
-    stats, base = None, 0
-    if keep_stats:
-        stats = x.new_empty((2, M), dtype=torch.float32)
-        base = stats.data_ptr()
-    _launch(_lib.load().dc_layer_norm, dev, x.data_ptr(), _ld_rows(x), _addr(w), _addr(b), wcode, y.data_ptr(), D,
-            base, base + 4 * M if base else 0, dt, M, D, eps)
-    return (y, None, None) if stats is None else (y, stats[0], stats[1])
-
-
-def _norm_affine(what: str, x: torch.Tensor, w, b):
-    """The affine vectors in one type the kernels take, and its code."""
-    D, dt, dev = x.shape[-1], x.dtype, x.get_device()
-    kind = None
-    for name, t in (("weight", w), ("bias", b)):
-        if t is not None:
-            if t.get_device() != dev or (t.dtype is not dt and t.dtype is not torch.float32):
-                raise TypeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {dt} or fp32 on {x.device}")
-            if t.dim() != 1 or t.shape[0] != D:
-                raise ValueError(f"{what}: {name} must have shape ({D},), got {tuple(t.shape)}")
-            kind = t.dtype if kind is None or kind is t.dtype else torch.float32
-    if kind is None:
-        return w, b, _DTYPE[dt]
-    if w is not None and (w.dtype is not kind or not w.is_contiguous()):
-        w = w.to(kind).contiguous()
-    if b is not None and (b.dtype is not kind or not b.is_contiguous()):
-        b = b.to(kind).contiguous()
-    return w, b, _DTYPE[kind]
+    type or fp32. ``mean`` and ``rstd`` are fp32 [M] when ``keep_stats``, else None."""
+    return _lib.text_ext().layer_norm_raw(x, w, b, eps, keep_stats)
 
 
 def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor | None, mean: torch.Tensor, rstd: torch.Tensor,
                     weight_grad: bool = True, bias_grad: bool = True, dtype: torch.dtype | None = None):
     """``(dx, dw, db)`` of :func:`layer_norm` (``dc_layer_norm_grad``). ``dw`` and ``db`` come in
     ``dtype`` (x's type or fp32; default: ``w``'s, else x's)."""
-    dt, dev = _check_text("layer_norm_grad", _DTYPE, dy, ("x", x))
-    M, D = x.shape
-    dtype = dtype or (x.dtype if w is None else w.dtype)
-    if w is not None and (w.dtype is not dtype or not w.is_contiguous()):
-        w = w.to(dtype).contiguous()
-    dy, x = _rows(dy), _rows(x)
-    dx = x.new_empty((M, D))
-    dw = db = ws = None
-    nbytes = 0
-    if weight_grad or bias_grad:
-        dw = x.new_empty((D,), dtype=dtype)
-        db = x.new_empty((D,), dtype=dtype) if bias_grad else None
-        nbytes = _workspace_bytes("dc_layer_norm_grad_workspace", M, D)
-        ws = _workspace(x, nbytes)
-    _launch(_lib.load().dc_layer_norm_grad, dev, dy.data_ptr(), _ld_rows(dy), x.data_ptr(), _ld_rows(x), _addr(w),
-            _DTYPE[dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D, _addr(dw), _addr(db), _addr(ws),
-            nbytes, dt, M, D)
-    return dx, dw if weight_grad else None, db
-
-
-def _check_ids(what: str, ids: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
-    """Flat contiguous ids."""
-    if ids.dtype not in (torch.int64, torch.int32) or ids.get_device() != like.get_device():
-        raise TypeError(f"{what}: ids must be int64 or int32 on {like.device}, got {ids.dtype} on {ids.device}")
-    if ids.dim() != 1:
-        ids = ids.reshape(-1)
-    return ids if ids.is_contiguous() else ids.contiguous()
+    return _lib.text_ext().layer_norm_grad_raw(dy, x, w, mean, rstd, weight_grad, bias_grad,
+                                               dtype or (x.dtype if w is None else w.dtype))
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """``scale * table[ids]`` [T, D] for flat ``ids`` and ``table`` [V, D] (``dc_embedding``)."""
-    dt, dev = _check_text("embedding", _DTYPE, table)
-    ids = _check_ids("embedding", ids, table)
-    V, D = table.shape
-    table = _rows(table)
-    if V > 1 and table.stride(0) < D:
-        table = table.contiguous()
-    T = ids.shape[0]
-    out = table.new_empty((T, D))
-    _launch(_lib.load().dc_embedding, dev, ids.data_ptr(), ids.dtype is torch.int64, T, table.data_ptr(),
-            _ld_rows(table), V, D, scale, out.data_ptr(), D, dt)
-    return out
+    return _lib.text_ext().embedding_raw(ids, table, scale)
 
 
 def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, V: int, scale: float = 1.0,
                    padding_idx: int = -1) -> torch.Tensor:
     """The dense gradient [V, D] of :func:`embedding`'s table (``dc_embedding_grad``)."""
-    dt, dev = _check_text("embedding_grad", _DTYPE, dy)
-    ids = _check_ids("embedding_grad", ids, dy)
-    T, D = dy.shape
-    if ids.shape[0] != T:
-        raise ValueError(f"embedding_grad: {ids.shape[0]} ids for {T} rows")
-    dy = _rows(dy)
-    nbytes = _workspace_bytes("dc_embedding_grad_workspace", T, V, D)
-    ws = _workspace(dy, nbytes)
-    out = dy.new_empty((V, D))
-    _launch(_lib.load().dc_embedding_grad, dev, dy.data_ptr(), _ld_rows(dy), ids.data_ptr(), ids.dtype is torch.int64,
-            T, V, D, padding_idx, scale, out.data_ptr(), ws.data_ptr(), nbytes, dt)
-    return out
+    return _lib.text_ext().embedding_grad_raw(dy, ids, V, scale, padding_idx)

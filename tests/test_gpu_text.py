@@ -434,3 +434,25 @@ def test_refusals():
         text.embedding(torch.zeros(3, dtype=torch.long, device=DEV), w, padding_idx=8)
     with pytest.raises(ValueError, match="rows"):
         kernels.embedding_grad(x, torch.zeros(3, dtype=torch.long, device=DEV), 8)
+
+
+def test_create_graph_gives_gradients_that_cannot_be_differentiated_again():
+    g = gen("twice")
+    x, w = rand(g, 6, 16).requires_grad_(), rand(g, 8, 16).requires_grad_()
+    plain, = torch.autograd.grad(text.linear(x, w, activation="silu").sum(), x)
+    dx, = torch.autograd.grad(text.linear(x, w, activation="silu").sum(), x, create_graph=True)
+    assert torch.equal(dx.detach(), plain)
+    with pytest.raises(RuntimeError):                      # no path back to x
+        torch.autograd.grad(dx.sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        dx.sum().backward()
+
+
+def test_operand_changed_in_place_is_noticed():
+    g = gen("in place")
+    x, w = rand(g, 6, 16).requires_grad_(), rand(g, 8, 16).requires_grad_()
+    y = text.linear(x, w)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()

@@ -105,11 +105,11 @@ def test_functions_refuse_cpu_tensors_and_bad_shapes():
 
 def test_matrix_operand_pads_only_what_a_tile_load_cannot_take():
     t = torch.randn(6, 24).to(torch.bfloat16)
-    assert kernels.matrix_operand(t) is t
+    assert kernels.matrix_operand(t).data_ptr() == t.data_ptr()
     assert kernels.matrix_operand(t[:, :20]).data_ptr() == t.data_ptr()      # rows stay 48 bytes apart
     for v in (t[:, 1:], torch.randn(5, 21).to(torch.bfloat16), t.t(), t[:1].expand(4, 24), t[:, :1]):
         m = kernels.matrix_operand(v)
         assert torch.equal(m, v) and m.stride(0) % 8 == 0 and m.data_ptr() % 16 == 0 and m.stride(1) == 1
         assert m.stride(0) >= m.shape[1]
     one = torch.randn(3, 17).to(torch.bfloat16)[:1]
-    assert kernels.matrix_operand(one) is one and kernels._ld(one) == 24     # one row: any pitch
+    assert kernels.matrix_operand(one).data_ptr() == one.data_ptr()          # one row: any pitch
