@@ -134,7 +134,7 @@ int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const 
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(dc::kHThreads);
+  cfg.blockDim = dim3(pair ? dc::kPairThreads : dc::kHThreads);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
