@@ -43,6 +43,7 @@ template <typename T, int E>
 __global__ void __launch_bounds__(256)
 embed_fwd_kernel(const EmbedIds ids, const T* __restrict__ table, int64_t ldt, T* __restrict__ out, int64_t ldo,
                  int D, float scale) {
+  pdl_enter();
   const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if (t >= ids.T) return;
   const int64_t id = id_at(ids, t);
@@ -92,6 +93,7 @@ constexpr int kRankWarps = 8;
 __global__ void __launch_bounds__(32 * kRankWarps)
 embed_rank_kernel(const EmbedIds ids, uint32_t* __restrict__ skey, uint32_t* __restrict__ sidx, int ctas,
                   const FillSlice fill) {
+  pdl_enter();
   if (static_cast<int>(blockIdx.x) >= ctas) {
     fill_slice(fill, static_cast<int>(blockIdx.x) - ctas);
     return;
@@ -134,6 +136,7 @@ template <bool FIRST>
 __global__ void __launch_bounds__(32 * kRadixWarps)
 radix_hist_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, uint32_t* __restrict__ hist, int shift,
                   int bits, int tiles, const FillSlice fill) {
+  pdl_enter();
   if (static_cast<int>(blockIdx.x) >= tiles) {
     fill_slice(fill, static_cast<int>(blockIdx.x) - tiles);
     return;
@@ -160,6 +163,7 @@ __global__ void __launch_bounds__(32 * kRadixWarps)
 radix_scatter_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ idx,
                      const uint32_t* __restrict__ hist, uint32_t* __restrict__ keys_out,
                      uint32_t* __restrict__ idx_out, int shift, int bits, int tiles, const FillSlice fill) {
+  pdl_enter();
   if (static_cast<int>(blockIdx.x) >= tiles) {
     fill_slice(fill, static_cast<int>(blockIdx.x) - tiles);
     return;
@@ -267,6 +271,7 @@ struct EmbedSumParams {
 template <typename T, int E>
 __global__ void __launch_bounds__(kSumThreads)
 embed_sum_kernel(const EmbedSumParams p) {
+  pdl_enter();
   constexpr uint32_t kNone = 0xFFFFFFFFu;       // never a key
   __shared__ uint32_t key[2 * kSumChunkMax + 2];
   __shared__ uint32_t idx[2 * kSumChunkMax];
@@ -339,6 +344,7 @@ constexpr int kJoinChunks = 8;
 template <typename T, int E>
 __global__ void __launch_bounds__(kSumThreads * kJoinGroups)
 embed_join_kernel(const EmbedSumParams p) {
+  pdl_enter();
   __shared__ float part[kJoinGroups][E][kSumThreads];
   __shared__ uint32_t found;
   if (threadIdx.x < 32) {

@@ -309,6 +309,7 @@ hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_const
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  pdl_enter();
   const uint32_t tmem_base = tmem_base_slot;
   volatile int* abort = &abort_flag;
 
@@ -553,6 +554,7 @@ hgemm_cluster_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_enter();
   const uint32_t tmem_base = tmem_base_slot;
   volatile int* abort = &abort_flag;
 

@@ -183,6 +183,7 @@ norm_fwd_kernel(const NormParams p) {
   constexpr int kRows = NormCta<TPR>::kThreads / TPR;
   using Unit = typename NormUnit<T, VEC>::type;
   __shared__ float2 red[2 * (TPR / 32)];
+  pdl_enter();
   int turn = 0;
   const int t = threadIdx.x % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
@@ -280,6 +281,7 @@ norm_ring_kernel(const NormParams p) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], kWarps); }
     fence_barrier_init();
   }
+  pdl_enter();
   __syncthreads();
 
   // Warp 0: the copies of a block's rows into a stage, lane r row r.
@@ -474,41 +476,43 @@ norm_ring_kernel(const NormParams p) {
       }
     }
   }
-  if (!BWD || p.part_w == nullptr) return;
-  float fw[EPT], fb[EPT];
+  if constexpr (BWD) {
+    if (p.part_w == nullptr) return;
+    float fw[EPT], fb[EPT];
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    const float2 x = split(sw[i]), y = split(sb[i]);
-    fw[2 * i] = x.x; fw[2 * i + 1] = x.y;
-    fb[2 * i] = y.x; fb[2 * i + 1] = y.y;
-  }
-  if (kRows > 1) {
-    // The CTA's row groups hold sums of the same columns: added in the order of the groups.
-    float* acc = reinterpret_cast<float*>(ring);         // no copy is under way any more
-    for (int g = 0; g < kRows; ++g) {
-      __syncthreads();
-      if (sub == g) {
+    for (int i = 0; i < kPairs; ++i) {
+      const float2 x = split(sw[i]), y = split(sb[i]);
+      fw[2 * i] = x.x; fw[2 * i + 1] = x.y;
+      fb[2 * i] = y.x; fb[2 * i + 1] = y.y;
+    }
+    if (kRows > 1) {
+      // The CTA's row groups hold sums of the same columns: added in the order of the groups.
+      float* acc = reinterpret_cast<float*>(ring);         // no copy is under way any more
+      for (int g = 0; g < kRows; ++g) {
+        __syncthreads();
+        if (sub == g) {
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-          const int k = i * TPR + t;
-          acc[k] = g == 0 ? fw[i] : acc[k] + fw[i];
-          acc[TPR * EPT + k] = g == 0 ? fb[i] : acc[TPR * EPT + k] + fb[i];
+          for (int i = 0; i < EPT; ++i) {
+            const int k = i * TPR + t;
+            acc[k] = g == 0 ? fw[i] : acc[k] + fw[i];
+            acc[TPR * EPT + k] = g == 0 ? fb[i] : acc[TPR * EPT + k] + fb[i];
+          }
         }
       }
+      __syncthreads();
+      if (sub != 0) return;
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) { fw[i] = acc[i * TPR + t]; fb[i] = acc[TPR * EPT + i * TPR + t]; }
     }
-    __syncthreads();
-    if (sub != 0) return;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) { fw[i] = acc[i * TPR + t]; fb[i] = acc[TPR * EPT + i * TPR + t]; }
-  }
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * E;
+      if (c < p.D) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * E;
-    if (c < p.D) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        p.part_w[blockIdx.x * p.ldp + c + j] = fw[i * E + j];
-        p.part_b[blockIdx.x * p.ldp + c + j] = fb[i * E + j];
+        for (int j = 0; j < E; ++j) {
+          p.part_w[blockIdx.x * p.ldp + c + j] = fw[i * E + j];
+          p.part_b[blockIdx.x * p.ldp + c + j] = fb[i * E + j];
+        }
       }
     }
   }
@@ -580,6 +584,7 @@ norm_bwd_kernel(const NormParams p) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], kWarps); }
     fence_barrier_init();
   }
+  pdl_enter();
   Affine::store(smem, p.w, units, 1.0f);
   __syncthreads();
   auto issue = [&](int stage, int64_t row) {              // thread 0
@@ -700,6 +705,7 @@ template <typename T>
 __global__ void __launch_bounds__(kNormWide)
 norm_fwd_wide_kernel(const NormParams p) {
   __shared__ float2 red[2 * (kNormWide / 32)];
+  pdl_enter();
   int turn = 0;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
@@ -724,6 +730,7 @@ template <typename T, int E>
 __global__ void __launch_bounds__(kNormWide)
 norm_dx_wide_kernel(const NormParams p) {
   __shared__ float2 red[2 * (kNormWide / 32)];
+  pdl_enter();
   int turn = 0;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
@@ -764,6 +771,7 @@ norm_dx_wide_kernel(const NormParams p) {
 template <typename T, int E>
 __global__ void __launch_bounds__(128)
 norm_dw_wide_kernel(const NormParams p, int rows_per_block) {
+  pdl_enter();
   const int c = (blockIdx.x * 128 + threadIdx.x) * E;
   if (c >= p.D) return;
   const int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows_per_block;

@@ -84,6 +84,7 @@ rowdot_kernel(const RowDotParams p) {
   constexpr int kCols = GATED ? 8 : 16;         // output columns per warp
   constexpr int kRows = 8 * NT;                 // rows of x, padded
   extern __shared__ float sums[];               // [warp][16 weight rows][kRows]
+  pdl_enter();
   const int warp = warp_id(), lane = lane_id();
   const int warps = static_cast<int>(blockDim.x) >> 5;
   const int groups = warps / p.ks;              // column groups per CTA

@@ -369,6 +369,18 @@ __device__ __forceinline__ void mma_commit_pair_both(uint64_t* bar) {
                :: "r"(smem_u32(bar)), "h"(both) : "memory");
 }
 
+// Programmatic dependent launch: a kernel launched with the attribute may start while the one before it
+// in the stream still runs, once all of that one's CTAs have called pdl_trigger() or ended. pdl_wait()
+// returns when every kernel before it is complete and its writes are visible. Each thread that
+// touches global memory calls it first; a kernel must not end without it, or the kernels after it
+// could run before the ones before it have ended.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_enter() {
+  pdl_wait();
+  pdl_trigger();
+}
+
 __device__ __forceinline__ int warp_id() { return threadIdx.x >> 5; }
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 

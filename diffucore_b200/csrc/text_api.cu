@@ -34,6 +34,27 @@ bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t elem_size(int dtype) { return dtype == DC_DTYPE_F32 ? 4 : 2; }
 
+// Every kernel of this file is launched with programmatic stream serialization (see pdl_wait), in
+// clusters of `cluster` CTAs where that is above 0.
+template <typename... P, typename... A>
+int launch(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster,
+           const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster); attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e != cudaSuccess ? cuda_fail(e, what) : DC_OK;
+}
+
 // ------------------------------------------------------------------------------ projections
 
 // An operand of the contraction as the tensor core sees it: `rows` row indices x `k` contraction
@@ -130,49 +151,27 @@ int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const 
   if (b1.p == nullptr) mb1 = mb0;
   else if ((r = operand_map(&mb1, b1, BMN, box_b))) return r;
 
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(pair ? dc::kPairThreads : dc::kHThreads);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e;
   if (pair) {
     auto kernel = dc::hgemm_pair_kernel<AMN, BMN, EPI>;
     if ((r = set_smem(kernel, dc::kPairSmem))) return r;
     p.splits = 1;
-    attr[0].val.clusterDim.x = 2;
-    cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min(p.num_tiles, sms / 2)));
-    cfg.dynamicSmemBytes = dc::kPairSmem;
-    e = cudaLaunchKernelEx(&cfg, kernel, ma0, ma1, mb0, mb1, p);
-  } else {
-    auto kernel = dc::hgemm_cluster_kernel<AMN, BMN, EPI>;
-    if ((r = set_smem(kernel, dc::kClSmem))) return r;
-    p.splits = 1;
-    while (p.splits < 8 && 2 * p.splits * tiles <= 2 * sms && (p.kb0 + p.kb1) / (2 * p.splits) >= 4) p.splits *= 2;
-    if (const char* env = getenv("DC_HGEMM_SPLITS")) p.splits = atoi(env);
-    attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits));
-    cfg.dynamicSmemBytes = dc::kClSmem;
-    e = cudaLaunchKernelEx(&cfg, kernel, ma0, ma1, mb0, mb1, p);
+    return launch("projection launch", kernel, dim3(2 * static_cast<unsigned>(std::min(p.num_tiles, sms / 2))),
+                  dim3(dc::kPairThreads), dc::kPairSmem, st, 2, ma0, ma1, mb0, mb1, p);
   }
-  if (e != cudaSuccess) return cuda_fail(e, "projection launch");
-  DC_CHECK_LAUNCH("projection launch");
-  return DC_OK;
+  auto kernel = dc::hgemm_cluster_kernel<AMN, BMN, EPI>;
+  if ((r = set_smem(kernel, dc::kClSmem))) return r;
+  p.splits = 1;
+  while (p.splits < 8 && 2 * p.splits * tiles <= 2 * sms && (p.kb0 + p.kb1) / (2 * p.splits) >= 4) p.splits *= 2;
+  return launch("projection launch", kernel, dim3(static_cast<unsigned>(tiles * p.splits)), dim3(dc::kHThreads), dc::kClSmem, st,
+                p.splits, ma0, ma1, mb0, mb1, p);
 }
 
 template <int NT, bool GATED, int AHEAD>
-void launch_rowdot_rows(const dc::RowDotParams& p, bool vec, bool bf16, unsigned ctas, unsigned threads, cudaStream_t st) {
+int launch_rowdot_rows(const dc::RowDotParams& p, bool vec, bool bf16, unsigned ctas, unsigned threads, cudaStream_t st) {
   const size_t smem = threads / 32 * 16 * 8 * NT * sizeof(float);     // at most 16 KB
-  if (vec) {
-    if (bf16) dc::rowdot_kernel<NT, GATED, true, true, AHEAD><<<ctas, threads, smem, st>>>(p);
-    else dc::rowdot_kernel<NT, GATED, true, false, AHEAD><<<ctas, threads, smem, st>>>(p);
-  } else {
-    if (bf16) dc::rowdot_kernel<NT, GATED, false, true, 4><<<ctas, threads, smem, st>>>(p);
-    else dc::rowdot_kernel<NT, GATED, false, false, 4><<<ctas, threads, smem, st>>>(p);
-  }
+  auto go = [&](auto kernel) { return launch("projection launch", kernel, ctas, threads, smem, st, 0, p); };
+  if (vec) return bf16 ? go(dc::rowdot_kernel<NT, GATED, true, true, AHEAD>) : go(dc::rowdot_kernel<NT, GATED, true, false, AHEAD>);
+  return bf16 ? go(dc::rowdot_kernel<NT, GATED, false, true, 4>) : go(dc::rowdot_kernel<NT, GATED, false, false, 4>);
 }
 
 template <bool GATED>
@@ -190,11 +189,9 @@ int launch_rowdot(dc::RowDotParams p, bool bf16, cudaStream_t st) {
   // Up to two CTAs per SM there are registers for eight steps in flight instead of four: 10.2 us
   // against 11.6 at 4096 x 4096; with more CTAs they cost occupancy (gated 2 x 10240 x 4096: 34.8
   // against 29.9).
-  if (p.M > 8) launch_rowdot_rows<2, GATED, 4>(p, vec, bf16, ctas, threads, st);
-  else if (ctas <= 2 * 148) launch_rowdot_rows<1, GATED, 8>(p, vec, bf16, ctas, threads, st);
-  else launch_rowdot_rows<1, GATED, 4>(p, vec, bf16, ctas, threads, st);
-  DC_CHECK_LAUNCH("projection launch");
-  return DC_OK;
+  if (p.M > 8) return launch_rowdot_rows<2, GATED, 4>(p, vec, bf16, ctas, threads, st);
+  if (ctas <= 2 * 148) return launch_rowdot_rows<1, GATED, 8>(p, vec, bf16, ctas, threads, st);
+  return launch_rowdot_rows<1, GATED, 4>(p, vec, bf16, ctas, threads, st);
 }
 
 // Operands of the few-row path: any rows with element alignment.
@@ -336,10 +333,8 @@ int64_t grad_row_blocks(int64_t M, int64_t N) {
 
 int colsum_finish(const float* p0, const float* p1, int64_t ldp, int64_t P, int64_t N, void* o0, void* o1, int dtype,
                   cudaStream_t st) {
-  dc::colsum_finish_kernel<<<dim3(static_cast<unsigned>(ceil_div(N, 32)), o1 != nullptr ? 2 : 1), 256, 0, st>>>(
-      p0, p1, ldp, static_cast<int>(P), N, o0, o1, dtype);
-  DC_CHECK_LAUNCH("column sums launch");
-  return DC_OK;
+  return launch("column sums launch", dc::colsum_finish_kernel, dim3(static_cast<unsigned>(ceil_div(N, 32)), o1 != nullptr ? 2 : 1),
+                256, 0, st, 0, p0, p1, ldp, static_cast<int>(P), N, o0, o1, dtype);
 }
 
 }  // namespace
@@ -389,10 +384,8 @@ int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, i
   const cudaStream_t st = as_stream(stream);
   const dim3 grid(static_cast<unsigned>(ceil_div(N, dc::kGradCols)), static_cast<unsigned>(blocks));
   const dim3 block(dc::kGradX, dc::kGradY);
-  if (z1 != nullptr) dc::act_grad_kernel<2><<<grid, block, 0, st>>>(p);
-  else if (z != nullptr) dc::act_grad_kernel<1><<<grid, block, 0, st>>>(p);
-  else dc::act_grad_kernel<0><<<grid, block, 0, st>>>(p);
-  DC_CHECK_LAUNCH("act_grad launch");
+  const auto kernel = z1 != nullptr ? dc::act_grad_kernel<2> : z != nullptr ? dc::act_grad_kernel<1> : dc::act_grad_kernel<0>;
+  if ((r = launch("act_grad launch", kernel, grid, block, 0, st, 0, p))) return r;
   if (db != nullptr) return colsum_finish(p.part0, p.part1, ldp, blocks, N, db, db1, dtype, st);
   return DC_OK;
 }
@@ -454,9 +447,7 @@ int launch_norm_bwd(dc::NormParams p, const NormBwdPlan& n, cudaStream_t st) {
   p.stages = n.stages;
   auto go = [&](auto kernel) {
     if (int r = set_smem(kernel, n.smem)) return r;
-    kernel<<<static_cast<unsigned>(p.parts), dc::kBwdThreads, n.smem, st>>>(p);
-    DC_CHECK_LAUNCH("layer_norm_grad launch");
-    return DC_OK;
+    return launch("layer_norm_grad launch", kernel, static_cast<unsigned>(p.parts), dc::kBwdThreads, n.smem, st, 0, p);
   };
   if constexpr (sizeof(T) == 2) {
     if (p.w_f32) return go(dc::norm_bwd_kernel<T, true>);
@@ -470,9 +461,7 @@ int launch_ring(dc::NormParams p, const RingPlan& n, cudaStream_t st) {
   p.stages = n.stages;
   auto kernel = dc::norm_ring_kernel<T, E, EPT, TPR, BWD>;
   if (int r = set_smem(kernel, n.smem)) return r;
-  kernel<<<static_cast<unsigned>(n.ctas), dc::RingCta<TPR, EPT, BWD>::kThreads, n.smem, st>>>(p);
-  DC_CHECK_LAUNCH("layer_norm launch");
-  return DC_OK;
+  return launch("layer_norm launch", kernel, static_cast<unsigned>(n.ctas), dc::RingCta<TPR, EPT, BWD>::kThreads, n.smem, st, 0, p);
 }
 
 template <typename T, int E, bool BWD>
@@ -495,39 +484,29 @@ int launch_ring_rows(const dc::NormParams& p, const RingPlan& n, cudaStream_t st
 
 template <typename T, int E>
 int launch_norm_grad_wide(const dc::NormParams& p, cudaStream_t st) {
-  dc::norm_dx_wide_kernel<T, E><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
-  DC_CHECK_LAUNCH("layer_norm_grad launch");
+  if (int status = launch("layer_norm_grad launch", dc::norm_dx_wide_kernel<T, E>, static_cast<unsigned>(p.M), dc::kNormWide, 0, st, 0, p)) return status;
   if (p.part_w == nullptr) return DC_OK;
-  dc::norm_dw_wide_kernel<T, E><<<dim3(static_cast<unsigned>(ceil_div(p.D, 128 * E)), static_cast<unsigned>(p.parts)), 128, 0, st>>>(
-      p, static_cast<int>(ceil_div(p.M, p.parts)));
-  DC_CHECK_LAUNCH("layer_norm_grad launch");
-  return DC_OK;
+  return launch("layer_norm_grad launch", dc::norm_dw_wide_kernel<T, E>, dim3(static_cast<unsigned>(ceil_div(p.D, 128 * E)), static_cast<unsigned>(p.parts)), 128, 0, st, 0, p, static_cast<int>(ceil_div(p.M, p.parts)));
 }
 
 // The forward register kernel, for few rows and narrow ones: the fewest threads per row that hold it
-// in two units (eight single values) each, up to 512 threads and eight units. False: too wide.
+// in two units (eight single values) each, up to 512 threads and eight units (32 values). Wider rows
+// take the kernel for any width.
 template <typename T, bool VEC>
-bool launch_norm_reg(const dc::NormParams& p, cudaStream_t st) {
+int launch_norm_reg(const dc::NormParams& p, cudaStream_t st) {
   constexpr int E = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
   const int64_t units = ceil_div(p.D, E);
   constexpr int most = VEC ? 2 : 8, top = VEC ? 8 : 32;
   const int tpr = units <= 32 * most ? 32 : units <= 128 * most ? 128 : 512;
-  const int nu = static_cast<int>(ceil_div(units, tpr));
-  if (nu > top) return false;
-  const unsigned ctas = static_cast<unsigned>(ceil_div(p.M, tpr == 32 ? 8 : 1));
-  auto go = [&](auto t, auto n) {
-    constexpr int TPR = decltype(t)::value, NU = decltype(n)::value;
-    dc::norm_fwd_kernel<T, VEC, NU, TPR><<<ctas, dc::NormCta<TPR>::kThreads, 0, st>>>(p);
+  const int64_t nu = ceil_div(units, tpr);
+  auto go = [&](auto kernel, int threads, int rows) {
+    return launch("layer_norm launch", kernel, static_cast<unsigned>(ceil_div(p.M, rows)), threads, 0, st, 0, p);
   };
-  using std::integral_constant;
-  using I32 = integral_constant<int, 32>;
-  using I128 = integral_constant<int, 128>;
-  using I512 = integral_constant<int, 512>;
-  if (tpr == 32) go(I32{}, integral_constant<int, most>{});
-  else if (tpr == 128) go(I128{}, integral_constant<int, most>{});
-  else if (nu <= most) go(I512{}, integral_constant<int, most>{});
-  else go(I512{}, integral_constant<int, top>{});
-  return true;
+  if (tpr == 32) return go(dc::norm_fwd_kernel<T, VEC, most, 32>, dc::NormCta<32>::kThreads, 8);
+  if (tpr == 128) return go(dc::norm_fwd_kernel<T, VEC, most, 128>, 128, 1);
+  if (nu <= most) return go(dc::norm_fwd_kernel<T, VEC, most, 512>, 512, 1);
+  if (nu <= top) return go(dc::norm_fwd_kernel<T, VEC, top, 512>, 512, 1);
+  return go(dc::norm_fwd_wide_kernel<T>, dc::kNormWide, 1);
 }
 
 // Which kernel a gradient runs in, and its partial rows: the ring, for unaligned rows where the window
@@ -560,10 +539,7 @@ int launch_norm(const dc::NormParams& p, bool vec, cudaStream_t st) {
       if (vec && p.D > 256) return launch_ring_rows<T, E, false>(p, n, st);
       if (!vec && apart) return launch_ring_rows<T, 1, false>(p, n, st);
     }
-    if (!(vec ? launch_norm_reg<T, true>(p, st) : launch_norm_reg<T, false>(p, st)))
-      dc::norm_fwd_wide_kernel<T><<<static_cast<unsigned>(p.M), dc::kNormWide, 0, st>>>(p);
-    DC_CHECK_LAUNCH("layer_norm launch");
-    return DC_OK;
+    return vec ? launch_norm_reg<T, true>(p, st) : launch_norm_reg<T, false>(p, st);
   }
 }
 
@@ -671,10 +647,7 @@ int launch_embed_fwd(const dc::EmbedIds& ids, const void* table, int64_t ldt, vo
   unsigned bx = 8;
   while (bx < 128 && bx < vecs) bx *= 2;
   const unsigned by = 128 / bx;
-  dc::embed_fwd_kernel<T, E><<<static_cast<unsigned>(ceil_div(ids.T, by)), dim3(bx, by), 0, st>>>(
-      ids, static_cast<const T*>(table), ldt, static_cast<T*>(out), ldo, static_cast<int>(D), scale);
-  DC_CHECK_LAUNCH("embedding launch");
-  return DC_OK;
+  return launch("embedding launch", dc::embed_fwd_kernel<T, E>, static_cast<unsigned>(ceil_div(ids.T, by)), dim3(bx, by), 0, st, 0, ids, static_cast<const T*>(table), ldt, static_cast<T*>(out), ldo, static_cast<int>(D), scale);
 }
 
 // Workspace of the gradient: two (key, index) pairs of arrays, the radix histogram, the partials.
@@ -710,13 +683,10 @@ template <typename T, int E>
 int launch_embed_sum(const dc::EmbedSumParams& p, int64_t chunks, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(p.D, E * dc::kSumThreads)));
   if (grid.y > 65535) return fail("embedding_grad: rows of %d values are too wide", p.D);
-  dc::embed_sum_kernel<T, E><<<grid, dc::kSumThreads, 0, st>>>(p);
-  DC_CHECK_LAUNCH("embedding_grad sum launch");
+  if (int status = launch("embedding_grad sum launch", dc::embed_sum_kernel<T, E>, grid, dc::kSumThreads, 0, st, 0, p)) return status;
   if (chunks <= 2) return DC_OK;             // no run can go on behind the chunk after its first
   const dim3 join(static_cast<unsigned>(ceil_div(chunks, dc::kJoinChunks)), grid.y);
-  dc::embed_join_kernel<T, E><<<join, dc::kSumThreads * dc::kJoinGroups, 0, st>>>(p);
-  DC_CHECK_LAUNCH("embedding_grad join launch");
-  return DC_OK;
+  return launch("embedding_grad join launch", dc::embed_join_kernel<T, E>, join, dc::kSumThreads * dc::kJoinGroups, 0, st, 0, p);
 }
 
 }  // namespace
@@ -797,8 +767,7 @@ int dc_embedding_grad(const void* dy, int64_t lddy, const void* ids, int ids_i64
   if (plan.rank) {
     const dc::FillSlice fill = slice(0);
     const int ctas = static_cast<int>(ceil_div(T, dc::kRankItems));
-    dc::embed_rank_kernel<<<ctas + fill.ctas, 32 * dc::kRankWarps, 0, st>>>(e, u32(plan.keys[0]), u32(plan.idx[0]), ctas, fill);
-    DC_CHECK_LAUNCH("embedding_grad sort launch");
+    if (int status = launch("embedding_grad sort launch", dc::embed_rank_kernel, ctas + fill.ctas, 32 * dc::kRankWarps, 0, st, 0, e, u32(plan.keys[0]), u32(plan.idx[0]), ctas, fill)) return status;
   } else {
     const int tiles = static_cast<int>(plan.tiles);
     const unsigned threads = 32 * dc::kRadixWarps;
@@ -807,17 +776,15 @@ int dc_embedding_grad(const void* dy, int64_t lddy, const void* ids, int ids_i64
       uint32_t* hist = u32(plan.hist);
       const dc::FillSlice f0 = slice(2 * pass), f1 = slice(2 * pass + 1);
       const unsigned g0 = tiles + f0.ctas, g1 = tiles + f1.ctas;
-      if (pass == 0) {
-        dc::radix_hist_kernel<true><<<g0, threads, 0, st>>>(e, nullptr, hist, shift, plan.bits, tiles, f0);
-        dc::radix_scatter_kernel<true><<<g1, threads, 0, st>>>(e, nullptr, nullptr, hist, u32(plan.keys[out]),
-                                                               u32(plan.idx[out]), shift, plan.bits, tiles, f1);
-      } else {
-        dc::radix_hist_kernel<false><<<g0, threads, 0, st>>>(e, u32(plan.keys[in]), hist, shift, plan.bits, tiles, f0);
-        dc::radix_scatter_kernel<false><<<g1, threads, 0, st>>>(e, u32(plan.keys[in]), u32(plan.idx[in]), hist,
-                                                                u32(plan.keys[out]), u32(plan.idx[out]), shift, plan.bits,
-                                                                tiles, f1);
-      }
-      DC_CHECK_LAUNCH("embedding_grad sort launch");
+      // the first pass reads the ids, whatever the key arrays hold
+      const auto count = pass == 0 ? dc::radix_hist_kernel<true> : dc::radix_hist_kernel<false>;
+      const auto scatter = pass == 0 ? dc::radix_scatter_kernel<true> : dc::radix_scatter_kernel<false>;
+      if ((r = launch("embedding_grad sort launch", count, g0, threads, 0, st, 0, e, u32(plan.keys[in]), hist, shift, plan.bits,
+                      tiles, f0)))
+        return r;
+      if ((r = launch("embedding_grad sort launch", scatter, g1, threads, 0, st, 0, e, u32(plan.keys[in]), u32(plan.idx[in]), hist,
+                      u32(plan.keys[out]), u32(plan.idx[out]), shift, plan.bits, tiles, f1)))
+        return r;
       cur = out;
     }
   }

@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(kGradX * kGradY)
 act_grad_kernel(const ActGradParams p) {
   constexpr int kAhead = FORM == 0 ? 8 : FORM == 1 ? 3 : 2;
   __shared__ float red[FORM == 2 ? 2 : 1][kGradY][kGradCols];
+  pdl_enter();
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kGradCols + threadIdx.x * 8;
   const int n = static_cast<int>(min(static_cast<int64_t>(8), p.N - col));      // may be <= 0
   const bool z_hi = n > 4;                  // z rows are padded to 4 values
@@ -140,6 +141,7 @@ __device__ __forceinline__ void store_as(void* dst, int64_t i, float v, int dtyp
 __global__ void __launch_bounds__(256)
 colsum_finish_kernel(const float* __restrict__ part0, const float* __restrict__ part1, int64_t ldp, int P, int64_t N,
                      void* out0, void* out1, int dtype) {
+  pdl_enter();
   const float* part = blockIdx.y ? part1 : part0;
   void* out = blockIdx.y ? out1 : out0;
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
