@@ -516,9 +516,81 @@ __device__ __forceinline__ float4 load4(const uint16_t* src, int n, bool vec, in
   return make_float4(h_to_f(a & 0xFFFFu, bf16), h_to_f(a >> 16, bf16), h_to_f(b & 0xFFFFu, bf16), h_to_f(b >> 16, bf16));
 }
 
-// One CTA of a cluster computes its share of a tile's k-blocks; the fp32 partials are left in
-// shared memory and each CTA of the cluster adds up and finishes its share of the rows, in the
-// order of the CTAs (the same sums on every call).
+// fp32 partial tiles in the shared memory of a cluster's CTAs, added in the order of the CTAs (the
+// same sums on every call) and finished: bias, pre-activations, activation, residual or gate, store.
+// A partial row is kClUnits float4, unit u at u ^ (row & 7). Tile row 0 and column 0 are output
+// (row0, col0); this CTA finishes rows [r_begin, r_end).
+constexpr int kClUnits = kClBN / 4;
+
+template <int EPI>
+__device__ __forceinline__ void finish_tile(const HGemmParams& p, const float* part, int r_begin, int r_end, int64_t row0,
+                                            int col0, uint16_t* out) {
+  constexpr int kOutUnits = EPI == kEpiGated ? kClUnits / 2 : kClUnits;      // the gate's units, then the up projection's
+  const uint32_t part_u = smem_u32(part);
+  auto sum4 = [&](int r, int u) {
+    const int off = r * kClUnits + (u ^ (r & 7));
+    if (p.splits == 1) return reinterpret_cast<const float4*>(part)[off];
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < p.splits; ++c) {
+      uint32_t a;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(part_u + off * 16), "r"(c));
+      const float4 v = ld_cluster_f4(a);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    return s;
+  };
+  for (int i = r_begin * kOutUnits + static_cast<int>(threadIdx.x); i < r_end * kOutUnits; i += kHThreads) {
+    const int r = i / kOutUnits, u = i % kOutUnits;
+    const int col = col0 + 4 * u;
+    const int n = p.N - col;                             // columns left, from this unit on
+    if (n <= 0) continue;
+    const int64_t row = row0 + r;
+    float4 s = sum4(r, u);
+    if (p.bias != nullptr) {
+      const float4 b = load4(reinterpret_cast<const uint16_t*>(p.bias) + col, n, false, p.bf16);
+      s.x += b.x; s.y += b.y; s.z += b.z; s.w += b.w;
+    }
+    if (p.z0 != nullptr) *reinterpret_cast<float4*>(p.z0 + row * p.ldz + col) = s;     // rows are padded to 4 floats
+    float v[4] = {s.x, s.y, s.z, s.w};
+    act_values(v, p.act);
+    if (EPI == kEpiGated) {
+      float4 w = sum4(r, u + kOutUnits);
+      if (p.bias1 != nullptr) {
+        const float4 b = load4(reinterpret_cast<const uint16_t*>(p.bias1) + col, n, false, p.bf16);
+        w.x += b.x; w.y += b.y; w.z += b.z; w.w += b.w;
+      }
+      if (p.z1 != nullptr) *reinterpret_cast<float4*>(p.z1 + row * p.ldz + col) = w;
+      v[0] *= w.x; v[1] *= w.y; v[2] *= w.z; v[3] *= w.w;
+    } else if (p.residual != nullptr) {
+      const float4 b = load4(reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr + col, n, p.res_vec, p.bf16);
+      v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+    }
+    const uint32_t lo = pack_h2(v[0], v[1], p.bf16), hi = pack_h2(v[2], v[3], p.bf16);
+    uint16_t* dst = out + row * p.ldo + col;
+    if (p.out_vec && n >= 4) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    } else {
+      dst[0] = static_cast<uint16_t>(lo);
+      if (n > 1) dst[1] = static_cast<uint16_t>(lo >> 16);
+      if (n > 2) dst[2] = static_cast<uint16_t>(hi);
+      if (n > 3) dst[3] = static_cast<uint16_t>(hi >> 16);
+    }
+  }
+}
+
+// Columns [c, c + 32) of this warp's 32 TMEM lanes to the partial tile.
+__device__ __forceinline__ void drain_block(uint32_t taddr, int c, float* part, int row) {
+  uint32_t v[32];
+  tmem_ld32(taddr + c, v);
+  tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 32; j += 4)
+    reinterpret_cast<uint4*>(part)[row * kClUnits + (((c + j) >> 2) ^ (row & 7))] = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+}
+
+// One CTA of a cluster computes its share of a tile's k-blocks and leaves its fp32 partials in shared
+// memory; each CTA of the cluster finishes its share of the rows.
 template <bool AMN, bool BMN, int EPI>
 __global__ void __launch_bounds__(kHThreads, 2)
 hgemm_cluster_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
@@ -611,20 +683,12 @@ hgemm_cluster_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_co
   bool ok = mbar_wait(&acc_full, 0, nullptr);
   ok = __all_sync(0xffffffffu, ok && *abort == 0);
   tc_fence_after();
-  // Partial tile in shared memory: row r at r * 512 bytes, 16-byte units XORed with r & 7.
   float* part = reinterpret_cast<float*>(smem);
   if (warp >= 2) {
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const int r = quarter * 32 + lane;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
-    for (int c = half * (kClBN / 2); c < (half + 1) * (kClBN / 2); c += 32) {
-      uint32_t v[32];
-      tmem_ld32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c, v);
-      tmem_wait_ld();
-#pragma unroll
-      for (int j = 0; j < 32; j += 4)
-        reinterpret_cast<uint4*>(part)[r * 32 + (((c + j) >> 2) ^ (r & 7))] = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    }
+    for (int c = half * (kClBN / 2); c < (half + 1) * (kClBN / 2); c += 32) drain_block(taddr, c, part, quarter * 32 + lane);
   }
   tc_fence_before();
   if (p.splits > 1) cluster_sync();
@@ -632,61 +696,9 @@ hgemm_cluster_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_co
   if (ok) {
     const int rows = min(128, p.M - row0);
     const int per = (rows + p.splits - 1) / p.splits;
-    const int r_begin = rank * per, r_end = min(rows, r_begin + per);
-    const uint32_t part_u = smem_u32(part);
-    uint16_t* out = reinterpret_cast<uint16_t*>(second ? p.out1 : p.out);
-    constexpr int kUnits = kOutCols / 4;
-    auto sum4 = [&](int r, int u) {
-      const int off = r * 32 + (u ^ (r & 7));
-      if (p.splits == 1) return reinterpret_cast<const float4*>(part)[off];
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = 0; c < p.splits; ++c) {
-        uint32_t a;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(part_u + off * 16), "r"(c));
-        const float4 t = ld_cluster_f4(a);
-        s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
-      }
-      return s;
-    };
-    for (int i = r_begin * kUnits + static_cast<int>(threadIdx.x); i < r_end * kUnits; i += kHThreads) {
-      const int r = i / kUnits, u = i % kUnits;
-      const int col = tn * kOutCols + 4 * u;
-      const int n = p.N - col;                           // columns left, from this unit on
-      if (n <= 0) continue;
-      const int64_t row = row0 + r;
-      float4 s = sum4(r, u);
-      if (p.bias != nullptr) {
-        const float4 b = load4(reinterpret_cast<const uint16_t*>(p.bias) + col, n, false, p.bf16);
-        s.x += b.x; s.y += b.y; s.z += b.z; s.w += b.w;
-      }
-      if (p.z0 != nullptr) {
-        float* z = p.z0 + row * p.ldz + col;             // rows of z are padded to 4 floats
-        *reinterpret_cast<float4*>(z) = s;
-      }
-      s = make_float4(act_value(s.x, p.act), act_value(s.y, p.act), act_value(s.z, p.act), act_value(s.w, p.act));
-      if (EPI == kEpiGated) {
-        float4 t = sum4(r, u + kUnits);
-        if (p.bias1 != nullptr) {
-          const float4 b = load4(reinterpret_cast<const uint16_t*>(p.bias1) + col, n, false, p.bf16);
-          t.x += b.x; t.y += b.y; t.z += b.z; t.w += b.w;
-        }
-        if (p.z1 != nullptr) *reinterpret_cast<float4*>(p.z1 + row * p.ldz + col) = t;
-        s.x *= t.x; s.y *= t.y; s.z *= t.z; s.w *= t.w;
-      } else if (p.residual != nullptr) {
-        const float4 b = load4(reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr + col, n, p.res_vec, p.bf16);
-        s.x += b.x; s.y += b.y; s.z += b.z; s.w += b.w;
-      }
-      const uint32_t lo = pack_h2(s.x, s.y, p.bf16), hi = pack_h2(s.z, s.w, p.bf16);
-      uint16_t* dst = out + row * p.ldo + col;
-      if (p.out_vec && n >= 4) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-      } else {
-        dst[0] = static_cast<uint16_t>(lo);
-        if (n > 1) dst[1] = static_cast<uint16_t>(lo >> 16);
-        if (n > 2) dst[2] = static_cast<uint16_t>(hi);
-        if (n > 3) dst[3] = static_cast<uint16_t>(hi >> 16);
-      }
-    }
+    const int r_begin = min(rows, rank * per);
+    finish_tile<EPI>(p, part, r_begin, min(rows, r_begin + per), row0, tn * kOutCols,
+                     reinterpret_cast<uint16_t*>(second ? p.out1 : p.out));
   }
   // No CTA leaves while another may still read its partials.
   if (p.splits > 1) cluster_sync();

@@ -379,28 +379,35 @@ norm_ring_kernel(const NormParams p) {
     if (BWD && block + gridDim.x < blocks) load_stats(block + gridDim.x);
     mbar_wait(&full[stage], phase, nullptr);
     __syncwarp();
-    const uint8_t* a[2] = {nullptr, nullptr};
-    if (live) {
-#pragma unroll
-      for (int k = 0; k < kTensors; ++k) {
-        const uint8_t* g = src[k] + row * pitch[k];
-        a[k] = in_place(row) ? g : slot(stage, sub, k) + (reinterpret_cast<uintptr_t>(g) & 15);
-      }
-    }
     // Values past the row read as the mean: their deviation is 0 backward, and they add 0 forward.
     Pair h[kPairs], d[BWD ? kPairs : 1];
     {
       float hf[EPT], df[EPT];
+      const uint8_t* gx = src[0] + row * pitch[0];
+      const uint8_t* gd = src[1] + row * pitch[1];
+      auto take = [&](const T* x, const T* y) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + t) * E;
-        if (live && c < p.D) {
-          load_e<T, E>(reinterpret_cast<const T*>(a[0]) + c, hf + i * E);
-          if (BWD) load_e<T, E>(reinterpret_cast<const T*>(a[1]) + c, df + i * E);
-        } else {
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + t) * E;
+          if (live && c < p.D) {
+            load_e<T, E>(x + c, hf + i * E);
+            if (BWD) load_e<T, E>(y + c, df + i * E);
+          } else {
 #pragma unroll
-          for (int j = 0; j < E; ++j) { hf[i * E + j] = mu; df[i * E + j] = 0.f; }
+            for (int j = 0; j < E; ++j) { hf[i * E + j] = mu; df[i * E + j] = 0.f; }
+          }
         }
+      };
+      if (live && in_place(row)) {
+        take(reinterpret_cast<const T*>(gx), reinterpret_cast<const T*>(gd));
+      } else {
+        const uint8_t* sx = slot(stage, sub, 0);
+        const uint8_t* sd = slot(stage, sub, kTensors - 1);
+        if (E == 1) {                                    // where the row starts in its window
+          sx += reinterpret_cast<uintptr_t>(gx) & 15;
+          sd += reinterpret_cast<uintptr_t>(gd) & 15;
+        }
+        take(reinterpret_cast<const T*>(sx), reinterpret_cast<const T*>(sd));
       }
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {

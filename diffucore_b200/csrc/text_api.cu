@@ -94,20 +94,45 @@ int check_act(const char* what, int act) {
 // DC_HGEMM_PAIR = "0" / "1": force the cluster / the pair kernel (both compute every shape).
 int pair_override() {
   const char* env = getenv("DC_HGEMM_PAIR");
-  if (env == nullptr || (strcmp(env, "0") != 0 && strcmp(env, "1") != 0)) return -1;
+  if (env == nullptr || (env[0] != '0' && env[0] != '1') || env[1] != 0) return -1;
   return env[0] - '0';
 }
 
-// Tile width of the pair kernel: the one with the fewest waves over the `pairs` CTA pairs times a
-// tile's cost. A tile is bound by what it reads from L2, 256 rows of A and bn rows of B per k
-// (measured: 512 x 20480 x 4096 in three waves, 72.0 us with 192 columns and 82.9 with 256).
-int choose_pair_bn(int64_t m_tiles, int64_t cols, int pairs) {
-  if (const char* env = getenv("DC_HGEMM_BN")) return atoi(env);
-  int best = 256;
-  int64_t best_cost = INT64_MAX;
-  for (int bn = 256; bn >= 128; bn -= 32) {
-    const int64_t cost = ceil_div(m_tiles * ceil_div(cols, bn), pairs) * (256 + bn);
-    if (cost < best_cost) { best = bn; best_cost = cost; }
+// Kernel and tile of a product: the smallest estimate of its time on the GPU. Both kernels are bound by
+// what their CTAs read from L2, 128 bytes per row of A or B and 64-deep k-block; in nanoseconds,
+// measured with the operands in L2,
+//   pair      5400 + 4 bn + waves * k-blocks * 0.605 (256 + bn)
+//   cluster   5200 + (S > 1: 900 + 200 S rows / 128) + load * k-blocks / S * 1.29 (rows + 128)
+// with bn the pair's tile width, S the CTAs that divide a cluster tile's k-blocks, rows the tile's
+// rows of A (at most 128), and load the CTAs per SM (at least one; two are resident, so a second
+// wave counts as two more). Measured against the estimate, us: 300 x 4096 x 4096, pair 128 wide 22.1
+// (20.9), cluster S = 2 22.3 (20.2); 1024^3, pair 128 wide 9.5 (9.6), 256 wide 11.3 (11.4); 700 x 1280
+// x 5120, cluster S = 4 17.2 (17.6), pair 24.8 (24.6); 512 x 512 x 8192, cluster S = 8 14.4 (13.0), S = 4
+// 17.9 (17.5); 64 x 1024 x 1024, cluster S = 4 6.4 (7.5).
+struct HChoice { bool pair; int bn, splits; };
+
+HChoice choose_hgemm(int64_t M, int stack, int64_t cols, int64_t k, int sms) {
+  HChoice best = {true, 256, 1};
+  double best_ns = 1e30;
+  const int forced = pair_override();
+  const double kb = static_cast<double>(ceil_div(k, dc::kHBK));
+  if (forced != 0) {
+    const int64_t m_tiles = ceil_div(M, 256) * stack;
+    for (int bn = 256; bn >= 128; bn -= 32) {
+      const double waves = static_cast<double>(ceil_div(m_tiles * ceil_div(cols, bn), sms / 2));
+      const double ns = 5400 + 4.0 * bn + waves * kb * 0.605 * (256 + bn);
+      if (ns < best_ns) { best = {true, bn, 1}; best_ns = ns; }
+    }
+  }
+  if (forced != 1) {
+    const double tiles = static_cast<double>(ceil_div(M, 128) * stack * ceil_div(cols, dc::kClBN));
+    const double rows = static_cast<double>(std::min<int64_t>(M, 128));
+    for (int s = 1; s <= 8 && (s == 1 || kb >= 2 * s); s *= 2) {
+      const double ctas = tiles * s;
+      const double load = ctas <= 2 * sms ? std::max(1.0, ctas / sms) : 2 * std::ceil(ctas / (2 * sms));
+      const double ns = 5200 + (s > 1 ? 900 + 200 * s * rows / 128 : 0) + load * (kb / s) * 1.29 * (rows + 128);
+      if (ns < best_ns) { best = {false, 256, s}; best_ns = ns; }
+    }
   }
   return best;
 }
@@ -118,12 +143,13 @@ int choose_pair_bn(int64_t m_tiles, int64_t cols, int pairs) {
 template <bool AMN, bool BMN, int EPI>
 int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const Operand& b1, bool stacked,
                  dc::HGemmParams p, cudaStream_t st) {
-  const int sms = sm_count();
-  const int64_t m_tiles = ceil_div(p.M, 256) * (stacked ? 2 : 1);
-  p.bn = choose_pair_bn(m_tiles, EPI == dc::kEpiGated ? 2 * static_cast<int64_t>(p.N) : p.N, sms / 2);
-  const int64_t pair_tiles = m_tiles * ceil_div(EPI == dc::kEpiGated ? 2 * static_cast<int64_t>(p.N) : p.N, p.bn);
-  const int forced = pair_override();
-  const bool pair = forced >= 0 ? forced == 1 : p.M > 256 && pair_tiles * 4 >= sms;
+  const int sms = sm_count(), stack = stacked ? 2 : 1;
+  const int64_t cols = EPI == dc::kEpiGated ? 2 * static_cast<int64_t>(p.N) : p.N;        // accumulator columns
+  const int64_t k_all = a0.k + (!stacked && a1.p != nullptr ? a1.k : 0);
+  const HChoice choice = choose_hgemm(p.M, stack, cols, k_all, sms);
+  const bool pair = choice.pair;
+  p.bn = choice.bn;
+  p.splits = choice.splits;
   const int tile_m = pair ? 256 : 128;
   const int tile_n = (pair ? p.bn : dc::kClBN) / (EPI == dc::kEpiGated ? 2 : 1);
   const int bk = pair ? dc::kPairAtoms * dc::kHBK : dc::kHBK;
@@ -154,14 +180,11 @@ int launch_hgemm(const Operand& a0, const Operand& a1, const Operand& b0, const 
   if (pair) {
     auto kernel = dc::hgemm_pair_kernel<AMN, BMN, EPI>;
     if ((r = set_smem(kernel, dc::kPairSmem))) return r;
-    p.splits = 1;
     return launch("projection launch", kernel, dim3(2 * static_cast<unsigned>(std::min(p.num_tiles, sms / 2))),
                   dim3(dc::kPairThreads), dc::kPairSmem, st, 2, ma0, ma1, mb0, mb1, p);
   }
   auto kernel = dc::hgemm_cluster_kernel<AMN, BMN, EPI>;
   if ((r = set_smem(kernel, dc::kClSmem))) return r;
-  p.splits = 1;
-  while (p.splits < 8 && 2 * p.splits * tiles <= 2 * sms && (p.kb0 + p.kb1) / (2 * p.splits) >= 4) p.splits *= 2;
   return launch("projection launch", kernel, dim3(static_cast<unsigned>(tiles * p.splits)), dim3(dc::kHThreads), dc::kClSmem, st,
                 p.splits, ma0, ma1, mb0, mb1, p);
 }

@@ -99,8 +99,7 @@ constexpr int64_t kFewRows = 8;         // rows of x up to which the projections
 Tensor projection_operand(const Tensor& t, int64_t rows) {
   if (tile_loadable(t)) return t;
   if (rows <= kFewRows && t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1))) {
-    const char* env = getenv("DC_HGEMM_PAIR");
-    if (env == nullptr || (std::string(env) != "0" && std::string(env) != "1")) return t;
+    if (getenv("DC_HGEMM_PAIR") == nullptr) return t;
   }
   return matrix_operand(t);
 }
