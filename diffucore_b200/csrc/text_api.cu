@@ -437,16 +437,18 @@ RingPlan ring_plan(int64_t M, int64_t D, size_t es, bool vec, bool bwd) {
   if (!vec && n.tpr == 64) { n.tpr = 128; n.ept = 16; }
   if (D > 16384 || (bwd && D > 8192)) return n;
   const int threads = std::max(128, n.tpr), rows = threads / n.tpr;
-  const int sm_threads = n.ept > 16 ? (bwd ? 256 : 512) : (bwd ? 512 : 768);
+  const bool shared_w = bwd && n.ept > 16 && (es == 4 || n.tpr < 128);        // RingCta::kSharedW
+  const int sm_threads = n.ept > 16 ? (!bwd ? 512 : shared_w ? 384 : 256) : (bwd ? 512 : 768);
+  const int64_t w_bytes = shared_w ? n.tpr * n.ept * 4 : 0;
   n.slot = static_cast<int>(round_up(D * static_cast<int64_t>(es), 16)) + (vec ? 0 : 16);
   const int64_t stage = static_cast<int64_t>(rows) * (bwd ? 2 : 1) * n.slot;
   constexpr int64_t kSm = 200 << 10;
   int per_sm = std::max(1, sm_threads / threads);
-  while (per_sm > 0 && 2 * stage * per_sm > kSm) --per_sm;
+  while (per_sm > 0 && (w_bytes + 2 * stage) * per_sm > kSm) --per_sm;
   if (per_sm == 0) return n;
-  n.stages = static_cast<int>(std::min<int64_t>(dc::kRingMax, kSm / per_sm / stage));
+  n.stages = static_cast<int>(std::min<int64_t>(dc::kRingMax, (kSm / per_sm - w_bytes) / stage));
   const int64_t sums = rows > 1 ? 2 * n.tpr * n.ept * 4 : 0;
-  n.smem = static_cast<int>(std::max(n.stages * stage, sums));
+  n.smem = static_cast<int>(w_bytes + std::max(n.stages * stage, sums));
   n.ctas = std::min<int64_t>(ceil_div(M, rows), 148 * per_sm);
   return n;
 }
@@ -484,7 +486,7 @@ int launch_ring(dc::NormParams p, const RingPlan& n, cudaStream_t st) {
   p.stages = n.stages;
   auto kernel = dc::norm_ring_kernel<T, E, EPT, TPR, BWD>;
   if (int r = set_smem(kernel, n.smem)) return r;
-  return launch("layer_norm launch", kernel, static_cast<unsigned>(n.ctas), dc::RingCta<TPR, EPT, BWD>::kThreads, n.smem, st, 0, p);
+  return launch("layer_norm launch", kernel, static_cast<unsigned>(n.ctas), dc::RingCta<T, TPR, EPT, BWD>::kThreads, n.smem, st, 0, p);
 }
 
 template <typename T, int E, bool BWD>
