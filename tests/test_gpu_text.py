@@ -306,6 +306,34 @@ def test_layer_norm(M, D, dtype, affine):
         close(a, e)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,D", [(1300, 65), (1301, 999), (2, 2047), (17, 2047), (1201, 2049), (1190, 4095), (1185, 1028),
+                                 (1200, 300)])
+def test_layer_norm_rows_at_any_offset(M, D, dtype):
+    """Rows that start anywhere in a 16-byte window, alike in x, dy and dx (contiguous tensors, and ones
+    that begin off a boundary) and not alike (a view with another row pitch)."""
+    g = gen(M, D, "offset rows")
+    w, b = rand(g, D, dtype=dtype) + 1, rand(g, D, dtype=dtype)
+
+    def check(x, dy):
+        leaves = [x.detach().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()]
+        y = text.layer_norm(*leaves)
+        got = torch.autograd.grad(y, leaves, dy)
+        d = [t.detach().double().requires_grad_() for t in leaves]
+        want_y = norm64(*d)
+        close(y.detach(), want_y.detach())
+        for a, e in zip(got, torch.autograd.grad(want_y, d, dy.double())):
+            close(a.contiguous(), e)
+
+    x, dy = rand(g, M, D, dtype=dtype, std=2.0) + 0.5, rand(g, M, D, dtype=dtype)
+    check(x, dy)
+    off = rand(g, M * D + 3, dtype=dtype)
+    check(off[3:].view(M, D), dy)
+    wide = rand(g, M, D + 5, dtype=dtype)
+    check(wide[:, 1:D + 1], dy)
+    check(x, wide[:, 2:D + 2])
+
+
 def test_layer_norm_views_and_constant_rows():
     g = gen("norm views")
     base = rand(g, 6, 9, 300)
@@ -331,6 +359,37 @@ def test_layer_norm_large_offset():
     want = norm64(x.double(), None, None)
     # x itself is given to 2^-11 relative to a deviation of 1; the mean in fp32 to 4096 * 2^-24
     assert (text.layer_norm(x).double() - want).abs().max().item() < 4096 * 2 ** -22
+
+
+def test_graph_capture_and_replay():
+    """The calls enqueue work only: a training step captured once gives the same results when replayed
+    on new inputs."""
+    g = gen("graph")
+    x, w, b = (rand(g, *s).requires_grad_() for s in ((300, 128), (256, 128), (256,)))
+    nw = rand(g, 256).requires_grad_()
+    ids = torch.randint(0, 300, (500,), device=DEV)
+    dy = rand(g, 500, 256)
+
+    def step():
+        table = text.layer_norm(text.linear(x, w, b, activation="gelu"), nw)
+        return torch.autograd.grad(text.embedding(ids, table), (x, w, b, nw), dy)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        x.copy_(rand(g, 300, 128))
+        ids.copy_(torch.randint(0, 300, (500,), device=DEV))
+    graph.replay()
+    got = [t.clone() for t in out]
+    graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(got, out))
+    assert all(torch.equal(p, q) for p, q in zip(got, step()))
 
 
 # ─── embedding ──────────────────────────────────────────────────────────────────────────
