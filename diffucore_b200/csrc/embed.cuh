@@ -38,26 +38,39 @@ __device__ __forceinline__ uint32_t key_at(const EmbedIds& e, int64_t t) {
   return id >= 0 && id < e.V && id != e.padding ? static_cast<uint32_t>(id) : static_cast<uint32_t>(e.V);
 }
 
-// Bound by HBM: one read and one write of a row per token. blockDim (x: vectors of a row, y: tokens).
-template <typename T, int E>
+// Bound by HBM: one read and one write of a row per token. blockDim (x: vectors of a row, y: rows);
+// a row of threads takes kTokens tokens, whose loads are in flight together: four where a thread has
+// one vector of a row and tokens are many (500000 x 256 bf16 84 us, 134 with one), else one (65536 x
+// 2048 76 us, 80 with four).
+template <typename T, int E, int kTokens>
 __global__ void __launch_bounds__(256)
 embed_fwd_kernel(const EmbedIds ids, const T* __restrict__ table, int64_t ldt, T* __restrict__ out, int64_t ldo,
                  int D, float scale) {
   pdl_enter();
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (t >= ids.T) return;
-  const int64_t id = id_at(ids, t);
-  const bool ok = id >= 0 && id < ids.V;
-  if (!ok && threadIdx.x == 0) record_error(kErrTokenId);
-  const T* src = table + (ok ? id : 0) * ldt;
-  T* dst = out + t * ldo;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y) * kTokens;
+  const T* src[kTokens];
+  bool ok[kTokens];
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k) {
+    const int64_t id = t0 + k < ids.T ? id_at(ids, t0 + k) : 0;
+    ok[k] = id >= 0 && id < ids.V;
+    if (!ok[k] && threadIdx.x == 0) record_error(kErrTokenId);
+    src[k] = table + (ok[k] ? id : 0) * ldt;
+  }
 #pragma unroll 4
   for (int c = threadIdx.x * E; c < D; c += blockDim.x * E) {
-    float f[E];
-    if (ok) load_e<T, E>(src + c, f);
+    float f[kTokens][E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) f[j] = ok ? f[j] * scale : 0.f;
-    store_e<T, E>(dst + c, f);
+    for (int k = 0; k < kTokens; ++k)
+      if (t0 + k < ids.T) load_e<T, E>(src[k] + c, f[k]);
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      if (t0 + k < ids.T) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[k][j] = ok[k] ? f[k][j] * scale : 0.f;
+        store_e<T, E>(out + (t0 + k) * ldo + c, f[k]);
+      }
+    }
   }
 }
 
@@ -190,7 +203,7 @@ radix_scatter_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, cons
     const int d = threadIdx.x * kPerThread + j;
     total[j] = 0; before_tile[j] = 0;
     if (d < digits) {
-#pragma unroll 8
+#pragma unroll 16
       for (int i = 0; i < tiles; ++i) {
         const uint32_t c = hist[static_cast<int64_t>(i) * digits + d];
         total[j] += c;
@@ -273,6 +286,7 @@ __global__ void __launch_bounds__(kSumThreads)
 embed_sum_kernel(const EmbedSumParams p) {
   pdl_enter();
   constexpr uint32_t kNone = 0xFFFFFFFFu;       // never a key
+  using Unit = typename NormUnit<T, (E > 1)>::type;
   __shared__ uint32_t key[2 * kSumChunkMax + 2];
   __shared__ uint32_t idx[2 * kSumChunkMax];
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.chunk;
@@ -304,18 +318,21 @@ embed_sum_kernel(const EmbedSumParams p) {
   constexpr int kAhead = 8;
   for (int i0 = s0; i0 < e0; i0 += kAhead) {
     if (key[i0 + 1] == static_cast<uint32_t>(p.V)) return;         // sorted last: nothing follows
-    float v[kAhead][E];
+    // Kept packed until they are added: widened at the load they would take twice the registers, and
+    // the compiler would not keep all of them in flight.
+    Unit v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (i0 + u < e0) load_e<T, E>(dy + static_cast<int64_t>(idx[i0 + u]) * p.lddy, v[u]);
+      v[u] = *reinterpret_cast<const Unit*>(dy + static_cast<int64_t>(idx[min(i0 + u, e0 - 1)]) * p.lddy);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u;
       if (i >= e0) break;
       const uint32_t k = key[i + 1];
       if (k == static_cast<uint32_t>(p.V)) return;
+      const T* h = reinterpret_cast<const T*>(&v[u]);
 #pragma unroll
-      for (int j = 0; j < E; ++j) acc[j] += v[u][j];
+      for (int j = 0; j < E; ++j) acc[j] += to_f(h[j]);
       const bool ends = key[i + 2] != k;
       if (ends || i == e0 - 1) {
         if (ends && !from_before) {
@@ -335,11 +352,11 @@ embed_sum_kernel(const EmbedSumParams p) {
   }
 }
 
-// Runs that cover a whole chunk. A CTA looks at 8 chunks for one that such a run starts in, and adds
+// Runs that cover a whole chunk. A CTA looks at 4 chunks for one that such a run starts in, and adds
 // the run's partial rows: four groups of threads take a quarter of them each, then the quarters are
 // added in order.
 constexpr int kJoinGroups = 4;
-constexpr int kJoinChunks = 8;
+constexpr int kJoinChunks = 4;
 
 template <typename T, int E>
 __global__ void __launch_bounds__(kSumThreads * kJoinGroups)

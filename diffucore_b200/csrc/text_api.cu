@@ -357,7 +357,7 @@ int64_t grad_row_blocks(int64_t M, int64_t N) {
 int colsum_finish(const float* p0, const float* p1, int64_t ldp, int64_t P, int64_t N, void* o0, void* o1, int dtype,
                   cudaStream_t st) {
   return launch("column sums launch", dc::colsum_finish_kernel, dim3(static_cast<unsigned>(ceil_div(N, 32)), o1 != nullptr ? 2 : 1),
-                256, 0, st, 0, p0, p1, ldp, static_cast<int>(P), N, o0, o1, dtype);
+                32 * dc::kFinishGroups, 0, st, 0, p0, p1, ldp, static_cast<int>(P), N, o0, o1, dtype);
 }
 
 }  // namespace
@@ -672,7 +672,12 @@ int launch_embed_fwd(const dc::EmbedIds& ids, const void* table, int64_t ldt, vo
   unsigned bx = 8;
   while (bx < 128 && bx < vecs) bx *= 2;
   const unsigned by = 128 / bx;
-  return launch("embedding launch", dc::embed_fwd_kernel<T, E>, static_cast<unsigned>(ceil_div(ids.T, by)), dim3(bx, by), 0, st, 0, ids, static_cast<const T*>(table), ldt, static_cast<T*>(out), ldo, static_cast<int>(D), scale);
+  auto go = [&](auto kernel, unsigned tokens) {
+    return launch("embedding launch", kernel, static_cast<unsigned>(ceil_div(ids.T, by * tokens)), dim3(bx, by), 0, st, 0, ids,
+                  static_cast<const T*>(table), ldt, static_cast<T*>(out), ldo, static_cast<int>(D), scale);
+  };
+  return vecs <= bx && ids.T >= 148 * 16 * static_cast<int64_t>(by) ? go(dc::embed_fwd_kernel<T, E, 4>, 4)
+                                                                    : go(dc::embed_fwd_kernel<T, E, 1>, 1);
 }
 
 // Workspace of the gradient: two (key, index) pairs of arrays, the radix histogram, the partials.

@@ -136,9 +136,12 @@ __device__ __forceinline__ void store_as(void* dst, int64_t i, float v, int dtyp
   else static_cast<__half*>(dst)[i] = __float2half_rn(v);
 }
 
-// out[n] = sum of P partial rows. A CTA of 32 columns x 8 row groups: group g adds rows g, g + 8,
-// ..., then the groups are added in order. blockIdx.y picks one of two sums.
-__global__ void __launch_bounds__(256)
+// out[n] = sum of P partial rows. A CTA of 32 columns x 32 row groups: group g adds rows g, g + 32,
+// ..., then the groups are added in order. Latency-bound (a few MB from L2), so every group's first
+// loads are in flight at once. blockIdx.y picks one of two sums.
+constexpr int kFinishGroups = 32;
+
+__global__ void __launch_bounds__(32 * kFinishGroups)
 colsum_finish_kernel(const float* __restrict__ part0, const float* __restrict__ part1, int64_t ldp, int P, int64_t N,
                      void* out0, void* out1, int dtype) {
   pdl_enter();
@@ -146,17 +149,17 @@ colsum_finish_kernel(const float* __restrict__ part0, const float* __restrict__ 
   void* out = blockIdx.y ? out1 : out0;
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  __shared__ float red[8][33];
+  __shared__ float red[kFinishGroups][33];
   float s = 0.f;
   if (col < N) {
-#pragma unroll 4
-    for (int r = g; r < P; r += 8) s += part[r * ldp + col];
+#pragma unroll 8
+    for (int r = g; r < P; r += kFinishGroups) s += part[r * ldp + col];
   }
   red[g][lane] = s;
   __syncthreads();
   if (g == 0 && col < N) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][lane];
+    for (int i = 1; i < kFinishGroups; ++i) s += red[i][lane];
     store_as(out, col, s, dtype);
   }
 }
