@@ -1,8 +1,8 @@
 """GPU numerics of the text operators (linear, gated linear, layer norm, embedding) against plain
 float64 implementations, forward and backward, through the public functions.
 
-Tolerances are relative 2-norms. A result rounded once to a type with unit roundoff u (bf16 2^-8 / 2,
-fp16 2^-11 / 2) is off by at most u in each value; a gradient product also reads dz rounded once, so
+Tolerances are relative 2-norms. A result rounded once to a type with unit roundoff u (bf16 2^-8,
+fp16 2^-11) is off by at most u in each value; a gradient product also reads dz rounded once, so
 its terms are off by u each, and the two add up to at most 2 u. fp32 results of sums over at most
 n values accumulate at most ~ n / 2 roundings of 2^-24 in the worst case and sqrt(n) of them in
 random order; n <= 2^14 here, so 2^-24 * 2^7 * 2 bounds them with room for the few operations around
@@ -515,3 +515,28 @@ def test_operand_changed_in_place_is_noticed():
         w.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("rows", [5, 1024])
+def test_activation_and_derivative_over_the_whole_range(act, dtype, rows):
+    """Value by value against float64, for z from the type's smallest to beyond where the activation is
+    z or 0: weights that are the identity make z = x, and dx = dy act'(z) (here dy = 1). The result is
+    the rounding of a value within the error of the fp32 arithmetic, so it lies between the roundings
+    of that interval's ends. The error: the tail polynomial 0.75e-7, and the exponential and the
+    reciprocal (2 units each plus 1.2 per unit of the exponent, on a probability <= 1/2) under 4e-7
+    together; times |z| in the value, and once more for z phi(z) in the derivative."""
+    n = rows * 64
+    mags = torch.logspace(-6, math.log10(40.0), n // 2 - 1, dtype=torch.float64)
+    z = torch.cat([-mags.flip(0), torch.zeros(2, dtype=torch.float64), mags]).to(dtype).view(rows, 64).to(DEV)
+    eye = torch.eye(64, dtype=dtype, device=DEV)
+    x = z.clone().requires_grad_()
+    y = text.linear(x, eye, activation=act)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    zd = z.double().requires_grad_()
+    want = act64(act, zd)
+    want_dx, = torch.autograd.grad(want.sum(), zd)
+    size = zd.detach().abs()
+    for got, exact, err in ((y.detach(), want.detach(), 5e-7 * size), (dx, want_dx, 1e-6 * (1 + size))):
+        assert ((got >= (exact - err).to(dtype)) & (got <= (exact + err).to(dtype))).all()
