@@ -68,86 +68,179 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b, int bf16) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// Activations in fp32. The tanh form of GELU is x * sigmoid(2 u) with u = sqrt(2/pi)(x + 0.044715 x^3)
-// (0.5 (1 + tanh u) = sigmoid(2 u)), which loses nothing for negative x. The erf form takes the
-// normal distribution's tail from Abramowitz and Stegun 7.1.26,
-//   erfc(x) = (a1 t + a2 t^2 + ... + a5 t^5) exp(-x^2),  t = 1 / (1 + 0.3275911 x),  x >= 0,
-// whose absolute error is at most 1.5e-7: one exponential and one reciprocal per value. The
-// epilogue of a 256 x 256 tile is issue-bound where K is small, and erff made a 1232 x 5120 x 1280
-// product with GELU 33.3 us, against 22.3 without it.
-__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
-// (P(X <= z), exp(-z^2 / 2)) of a standard normal X.
-__device__ __forceinline__ float2 normal_cdf(float z) {
-  const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.0f));
-  const float e = __expf(-0.5f * z * z);
-  float q = fmaf(t, 1.061405429f, -1.453152027f);
-  q = fmaf(t, q, 1.421413741f);
-  q = fmaf(t, q, -0.284496736f);
-  q = fmaf(t, q, 0.254829592f);
-  q *= 0.5f * t * e;
-  return make_float2(z < 0.0f ? q : 1.0f - q, e);
+// Two floats in one 64-bit register pair: the packed fp32 instructions of sm_100 do two operations per
+// issue slot, and issue slots are what bounds the epilogues and the norms of 16-bit rows.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
 }
-__device__ __forceinline__ float act_value(float z, int act) {
-  switch (act) {
-    case kActRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);
-    case kActSilu: return z * sigmoid_f(z);
-    case kActGelu: return z * normal_cdf(z).x;
-    case kActGeluTanh: return z * sigmoid_f(z * fmaf(0.0713548162726f, z * z, 1.5957691216057308f));
-    default: return z;
+__device__ __forceinline__ float2 split(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Eight values, as four pairs, from and to 16-bit words; the type is decided once per block.
+__device__ __forceinline__ void unpack8(const uint4& u, Pair (&f)[4], int bf16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if (bf16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[i] = pair(h.x, h.y);
+    }
   }
 }
-// Every value of a block through one activation; the switch stays outside the unrolled loops.
-template <int N, typename F>
-__device__ __forceinline__ void each_value(float (&v)[N], F f) {
+__device__ __forceinline__ uint4 pack8(const Pair* f, int bf16) {
+  uint32_t w[4];
+  if (bf16) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = f(v[j]);
+    for (int i = 0; i < 4; ++i) { const float2 v = split(f[i]); w[i] = pack_h2(v.x, v.y, 1); }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 v = split(f[i]); w[i] = pack_h2(v.x, v.y, 0); }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Activations in fp32, two values at a time. The tanh form of GELU is x * sigmoid(2 u) with
+// u = sqrt(2/pi)(x + 0.044715 x^3) (0.5 (1 + tanh u) = sigmoid(2 u)), which loses nothing for
+// negative x. The erf form takes the normal distribution's tail from Abramowitz and Stegun 7.1.26,
+//   erfc(x) = (a1 t + a2 t^2 + ... + a5 t^5) exp(-x^2),  t = 1 / (1 + 0.3275911 x),  x >= 0,
+// whose absolute error is at most 1.5e-7. Exponential and reciprocal are the instructions
+// ex2.approx and rcp.approx, whose results are good to about 2 units in the last place; what they
+// flush to zero is below 2^-126.
+__device__ __forceinline__ Pair both(float a) { return pair(a, a); }
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_ftz(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + 2^x) of both values.
+__device__ __forceinline__ Pair logistic2(Pair x) {
+  const float2 f = split(x);
+  const float2 d = split(pair(ex2_ftz(f.x), ex2_ftz(f.y)) + both(1.0f));
+  return pair(rcp_ftz(d.x), rcp_ftz(d.y));
+}
+__device__ __forceinline__ Pair silu_gate(Pair z) { return logistic2(z * both(-kLog2e)); }
+__device__ __forceinline__ Pair tanh_gate(Pair z) {
+  return logistic2(z * fma(z * z, both(-0.0713548162726f * kLog2e), both(-1.5957691216057308f * kLog2e)));
+}
+// P(X <= z) of a standard normal X, and e = exp(-z^2 / 2). |z| is cut at 40, where the tail has long
+// been 0; within it the two values can share one reciprocal, 1/a = b / (a b).
+__device__ __forceinline__ Pair normal_cdf(Pair z, Pair& e) {
+  const float2 f = split(z);
+  const Pair a = pair(fminf(fabsf(f.x), 40.0f), fminf(fabsf(f.y), 40.0f));
+  const float2 d = split(fma(a, both(0.3275911f * 0.70710678f), both(1.0f)));
+  const Pair t = pair(d.y, d.x) * both(rcp_ftz(d.x * d.y));
+  const float2 x = split(a * a * both(-0.5f * kLog2e));
+  e = pair(ex2_ftz(x.x), ex2_ftz(x.y));
+  Pair q = fma(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+  q = fma(t, q, both(0.5f * 1.421413741f));
+  q = fma(t, q, both(0.5f * -0.284496736f));
+  q = fma(t, q, both(0.5f * 0.254829592f));
+  const Pair tail = q * t * e;
+  const float2 lo = split(tail), hi = split(fma(tail, both(-1.0f), both(1.0f)));
+  return pair(f.x < 0.0f ? lo.x : hi.x, f.y < 0.0f ? lo.y : hi.y);
+}
+__device__ __forceinline__ Pair relu_pair(Pair z) {
+  const float2 f = split(z);
+  return pair(f.x <= 0.0f ? 0.0f : f.x, f.y <= 0.0f ? 0.0f : f.y);      // NaN stays
+}
+template <int ACT>
+__device__ __forceinline__ Pair act_pair(Pair z) {
+  Pair e;
+  if (ACT == kActRelu) return relu_pair(z);
+  if (ACT == kActSilu) return z * silu_gate(z);
+  if (ACT == kActGelu) return z * normal_cdf(z, e);
+  if (ACT == kActGeluTanh) return z * tanh_gate(z);
+  return z;
+}
+// Every value of a block through one activation; the switch stays outside the unrolled loops.
+template <int ACT, int N>
+__device__ __forceinline__ void each_pair(Pair (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = act_pair<ACT>(v[j]);
 }
 template <int N>
-__device__ __forceinline__ void act_values(float (&v)[N], int act) {
+__device__ __forceinline__ void act_values(Pair (&v)[N], int act) {
   switch (act) {
-    case kActRelu: each_value(v, [](float z) { return act_value(z, kActRelu); }); break;
-    case kActSilu: each_value(v, [](float z) { return act_value(z, kActSilu); }); break;
-    case kActGelu: each_value(v, [](float z) { return act_value(z, kActGelu); }); break;
-    case kActGeluTanh: each_value(v, [](float z) { return act_value(z, kActGeluTanh); }); break;
+    case kActRelu: each_pair<kActRelu>(v); break;
+    case kActSilu: each_pair<kActSilu>(v); break;
+    case kActGelu: each_pair<kActGelu>(v); break;
+    case kActGeluTanh: each_pair<kActGeluTanh>(v); break;
     default: break;
   }
 }
-// (activation, derivative)
-__device__ __forceinline__ float2 act_value_grad(float z, int act) {
-  switch (act) {
-    case kActRelu: return make_float2(z > 0.0f ? z : (z != z ? z : 0.0f), z > 0.0f ? 1.0f : 0.0f);
-    case kActSilu: {
-      const float s = sigmoid_f(z);
-      return make_float2(z * s, s * (1.0f + z * (1.0f - s)));
-    }
-    case kActGelu: {
-      const float2 c = normal_cdf(z);
-      return make_float2(z * c.x, c.x + z * c.y * 0.39894228040143268f);
-    }
-    case kActGeluTanh: {
-      const float s = sigmoid_f(z * fmaf(0.0713548162726f, z * z, 1.5957691216057308f));
-      const float du = fmaf(0.2140644488179f, z * z, 1.5957691216057308f);
-      const float q = s * (1.0f - s);            // 0 for a large |z|, where du may have overflowed
-      return make_float2(z * s, q == 0.0f ? s : s + z * q * du);
-    }
-    default: return make_float2(z, 1.0f);
+
+// Activation a and derivative da.
+template <int ACT>
+__device__ __forceinline__ void act_grad_pair(Pair z, Pair& a, Pair& da) {
+  a = z;
+  da = both(1.0f);
+  if (ACT == kActRelu) {
+    const float2 f = split(z);
+    a = relu_pair(z);
+    da = pair(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f);
+  } else if (ACT == kActSilu) {                 // s (1 + z (1 - s))
+    const Pair s = silu_gate(z);
+    a = z * s;
+    da = s * fma(z, fma(s, both(-1.0f), both(1.0f)), both(1.0f));
+  } else if (ACT == kActGelu) {                 // P(X <= z) + z phi(z)
+    Pair e;
+    const Pair c = normal_cdf(z, e);
+    a = z * c;
+    da = fma(z, e * both(0.39894228040143268f), c);
+  } else if (ACT == kActGeluTanh) {             // s + z s (1 - s) (2 u)'
+    const Pair s = tanh_gate(z);
+    a = z * s;
+    const Pair q = s * fma(s, both(-1.0f), both(1.0f));      // 0 for a large |z|, where (2 u)' may have overflowed
+    const Pair du = fma(z * z, both(0.2140644488179f), both(1.5957691216057308f));
+    const float2 qf = split(q), sf = split(s), g = split(fma(z * q, du, s));
+    da = pair(qf.x == 0.0f ? sf.x : g.x, qf.y == 0.0f ? sf.y : g.y);
   }
 }
-
-// f(j, activation, derivative) for every value of a block.
-template <int N, int ACT, typename F>
-__device__ __forceinline__ void each_grad(const float (&z)[N], F f) {
+// f(j, activation, derivative) for every pair of a block.
+template <int ACT, int N, typename F>
+__device__ __forceinline__ void each_grad(const Pair (&z)[N], F f) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) { const float2 a = act_value_grad(z[j], ACT); f(j, a.x, a.y); }
+  for (int j = 0; j < N; ++j) { Pair a, da; act_grad_pair<ACT>(z[j], a, da); f(j, a, da); }
 }
 template <int N, typename F>
-__device__ __forceinline__ void act_grads(const float (&z)[N], int act, F f) {
+__device__ __forceinline__ void act_grads(const Pair (&z)[N], int act, F f) {
   switch (act) {
-    case kActRelu: each_grad<N, kActRelu>(z, f); break;
-    case kActSilu: each_grad<N, kActSilu>(z, f); break;
-    case kActGelu: each_grad<N, kActGelu>(z, f); break;
-    case kActGeluTanh: each_grad<N, kActGeluTanh>(z, f); break;
-    default: each_grad<N, kActNone>(z, f); break;
+    case kActRelu: each_grad<kActRelu>(z, f); break;
+    case kActSilu: each_grad<kActSilu>(z, f); break;
+    case kActGelu: each_grad<kActGelu>(z, f); break;
+    case kActGeluTanh: each_grad<kActGeluTanh>(z, f); break;
+    default: each_grad<kActNone>(z, f); break;
   }
 }
 
@@ -247,19 +340,30 @@ __device__ __forceinline__ void block_load16(uint4* tile, const uint8_t* src, in
 }
 
 // 32 x 16 fp32 values (one row per lane) to `z`, 8 columns at a time.
-__device__ __forceinline__ void store_z(uint4* tile, const float (&v)[16], float* z, int64_t ldz, int rows, int cols) {
+__device__ __forceinline__ void store_z(uint4* tile, const Pair (&v)[8], float* z, int64_t ldz, int rows, int cols) {
   const int lane = lane_id();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (8 * h < cols) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        tile[block_unit(lane, u)] = make_uint4(__float_as_uint(v[8 * h + 4 * u]), __float_as_uint(v[8 * h + 4 * u + 1]),
-                                               __float_as_uint(v[8 * h + 4 * u + 2]), __float_as_uint(v[8 * h + 4 * u + 3]));
+      for (int u = 0; u < 2; ++u) {
+        const float2 a = split(v[4 * h + 2 * u]), b = split(v[4 * h + 2 * u + 1]);
+        tile[block_unit(lane, u)] = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+      }
       __syncwarp();
       block_store<4>(tile, reinterpret_cast<uint8_t*>(z + 8 * h), ldz * 4, rows, min(32, 4 * (cols - 8 * h)), true);
       __syncwarp();
     }
+  }
+}
+
+// Accumulator values and 16 biases (16-byte aligned, read by all lanes at once).
+__device__ __forceinline__ void add_bias(Pair (&v)[8], const uint32_t (&r)[16], const float* bias) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float4 b = reinterpret_cast<const float4*>(bias)[j];
+    v[2 * j] = pair(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])) + pair(b.x, b.y);
+    v[2 * j + 1] = pair(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])) + pair(b.z, b.w);
   }
 }
 
@@ -428,28 +532,24 @@ hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_const
           if (cols <= 0 || rows <= 0) continue;           // warp-uniform
           uint32_t r[16];
           tmem_ld16(taddr + c, r);
-          float v[16];
+          Pair v[8];
           if (EPI == kEpiGated) {
             uint32_t ru[16];
             tmem_ld16(taddr + out_cols + c, ru);
             tmem_wait_ld();
-            float u[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              v[j] = __uint_as_float(r[j]) + my_bias[bias_at + j];
-              u[j] = __uint_as_float(ru[j]) + my_bias[32 + bias_at + j];
-            }
+            Pair u[8];
+            add_bias(v, r, my_bias + bias_at);
+            add_bias(u, ru, my_bias + 32 + bias_at);
             if (p.z0 != nullptr) {
               store_z(tile_s, v, p.z0 + row0 * p.ldz + col0, p.ldz, rows, cols);
               store_z(tile_s, u, p.z1 + row0 * p.ldz + col0, p.ldz, rows, cols);
             }
             act_values(v, p.act);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] *= u[j];
+            for (int j = 0; j < 8; ++j) v[j] = v[j] * u[j];
           } else {
             tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) + my_bias[bias_at + j];
+            add_bias(v, r, my_bias + bias_at);
             if (p.z0 != nullptr) store_z(tile_s, v, p.z0 + row0 * p.ldz + col0, p.ldz, rows, cols);
             act_values(v, p.act);
             if (p.residual != nullptr) {
@@ -458,22 +558,16 @@ hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_const
               __syncwarp();
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                const uint4 w = tile_s[block_unit(lane, u)];
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                Pair f[4];
+                unpack8(tile_s[block_unit(lane, u)], f, p.bf16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  v[8 * u + 2 * i] += h_to_f(ws[i] & 0xFFFFu, p.bf16);
-                  v[8 * u + 2 * i + 1] += h_to_f(ws[i] >> 16, p.bf16);
-                }
+                for (int i = 0; i < 4; ++i) v[4 * u + i] = v[4 * u + i] + f[i];
               }
               __syncwarp();
             }
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            tile_s[block_unit(lane, u)] =
-                make_uint4(pack_h2(v[8 * u], v[8 * u + 1], p.bf16), pack_h2(v[8 * u + 2], v[8 * u + 3], p.bf16),
-                           pack_h2(v[8 * u + 4], v[8 * u + 5], p.bf16), pack_h2(v[8 * u + 6], v[8 * u + 7], p.bf16));
+          for (int u = 0; u < 2; ++u) tile_s[block_unit(lane, u)] = pack8(v + 4 * u, p.bf16);
           __syncwarp();
           block_store<2>(tile_s, out + (row0 * p.ldo + col0) * 2, p.ldo * 2, rows, 2 * cols, p.out_vec);
           __syncwarp();
@@ -552,7 +646,7 @@ __device__ __forceinline__ void finish_tile(const HGemmParams& p, const float* p
       s.x += b.x; s.y += b.y; s.z += b.z; s.w += b.w;
     }
     if (p.z0 != nullptr) *reinterpret_cast<float4*>(p.z0 + row * p.ldz + col) = s;     // rows are padded to 4 floats
-    float v[4] = {s.x, s.y, s.z, s.w};
+    Pair v[2] = {pair(s.x, s.y), pair(s.z, s.w)};
     act_values(v, p.act);
     if (EPI == kEpiGated) {
       float4 w = sum4(r, u + kOutUnits);
@@ -561,12 +655,15 @@ __device__ __forceinline__ void finish_tile(const HGemmParams& p, const float* p
         w.x += b.x; w.y += b.y; w.z += b.z; w.w += b.w;
       }
       if (p.z1 != nullptr) *reinterpret_cast<float4*>(p.z1 + row * p.ldz + col) = w;
-      v[0] *= w.x; v[1] *= w.y; v[2] *= w.z; v[3] *= w.w;
+      v[0] = v[0] * pair(w.x, w.y);
+      v[1] = v[1] * pair(w.z, w.w);
     } else if (p.residual != nullptr) {
       const float4 b = load4(reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr + col, n, p.res_vec, p.bf16);
-      v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+      v[0] = v[0] + pair(b.x, b.y);
+      v[1] = v[1] + pair(b.z, b.w);
     }
-    const uint32_t lo = pack_h2(v[0], v[1], p.bf16), hi = pack_h2(v[2], v[3], p.bf16);
+    const float2 v0 = split(v[0]), v1 = split(v[1]);
+    const uint32_t lo = pack_h2(v0.x, v0.y, p.bf16), hi = pack_h2(v1.x, v1.y, p.bf16);
     uint16_t* dst = out + row * p.ldo + col;
     if (p.out_vec && n >= 4) {
       *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);

@@ -60,35 +60,6 @@ __device__ __forceinline__ void load_w(const void* w, int64_t i, bool f32, float
   }
 }
 
-// Two floats in one 64-bit register pair: the packed fp32 instructions of sm_100 do two operations per
-// issue slot, and issue slots are what bounds the 16-bit rows.
-struct Pair { uint64_t v; };
-__device__ __forceinline__ Pair pair(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 split(Pair p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
-  return f;
-}
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-
 // A 16-byte unit of x's type as pairs of floats, and back.
 template <typename T>
 __device__ __forceinline__ void unit_pairs(const uint4& u, Pair (&f)[8 / sizeof(T)]) {

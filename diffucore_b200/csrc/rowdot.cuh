@@ -152,7 +152,9 @@ rowdot_kernel(const RowDotParams p) {
     }
     if (p.bias0 != nullptr) z += h_to_f(p.bias0[n], BF16);
     if (p.z0 != nullptr) p.z0[m * p.ldz + n] = z;
-    float y = act_value(z, p.act);
+    Pair v[1] = {both(z)};
+    act_values(v, p.act);
+    float y = dc::split(v[0]).x;
     if (GATED) {
       if (p.bias1 != nullptr) u += h_to_f(p.bias1[n], BF16);
       if (p.z1 != nullptr) p.z1[m * p.ldz + n] = u;
