@@ -435,10 +435,13 @@ RingPlan ring_plan(int64_t M, int64_t D, size_t es, bool vec, bool bwd) {
   n.tpr = D <= 1024 ? 32 : D <= 2048 ? 64 : D <= 4096 ? 128 : D <= 8192 ? 256 : 512;
   n.ept = D <= 256 ? 8 : D <= 512 ? 16 : 32;
   if (!vec && n.tpr == 64) { n.tpr = 128; n.ept = 16; }
+  // 16-bit rows of up to three quarters of a shape: the issue slots of absent values are what they
+  // wait for (19660 x 2560 bf16 46.9 us forward and 77.9 backward, 54.5 and 92.4 with 32).
+  if (es == 2 && n.ept == 32 && D <= n.tpr * 24) n.ept = 24;
   if (D > 16384 || (bwd && D > 8192)) return n;
   const int threads = std::max(128, n.tpr), rows = threads / n.tpr;
-  const bool shared_w = bwd && n.ept > 16 && (es == 4 || n.tpr < 128);        // RingCta::kSharedW
-  const int sm_threads = n.ept > 16 ? (!bwd ? 512 : shared_w ? 384 : 256) : (bwd ? 512 : 768);
+  const bool shared_w = bwd && n.ept == 32 && (es == 4 || n.tpr < 128);       // RingCta::kSharedW
+  const int sm_threads = n.ept > 16 ? (!bwd ? 512 : shared_w || n.ept == 24 ? 384 : 256) : (bwd ? 512 : 768);
   const int64_t w_bytes = shared_w ? n.tpr * n.ept * 4 : 0;
   n.slot = static_cast<int>(round_up(D * static_cast<int64_t>(es), 16)) + (vec ? 0 : 16);
   const int64_t stage = static_cast<int64_t>(rows) * (bwd ? 2 : 1) * n.slot;
@@ -492,19 +495,53 @@ int launch_ring(dc::NormParams p, const RingPlan& n, cudaStream_t st) {
 template <typename T, int E, bool BWD>
 int launch_ring_rows(const dc::NormParams& p, const RingPlan& n, cudaStream_t st) {
   switch (n.tpr * 100 + n.ept) {
-    case 3208: return launch_ring<T, E, 8, 32, BWD>(p, n, st);
-    case 3216: return launch_ring<T, E, 16, 32, BWD>(p, n, st);
     case 3232: return launch_ring<T, E, 32, 32, BWD>(p, n, st);
     case 12832: return launch_ring<T, E, 32, 128, BWD>(p, n, st);
     case 25632: return launch_ring<T, E, 32, 256, BWD>(p, n, st);
   }
+  if constexpr (E != 8) {                                 // narrower aligned rows: norm_narrow_kernel
+    if (n.ept == 16 && n.tpr == 32) return launch_ring<T, E, 16, 32, BWD>(p, n, st);
+  }
+  if constexpr (sizeof(T) == 2) {
+    switch (n.tpr * 100 + n.ept) {
+      case 3224: return launch_ring<T, E, 24, 32, BWD>(p, n, st);
+      case 12824: return launch_ring<T, E, 24, 128, BWD>(p, n, st);
+      case 25624: return launch_ring<T, E, 24, 256, BWD>(p, n, st);
+    }
+    if constexpr (E == 8) {
+      if (n.tpr == 64 && n.ept == 24) return launch_ring<T, E, 24, 64, BWD>(p, n, st);
+    }
+    if constexpr (!BWD) {
+      if (n.tpr == 512 && n.ept == 24) return launch_ring<T, E, 24, 512, BWD>(p, n, st);
+    }
+  }
   if constexpr (E == 1) {
+    if (n.ept == 8) return launch_ring<T, E, 8, 32, BWD>(p, n, st);
     if (n.tpr == 128) return launch_ring<T, E, 16, 128, BWD>(p, n, st);
   } else {
     if (n.tpr == 64) return launch_ring<T, E, 32, 64, BWD>(p, n, st);
   }
   if constexpr (!BWD) return launch_ring<T, E, 32, 512, BWD>(p, n, st);
   return fail("layer_norm: no kernel for rows of %d values", p.D);
+}
+
+// Narrow rows: threads per row of norm_narrow_kernel (0: too wide for it) and its CTAs.
+int narrow_threads(int64_t D, size_t es) {
+  const int64_t units = ceil_div(D * static_cast<int64_t>(es), 16);
+  for (int tpr = 4; tpr <= 32; tpr *= 2) {
+    if (units <= tpr * dc::kNarrowUnits) return tpr;
+  }
+  return 0;
+}
+int64_t narrow_ctas(int64_t M, int tpr, int per_sm) {
+  return std::min<int64_t>(ceil_div(M * tpr, dc::kNarrowThreads), 148 * per_sm);
+}
+template <typename T, bool BWD>
+int launch_narrow(const dc::NormParams& p, int tpr, cudaStream_t st) {
+  const unsigned ctas = static_cast<unsigned>(narrow_ctas(p.M, tpr, dc::NormNarrow<BWD>::kPerSm));
+  const auto kernel = tpr == 4 ? dc::norm_narrow_kernel<T, 4, BWD> : tpr == 8 ? dc::norm_narrow_kernel<T, 8, BWD>
+                    : tpr == 16 ? dc::norm_narrow_kernel<T, 16, BWD> : dc::norm_narrow_kernel<T, 32, BWD>;
+  return launch("layer_norm launch", kernel, ctas, dc::kNarrowThreads, 0, st, 0, p);
 }
 
 template <typename T, int E>
@@ -514,8 +551,8 @@ int launch_norm_grad_wide(const dc::NormParams& p, cudaStream_t st) {
   return launch("layer_norm_grad launch", dc::norm_dw_wide_kernel<T, E>, dim3(static_cast<unsigned>(ceil_div(p.D, 128 * E)), static_cast<unsigned>(p.parts)), 128, 0, st, 0, p, static_cast<int>(ceil_div(p.M, p.parts)));
 }
 
-// The forward register kernel, for few rows and narrow ones: the fewest threads per row that hold it
-// in two units (eight single values) each, up to 512 threads and eight units (32 values). Wider rows
+// The forward register kernel, for few rows that are not narrow: the fewest threads per row that hold
+// it in two units (eight single values) each, up to 512 threads and eight units (32 values). Wider rows
 // take the kernel for any width.
 template <typename T, bool VEC>
 int launch_norm_reg(const dc::NormParams& p, cudaStream_t st) {
@@ -527,17 +564,24 @@ int launch_norm_reg(const dc::NormParams& p, cudaStream_t st) {
   auto go = [&](auto kernel, int threads, int rows) {
     return launch("layer_norm launch", kernel, static_cast<unsigned>(ceil_div(p.M, rows)), threads, 0, st, 0, p);
   };
-  if (tpr == 32) return go(dc::norm_fwd_kernel<T, VEC, most, 32>, dc::NormCta<32>::kThreads, 8);
+  if constexpr (!VEC) {                                   // aligned rows of so few units are narrow
+    if (tpr == 32) return go(dc::norm_fwd_kernel<T, VEC, most, 32>, dc::NormCta<32>::kThreads, 8);
+  }
   if (tpr == 128) return go(dc::norm_fwd_kernel<T, VEC, most, 128>, 128, 1);
   if (nu <= most) return go(dc::norm_fwd_kernel<T, VEC, most, 512>, 512, 1);
   if (nu <= top) return go(dc::norm_fwd_kernel<T, VEC, top, 512>, 512, 1);
   return go(dc::norm_fwd_wide_kernel<T>, dc::kNormWide, 1);
 }
 
-// Which kernel a gradient runs in, and its partial rows: the ring, for unaligned rows where the window
-// of a row lies inside its neighbours; the kernel for wide aligned rows; else the ones for any width.
-enum NormGradPath { kNormGradRing, kNormGradLong, kNormGradWide };
+// Which kernel a gradient runs in, and its partial rows: the one for narrow aligned rows; the ring, for
+// unaligned rows where the window of a row lies inside its neighbours; the kernel for wide aligned
+// rows; else the ones for any width.
+enum NormGradPath { kNormGradNarrow, kNormGradRing, kNormGradLong, kNormGradWide };
 NormGradPath norm_grad_path(const dc::NormParams& p, bool vec, size_t es, int64_t* parts) {
+  if (const int tpr = vec ? narrow_threads(p.D, es) : 0) {
+    *parts = narrow_ctas(p.M, tpr, dc::NormNarrow<true>::kPerSm);
+    return kNormGradNarrow;
+  }
   const RingPlan r = ring_plan(p.M, p.D, es, vec, true);
   if (r.ctas > 0 && (vec || (p.ldx >= p.D && p.lddy >= p.D && p.D * es >= 16))) { *parts = r.ctas; return kNormGradRing; }
   if (vec && norm_bwd_plan(p.D, es, p.w_f32).stages > 0) { *parts = std::min<int64_t>(p.M, 148); return kNormGradLong; }
@@ -552,16 +596,17 @@ int launch_norm(const dc::NormParams& p, bool vec, cudaStream_t st) {
   if constexpr (BWD) {
     int64_t parts;
     switch (norm_grad_path(p, vec, sizeof(T), &parts)) {
+      case kNormGradNarrow: return launch_narrow<T, true>(p, narrow_threads(p.D, sizeof(T)), st);
       case kNormGradRing: return vec ? launch_ring_rows<T, E, true>(p, n, st) : launch_ring_rows<T, 1, true>(p, n, st);
       case kNormGradLong: return launch_norm_bwd<T>(p, norm_bwd_plan(p.D, sizeof(T), p.w_f32), st);
       default: return vec ? launch_norm_grad_wide<T, E>(p, st) : launch_norm_grad_wide<T, 1>(p, st);
     }
   } else {
-    // Many rows of more than 256 values (or unaligned ones) through the ring: 30000 x 2048 bf16 53 us
-    // against 66 in the register kernel; 100000 x 256 39 against 33.
+    if (const int tpr = vec ? narrow_threads(p.D, sizeof(T)) : 0) return launch_narrow<T, false>(p, tpr, st);
+    // Many wider rows through the ring: 30000 x 2048 bf16 53 us against 66 in the register kernel.
     const bool apart = p.ldx >= p.D && p.D * sizeof(T) >= 16;
     if (p.M >= 148 * 8 && n.ctas > 0) {
-      if (vec && p.D > 256) return launch_ring_rows<T, E, false>(p, n, st);
+      if (vec) return launch_ring_rows<T, E, false>(p, n, st);
       if (!vec && apart) return launch_ring_rows<T, 1, false>(p, n, st);
     }
     return vec ? launch_norm_reg<T, true>(p, st) : launch_norm_reg<T, false>(p, st);
