@@ -72,6 +72,8 @@ _SIGNATURES = {
     "dc_attn_int8_fwd_noalloc": (ctypes.c_int, [_c_p, _c_p, _c_p, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_i64,
                                                 _c_i64, _c_i64p, _c_i64p, _c_i64p, ctypes.c_float, ctypes.c_int,
                                                 _c_p, _c_i64p, _c_p]),
+    "dc_pad_rows": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(_c_p), _c_i64p, _c_i64p, _c_i64p, ctypes.POINTER(_c_p),
+                                   _c_i64p, _c_p]),
     "dc_linear": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64,
                                  ctypes.c_int, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p]),
     "dc_gated_linear": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p,

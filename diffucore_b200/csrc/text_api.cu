@@ -9,6 +9,7 @@
 #include "host.cuh"
 #include "sm100.cuh"
 #include "hgemm.cuh"
+#include "padrows.cuh"
 #include "rowdot.cuh"
 #include "textgrad.cuh"
 #include "norm.cuh"
@@ -243,6 +244,29 @@ int check_z(const char* what, const float* z, int64_t ldz, int64_t N) {
 }  // namespace
 
 extern "C" {
+
+int dc_pad_rows(int count, const void* const* src, const int64_t* ld, const int64_t* rows, const int64_t* cols,
+                void* const* dst, const int64_t* ldd, void* stream) {
+  if (count < 1 || count > dc::kPadMatrices) return fail("pad_rows: 1 to %d matrices", dc::kPadMatrices);
+  if (src == nullptr || ld == nullptr || rows == nullptr || cols == nullptr || dst == nullptr || ldd == nullptr)
+    return fail("pad_rows: null array");
+  dc::PadParams p = {};
+  for (int i = 0; i < count; ++i) {
+    if (rows[i] < 0 || cols[i] <= 0 || rows[i] > (1ll << 30) || cols[i] > (1ll << 30))
+      return fail("pad_rows: bad shape %lld x %lld", (long long)rows[i], (long long)cols[i]);
+    if (rows[i] == 0) continue;
+    if (src[i] == nullptr || dst[i] == nullptr) return fail("pad_rows: null pointer");
+    if (!aligned(src[i], 2) || !aligned(dst[i], 16)) return fail("pad_rows: src must be aligned to its element size, dst to 16 bytes");
+    if (ld[i] < 0 || ldd[i] % 8 || ldd[i] < cols[i] || ldd[i] > (1ll << 31) - 8) return fail("pad_rows: bad leading dimension");
+    p.m[p.count++] = {static_cast<const uint16_t*>(src[i]), static_cast<uint16_t*>(dst[i]), ld[i], ldd[i], rows[i],
+                      static_cast<int>(cols[i]), p.units};
+    p.units += rows[i] * (ldd[i] / 8);
+  }
+  if (p.count == 0) return DC_OK;
+  if (int r = check_sm100()) return r;
+  const int64_t ctas = std::min<int64_t>(ceil_div(p.units, dc::kPadThreads), 148 * 32);
+  return launch("pad_rows launch", dc::pad_rows_kernel, static_cast<unsigned>(ctas), dc::kPadThreads, 0, as_stream(stream), 0, p);
+}
 
 int dc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
               int64_t ldr, void* y, int64_t ldy, float* z, int64_t ldz, int dtype, int64_t M, int64_t N, int64_t K,

@@ -93,15 +93,44 @@ Tensor matrix_operand(const Tensor& t) {
 // Leading dimension of a matrix operand (any multiple of 8 will do for a single row).
 int64_t ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : pad(t.size(1), 8); }
 
+// The same for a call's operands, in place; those that need padding are copied by one launch.
+void matrix_operands(std::initializer_list<Tensor*> ts) {
+  const void* src[3];
+  void* dst[3];
+  int64_t ld_src[3], rows[3], cols[3], ld_dst[3];
+  int n = 0;
+  Tensor lead;
+  for (Tensor* t : ts) {
+    if (!t->defined() || tile_loadable(*t)) continue;
+    const bool same = !lead.defined() || lead.device() == t->device();
+    if (!t->is_cuda() || t->element_size() != 2 || t->stride(1) != 1 || !same || n == 3) {
+      *t = matrix_operand(*t);
+      continue;
+    }
+    if (!lead.defined()) lead = *t;
+    src[n] = t->data_ptr();
+    ld_src[n] = t->size(0) > 1 ? t->stride(0) : t->size(1);
+    rows[n] = t->size(0);
+    cols[n] = t->size(1);
+    ld_dst[n] = pad(cols[n], 8);
+    Tensor copy = at::empty({rows[n], ld_dst[n]}, t->options());
+    dst[n] = copy.data_ptr();
+    *t = copy.narrow(1, 0, cols[n]);
+    ++n;
+  }
+  if (n == 0) return;
+  Launch at_(lead);
+  check(dc_pad_rows(n, src, ld_src, rows, cols, dst, ld_dst, at_.stream));
+}
+
 constexpr int64_t kFewRows = 8;         // rows of x up to which the projections read any layout in place
 
-// A forward operand for `rows` rows of x. DC_HGEMM_PAIR forces the tiled kernels.
-Tensor projection_operand(const Tensor& t, int64_t rows) {
-  if (tile_loadable(t)) return t;
-  if (rows <= kFewRows && t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1))) {
-    if (getenv("DC_HGEMM_PAIR") == nullptr) return t;
-  }
-  return matrix_operand(t);
+// Forward operands for `rows` rows of x. DC_HGEMM_PAIR forces the tiled kernels.
+void projection_operands(std::initializer_list<Tensor*> ts, int64_t rows) {
+  bool in_place = rows <= kFewRows;
+  for (const Tensor* t : ts) in_place = in_place && t->stride(1) == 1 && (t->size(0) == 1 || t->stride(0) >= t->size(1));
+  if (in_place && getenv("DC_HGEMM_PAIR") == nullptr) return;
+  matrix_operands(ts);
 }
 
 // t [R, C] with unit inner stride, and its row stride (one row: its width).
@@ -155,7 +184,8 @@ std::pair<Tensor, Tensor> linear_raw(const Tensor& x_, const Tensor& w_, const O
     residual = unit_rows(*residual_);
   }
   Launch at_(x_);
-  const Tensor x = projection_operand(x_, M), w = projection_operand(w_, M);
+  Tensor x = x_, w = w_;
+  projection_operands({&x, &w}, M);
   Tensor y = at::empty({M, N}, x.options()), z;
   if (keep_z) z = at::empty({M, pad(N, 4)}, x.options().dtype(at::kFloat));
   check(dc_linear(ptr(x), ld(x), ptr(w), ld(w), ptr(bias), ptr(residual), residual.defined() ? residual.stride(0) : 0, ptr(y), N,
@@ -173,7 +203,8 @@ std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x_, const Tensor& wg_
   const int64_t M = x_.size(0), K = x_.size(1), N = wg_.size(0);
   const OptTensor bg = vector_arg("gated_linear", "b_gate", bg_, N), bu = vector_arg("gated_linear", "b_up", bu_, N);
   Launch at_(x_);
-  const Tensor x = projection_operand(x_, M), wg = projection_operand(wg_, M), wu = projection_operand(wu_, M);
+  Tensor x = x_, wg = wg_, wu = wu_;
+  projection_operands({&x, &wg, &wu}, M);
   Tensor h = at::empty({M, N}, x.options()), zg, zu;
   const int64_t ldz = pad(N, 4);
   if (keep_z) {
@@ -216,7 +247,8 @@ ActGrad act_grad_raw(const Tensor& dy_, const Tensor& z, const Tensor& z1, int a
 
 Tensor linear_dx_raw(const Tensor& dz_, const Tensor& w_, const Tensor& dz1, const Tensor& w1_) {
   Launch at_(dz_);
-  const Tensor dz = matrix_operand(dz_), w = matrix_operand(w_), w1 = w1_.defined() ? matrix_operand(w1_) : w1_;
+  Tensor dz = dz_, w = w_, w1 = w1_;
+  matrix_operands({&dz, &w, &w1});
   const int64_t M = dz.size(0), N = dz.size(1), K = w.size(1);
   Tensor dx = at::empty({M, K}, dz.options());
   check(dc_linear_dx(ptr(dz), ptr(dz1), ld(dz), ptr(w), ld(w), ptr(w1), w1.defined() ? ld(w1) : 0, ptr(dx), K,
@@ -226,7 +258,8 @@ Tensor linear_dx_raw(const Tensor& dz_, const Tensor& w_, const Tensor& dz1, con
 
 std::pair<Tensor, Tensor> linear_dw_raw(const Tensor& dz_, const Tensor& x_, const Tensor& dz1) {
   Launch at_(dz_);
-  const Tensor dz = matrix_operand(dz_), x = matrix_operand(x_);
+  Tensor dz = dz_, x = x_;
+  matrix_operands({&dz, &x});
   const int64_t M = dz.size(0), N = dz.size(1), K = x.size(1);
   Tensor dw = at::empty({N, K}, x.options()), dw1;
   if (dz1.defined()) dw1 = at::empty({N, K}, x.options());
@@ -361,7 +394,8 @@ struct Wants {
 struct LinearNode : torch::autograd::Function<LinearNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const OptTensor& bias, const OptTensor& residual,
                         int64_t act) {
-    const Tensor x = matrix_operand(x_), w = matrix_operand(w_);     // padded once for both passes
+    Tensor x = x_, w = w_;
+    matrix_operands({&x, &w});                                       // padded once for both passes
     const bool keep = act != DC_ACT_NONE && (x_.requires_grad() || w_.requires_grad() || (has(bias) && bias->requires_grad()));
     auto [y, z] = linear_raw(x, w, bias, static_cast<int>(act), residual, keep);
     ctx->save_for_backward({x, w, z});
@@ -385,7 +419,8 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       const ActGrad g = act_grad_raw(dy, z, Tensor(), static_cast<int>(ctx->saved_data["act"].toInt()), want[2], false);
       db = g.db;
       if (want[0] || want[1]) {
-        const Tensor dz = matrix_operand(g.dz);
+        Tensor dz = g.dz;
+        matrix_operands({&dz});
         if (want[0]) dx = linear_dx_raw(dz, w, Tensor(), Tensor());
         if (want[1]) dw = linear_dw_raw(dz, x, Tensor()).first;
       }
@@ -397,7 +432,8 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 struct GatedNode : torch::autograd::Function<GatedNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const OptTensor& bg,
                         const OptTensor& bu, int64_t act) {
-    const Tensor x = matrix_operand(x_), wg = matrix_operand(wg_), wu = matrix_operand(wu_);
+    Tensor x = x_, wg = wg_, wu = wu_;
+    matrix_operands({&x, &wg, &wu});
     auto [h, zg, zu] = gated_raw(x, wg, wu, bg, bu, static_cast<int>(act), true);
     ctx->save_for_backward({x, wg, wu, zg, zu});
     ctx->saved_data["act"] = act;
@@ -553,7 +589,10 @@ PYBIND11_MODULE(_text_ext, m) {
   m.def("gated_linear", &gated_linear, Free());
   m.def("layer_norm", &layer_norm, Free());
   m.def("embedding", &embedding, Free());
-  m.def("matrix_operand", &matrix_operand);
+  m.def("matrix_operand", [](Tensor t) {
+    matrix_operands({&t});
+    return t;
+  });
   m.def("linear_raw", [](const Tensor& x, const Tensor& w, const OptTensor& b, int act, const OptTensor& r, bool keep) {
     auto [y, z] = linear_raw(x, w, b, act, r, keep);
     return py::make_tuple(y, none_if_undefined(z));

@@ -267,6 +267,13 @@ int dc_selftest_wait_timeout(long long limit_cycles, int* status_dev, void* stre
 #define DC_ACT_GELU 3        /* 0.5 z (1 + erf(z / sqrt 2)) */
 #define DC_ACT_GELU_TANH 4   /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
 
+/* Copies of `count` (at most 3) matrices of 16-bit values with rows that are matrix operands:
+ * src[i] [rows[i], cols[i]] with row stride ld[i] (any, down to 0), element-aligned, to dst[i] with row
+ * stride ldd[i] (a multiple of 8 and at least cols[i]; what exceeds cols[i] becomes 0). The
+ * pointers are device pointers, the five arrays are the host's. */
+int dc_pad_rows(int count, const void* const* src, const int64_t* ld, const int64_t* rows, const int64_t* cols,
+                void* const* dst, const int64_t* ldd, void* stream);
+
 /* y[M, N] = act(z) + residual, z = x[M, K] . w[N, K]^T + bias. bias [N] and residual [M, N] (row
  * stride ldr, 0 for one row shared by all) may be null. `z`, if not null, receives z in fp32 for
  * the backward pass: 16-byte aligned, ldz a multiple of 4 and at least N rounded up to 4. */

@@ -540,3 +540,23 @@ def test_activation_and_derivative_over_the_whole_range(act, dtype, rows):
     size = zd.detach().abs()
     for got, exact, err in ((y.detach(), want.detach(), 5e-7 * size), (dx, want_dx, 1e-6 * (1 + size))):
         assert ((got >= (exact - err).to(dtype)) & (got <= (exact + err).to(dtype))).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (2, 7), (3, 8), (5, 9), (40, 17), (7, 4097), (1000, 333)])
+def test_operand_rows_of_any_alignment(rows, cols, dtype):
+    """Exact copies, zeros behind them, whatever the offset and the pitch; nothing outside the view is
+    read: the values around it are NaN."""
+    g = gen(rows, cols, dtype)
+    for offset in range(4):
+        for pitch in (cols, cols + 1, cols + 2, cols + 5):
+            store = torch.full((offset + rows * pitch + 3,), float("nan"), dtype=dtype, device=DEV)
+            view = store[offset:offset + rows * pitch].as_strided((rows, cols), (pitch, 1))
+            view.copy_(rand(g, rows, cols, dtype=dtype))
+            m = kernels.matrix_operand(view)
+            assert torch.equal(m, view) and m.data_ptr() % 16 == 0
+            if m.data_ptr() != view.data_ptr():
+                wide = m.as_strided((rows, m.stride(0)), (m.stride(0), 1))
+                assert wide.shape[1] % 8 == 0 and (wide[:, cols:] == 0).all()
+    shared = rand(g, 1, cols, dtype=dtype).expand(rows, cols)
+    assert torch.equal(kernels.matrix_operand(shared), shared)

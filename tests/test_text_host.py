@@ -113,3 +113,27 @@ def test_matrix_operand_pads_only_what_a_tile_load_cannot_take():
         assert m.stride(0) >= m.shape[1]
     one = torch.randn(3, 17).to(torch.bfloat16)[:1]
     assert kernels.matrix_operand(one).data_ptr() == one.data_ptr()          # one row: any pitch
+
+
+@no_gpu
+def test_pad_rows_arguments():
+    lib = _lib.load()
+
+    def pad(count=1, src=A, ld=21, rows=5, cols=21, dst=A, ldd=24):
+        i64 = ctypes.c_int64 * 1
+        ptr = ctypes.c_void_p * 1
+        return lib.dc_pad_rows(count, ptr(src), i64(ld), i64(rows), i64(cols), ptr(dst), i64(ldd), None)
+
+    refused(pad(count=0), b"1 to 3")
+    refused(pad(count=4), b"1 to 3")
+    refused(lib.dc_pad_rows(1, None, None, None, None, None, None, None), b"null array")
+    refused(pad(cols=0), b"bad shape")
+    refused(pad(rows=-1), b"bad shape")
+    refused(pad(src=None), b"null pointer")
+    refused(pad(src=A + 1), b"aligned")
+    refused(pad(dst=A + 8), b"aligned")
+    refused(pad(ldd=20), b"leading dimension")
+    refused(pad(ldd=16), b"leading dimension")
+    refused(pad(ld=-1), b"leading dimension")
+    assert pad(rows=0, src=None) == 0
+    refused(pad(), b"")                                     # no device here
