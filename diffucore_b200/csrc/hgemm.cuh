@@ -523,6 +523,15 @@ hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_const
       const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.M - row0));   // may be <= 0
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kPairBN;
       uint8_t* out = reinterpret_cast<uint8_t*>(second ? p.out1 : p.out);
+      // The accumulator goes back to the MMA thread once this warp's last block of it is in
+      // registers, before that block's arithmetic and stores.
+      bool returned = false;
+      auto give_back = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(&acc_empty[buf], 0));
+        returned = true;
+      };
 #pragma unroll 1
       for (int b = group; b < blocks; b += 4) {
 #pragma unroll 1
@@ -537,6 +546,7 @@ hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_const
             uint32_t ru[16];
             tmem_ld16(taddr + out_cols + c, ru);
             tmem_wait_ld();
+            if (b + 4 >= blocks && h == 1) give_back();
             Pair u[8];
             add_bias(v, r, my_bias + bias_at);
             add_bias(u, ru, my_bias + 32 + bias_at);
@@ -549,6 +559,7 @@ hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_const
             for (int j = 0; j < 8; ++j) v[j] = v[j] * u[j];
           } else {
             tmem_wait_ld();
+            if (b + 4 >= blocks && h == 1) give_back();
             add_bias(v, r, my_bias + bias_at);
             if (p.z0 != nullptr) store_z(tile_s, v, p.z0 + row0 * p.ldz + col0, p.ldz, rows, cols);
             act_values(v, p.act);
@@ -573,9 +584,7 @@ hgemm_pair_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_const
           __syncwarp();
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
+      if (!returned) give_back();
     }
   }
 

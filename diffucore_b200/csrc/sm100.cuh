@@ -288,6 +288,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(addr) : "memory");
 }
 
+// The same without ordering this thread's memory writes before it, for an arrival that hands over
+// tensor memory alone (its reads have completed: tcgen05.wait::ld, tcgen05.fence::before_thread_sync):
+// a release at cluster scope waits until the thread's stores to global memory have been performed.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" :: "r"(addr) : "memory");
+}
+
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
