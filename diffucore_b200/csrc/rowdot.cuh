@@ -77,6 +77,14 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// One value through an activation. A call of its own: inlined, its registers change the order of the
+// main loop's loads (gated 4 x 2 x 10240 x 4096 33.8 us, 29.1 so).
+__device__ __noinline__ float act_one(float z, int act) {
+  Pair v[1] = {both(z)};
+  act_values(v, act);
+  return dc::split(v[0]).x;
+}
+
 // NT: blocks of 8 rows of x (1 or 2). kAhead: steps whose loads are in flight at once.
 template <int NT, bool GATED, bool VEC, bool BF16, int kAhead>
 __global__ void __launch_bounds__(512)
@@ -152,9 +160,7 @@ rowdot_kernel(const RowDotParams p) {
     }
     if (p.bias0 != nullptr) z += h_to_f(p.bias0[n], BF16);
     if (p.z0 != nullptr) p.z0[m * p.ldz + n] = z;
-    Pair v[1] = {both(z)};
-    act_values(v, p.act);
-    float y = dc::split(v[0]).x;
+    float y = act_one(z, p.act);
     if (GATED) {
       if (p.bias1 != nullptr) u += h_to_f(p.bias1[n], BF16);
       if (p.z1 != nullptr) p.z1[m * p.ldz + n] = u;
