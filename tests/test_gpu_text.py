@@ -560,3 +560,41 @@ def test_operand_rows_of_any_alignment(rows, cols, dtype):
                 assert wide.shape[1] % 8 == 0 and (wide[:, cols:] == 0).all()
     shared = rand(g, 1, cols, dtype=dtype).expand(rows, cols)
     assert torch.equal(kernels.matrix_operand(shared), shared)
+
+
+@pytest.mark.parametrize("D", [4, 8, 16, 32, 40, 64, 128, 200, 256, 264, 512, 520, 640, 768, 1152, 1536, 2560, 3008, 4160,
+                               6144, 8200, 12288, 601, 1201, 2301, 5001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,affine", [(1, "same"), (1290, "same"), (1290, "fp32")])
+def test_layer_norm_widths(M, D, dtype, affine):
+    """Every width's launch shape, for one row and for more rows than there are row groups on the GPU: the
+    last of them are partly empty."""
+    M = M if M == 1 or D > 512 else 20011
+    test_layer_norm(M, D, dtype, affine)
+
+
+@pytest.mark.parametrize("D", [64, 96, 512])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_layer_norm_narrow_views_and_bad_rows(D, dtype):
+    """Row pitches of heads inside a wider projection; a row of NaN or infinities stays in its row of y
+    and dx, whatever rows share its warp."""
+    g = gen("heads", D, dtype)
+    wide, dys = rand(g, 300, 3 * D, dtype=dtype), rand(g, 300, 2 * D, dtype=dtype)
+    w, b = rand(g, D, dtype=dtype), rand(g, D, dtype=dtype)
+    x, dy = wide[:, D:2 * D], dys[:, D:]
+    leaf = x.detach().clone().requires_grad_()
+    want = text.layer_norm(leaf, w, b)
+    want_dx, = torch.autograd.grad(want, leaf, dy.contiguous())
+    view = x.detach().requires_grad_()
+    got = text.layer_norm(view, w, b)
+    got_dx, = torch.autograd.grad(got, view, dy)
+    assert torch.equal(got, want) and torch.equal(got_dx, want_dx)
+    bad = x.clone()
+    bad[7, 3], bad[100, 0], bad[299, D - 1] = float("nan"), float("inf"), -float("inf")
+    leaf = bad.requires_grad_()
+    y = text.layer_norm(leaf, w, b)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    keep = torch.ones(300, dtype=torch.bool, device=DEV)
+    keep[[7, 100, 299]] = False
+    assert torch.equal(y[keep], want[keep]) and torch.equal(dx[keep], want_dx[keep])
+    assert y[~keep].isnan().any(-1).all() and dx[~keep].isnan().any(-1).all()
