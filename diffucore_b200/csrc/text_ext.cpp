@@ -78,6 +78,10 @@ Tensor workspace(const Tensor& like, size_t bytes) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
 int64_t pad(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+// Rows of the tensors that only the kernels see (kept pre-activations, dz) start on 64 bytes: rows on
+// 16 split the kernels' 32-byte accesses over two sectors (6580 x 3291 x 256 with z kept 51.8 us,
+// 75.2 on 16 bytes).
+constexpr int64_t kZPad = 16, kDzPad = 32;
 
 // Whether a TMA tile load takes the rows of t [R, C]: unit inner stride, 16-byte aligned rows that do
 // not overlap.
@@ -187,7 +191,7 @@ std::pair<Tensor, Tensor> linear_raw(const Tensor& x_, const Tensor& w_, const O
   Tensor x = x_, w = w_;
   projection_operands({&x, &w}, M);
   Tensor y = at::empty({M, N}, x.options()), z;
-  if (keep_z) z = at::empty({M, pad(N, 4)}, x.options().dtype(at::kFloat));
+  if (keep_z) z = at::empty({M, pad(N, kZPad)}, x.options().dtype(at::kFloat));
   check(dc_linear(ptr(x), ld(x), ptr(w), ld(w), ptr(bias), ptr(residual), residual.defined() ? residual.stride(0) : 0, ptr(y), N,
                   fptr(z), keep_z ? z.size(1) : 0, dt, M, N, K, act, at_.stream));
   return {y, z};
@@ -206,7 +210,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x_, const Tensor& wg_
   Tensor x = x_, wg = wg_, wu = wu_;
   projection_operands({&x, &wg, &wu}, M);
   Tensor h = at::empty({M, N}, x.options()), zg, zu;
-  const int64_t ldz = pad(N, 4);
+  const int64_t ldz = pad(N, kZPad);
   if (keep_z) {
     zg = at::empty({M, ldz}, x.options().dtype(at::kFloat));
     zu = at::empty({M, ldz}, x.options().dtype(at::kFloat));
@@ -225,7 +229,7 @@ ActGrad act_grad_raw(const Tensor& dy_, const Tensor& z, const Tensor& z1, int a
     g.dz = dy_;
     return g;
   }
-  const int64_t M = dy_.size(0), N = dy_.size(1), lddz = pad(N, 8);
+  const int64_t M = dy_.size(0), N = dy_.size(1), lddz = pad(N, kDzPad);
   Launch at_(dy_);
   Tensor dy = unit_rows(dy_);
   if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
