@@ -431,7 +431,8 @@ int dc_act_grad(const void* dy, int64_t lddy, const float* z, const float* z1, i
   const cudaStream_t st = as_stream(stream);
   const dim3 grid(static_cast<unsigned>(ceil_div(N, dc::kGradCols)), static_cast<unsigned>(blocks));
   const dim3 block(dc::kGradX, dc::kGradY);
-  const auto kernel = z1 != nullptr ? dc::act_grad_kernel<2> : z != nullptr ? dc::act_grad_kernel<1> : dc::act_grad_kernel<0>;
+  const auto kernel = z1 != nullptr ? (p.dy_vec ? dc::act_grad_kernel<2, false> : dc::act_grad_kernel<2, true>)
+                      : z != nullptr ? dc::act_grad_kernel<1, false> : dc::act_grad_kernel<0, false>;
   if ((r = launch("act_grad launch", kernel, grid, block, 0, st, 0, p))) return r;
   if (db != nullptr) return colsum_finish(p.part0, p.part1, ldp, blocks, N, db, db1, dtype, st);
   return DC_OK;

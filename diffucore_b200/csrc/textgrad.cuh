@@ -39,6 +39,40 @@ __device__ __forceinline__ uint4 load8_bits(const uint16_t* src, int n, bool vec
   for (int i = 0; i < 8; ++i) h[i] = i < n ? __ldg(src + i) : 0u;
   return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
+// Eight values at any even address as the words that hold them (WORDS), five where the first value is the
+// second half of a word. Near the ends of the matrix [base, end), where a word could reach outside,
+// and for fewer than 8 values they are read one by one into the same layout.
+template <bool WORDS> struct Raw8 { uint4 w; };
+template <> struct Raw8<true> { uint4 w; uint32_t last; };
+__device__ __forceinline__ Raw8<true> load8_words(const uint16_t* src, int n, const uint16_t* base, const uint16_t* end) {
+  Raw8<true> v;
+  const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 2) >> 1);
+  if (n >= 8 && (skip == 0 || (src > base && src + 9 <= end))) {
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(src - skip);
+    v.w = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+    v.last = skip ? __ldg(q + 4) : 0u;
+    return v;
+  }
+  uint32_t h[9];
+#pragma unroll
+  for (int i = 0; i < 9; ++i) {
+    const int k = i - skip;
+    h[i] = k >= 0 && k < n && k < 8 ? __ldg(src + k) : 0u;
+  }
+  v.w = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+  v.last = h[8];
+  return v;
+}
+template <bool WORDS>
+__device__ __forceinline__ uint4 bits8(const Raw8<WORDS>& v, const uint16_t* src) {
+  if constexpr (WORDS) {
+    if (reinterpret_cast<uintptr_t>(src) & 2)
+      return make_uint4(__funnelshift_r(v.w.x, v.w.y, 16), __funnelshift_r(v.w.y, v.w.z, 16), __funnelshift_r(v.w.z, v.w.w, 16),
+                        __funnelshift_r(v.w.w, v.last, 16));
+  }
+  return v.w;
+}
+
 struct Float8 { float4 a, b; };
 __device__ __forceinline__ Float8 load8_floats(const float* src, bool hi) {
   const float4* q = reinterpret_cast<const float4*>(src);
@@ -55,8 +89,10 @@ __device__ __forceinline__ void pairs_of(const Float8& v, Pair (&f)[4]) {
 // loaded they wait for each row in turn (57.3 us against 41.8 for 8192 x 4096 without an activation).
 // Three CTAs per SM where registers allow it (gelu_tanh 45.7 us, 49.3 with two); at 8192 x 4096
 // 41.8 us without an activation (6430 GB/s), 45.9 with GELU, 4.9 more with the bias's gradient;
-// gated 4173 x 5464 with SiLU 51.6 us (6190 GB/s).
-template <int FORM>
+// gated 4173 x 5464 with SiLU 51.6 us (6190 GB/s). Rows of dy that 16-byte accesses do not fit are read
+// as words in the gated form (4173 x 5461 with biases 68.1 us, 77.5 by values); the other forms have no
+// registers to spare for them (20000 x 1001 46.9 us, 43.7 by values).
+template <int FORM, bool WORDS>
 __global__ void __launch_bounds__(kGradX * kGradY, FORM == 2 ? 2 : 3)
 act_grad_kernel(const ActGradParams p) {
   constexpr int kAhead = FORM == 0 ? 8 : FORM == 1 ? 3 : 2;
@@ -72,13 +108,15 @@ act_grad_kernel(const ActGradParams p) {
   for (int j = 0; j < 4; ++j) s0[j] = s1[j] = both(0.f);
   if (n > 0) {
     for (int64_t rb = r0 + threadIdx.y; rb < r1; rb += kGradY * kAhead) {
-      uint4 dv[kAhead];
+      Raw8<WORDS> dv[kAhead];
       Float8 zv[kAhead], uv[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int64_t r = rb + k * kGradY;
         if (r < r1) {
-          dv[k] = load8_bits(p.dy + r * p.lddy + col, n, p.dy_vec);
+          const uint16_t* dy = p.dy + r * p.lddy + col;
+          if constexpr (WORDS) dv[k] = load8_words(dy, n, p.dy, p.dy + (p.M - 1) * p.lddy + p.N);
+          else dv[k].w = load8_bits(dy, n, p.dy_vec);
           if (FORM >= 1) zv[k] = load8_floats(p.z0 + r * p.ldz + col, z_hi);
           if (FORM == 2) uv[k] = load8_floats(p.z1 + r * p.ldz + col, z_hi);
         }
@@ -88,7 +126,7 @@ act_grad_kernel(const ActGradParams p) {
         const int64_t r = rb + k * kGradY;
         if (r >= r1) break;
         Pair d[4], z[4], u[4];
-        unpack8(dv[k], d, p.bf16);
+        unpack8(bits8<WORDS>(dv[k], p.dy + r * p.lddy + col), d, p.bf16);
         if (FORM >= 1) pairs_of(zv[k], z);
         if (FORM == 2) pairs_of(uv[k], u);
         if (FORM == 1) {
