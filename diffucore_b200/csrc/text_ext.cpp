@@ -97,7 +97,8 @@ Tensor matrix_operand(const Tensor& t) {
 // Leading dimension of a matrix operand (any multiple of 8 will do for a single row).
 int64_t ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : pad(t.size(1), 8); }
 
-// The same for a call's operands, in place; those that need padding are copied by one launch.
+// The same for a call's operands, in place; those that need padding are copied by one launch (a fourth
+// by torch).
 void matrix_operands(std::initializer_list<Tensor*> ts) {
   const void* src[3];
   void* dst[3];
@@ -222,8 +223,30 @@ std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x_, const Tensor& wg_
 
 struct ActGrad { Tensor dz, dz1, db, db1; };
 
+// A kept pre-activation of dy [M, N]: fp32 rows whose memory holds N rounded up to 4 values, as the
+// kernels read it.
+void check_kept(const char* name, const Tensor& z, const Tensor& dy) {
+  if (!z.defined()) return;
+  if (z.scalar_type() != at::kFloat || z.device() != dy.device())
+    throw py::type_error(cat("act_grad: ", name, " is ", z.scalar_type(), " on ", z.device(), ", expected fp32 on ", dy.device()));
+  const int64_t M = dy.size(0), N = dy.size(1);
+  if (z.dim() != 2 || z.size(0) != M || z.size(1) < N || (z.size(1) > 1 && z.stride(1) != 1))
+    throw py::value_error(cat("act_grad: ", name, " ", shape_of(z), " is not the kept pre-activation of dy ", shape_of(dy)));
+  const int64_t room = static_cast<int64_t>(z.storage().nbytes() / sizeof(float)) - z.storage_offset();
+  if (M > 0 && (M - 1) * z.stride(0) + pad(N, 4) > room)
+    throw py::value_error(cat("act_grad: the rows of ", name, " must hold ", pad(N, 4), " values, ", N, " rounded up to 4"));
+}
+
 // dz (dy itself without z), dz1, db and db1 from dy and the kept pre-activations.
 ActGrad act_grad_raw(const Tensor& dy_, const Tensor& z, const Tensor& z1, int act, bool bias, bool bias1) {
+  check_text("act_grad", dy_, false);
+  if (dy_.dim() != 2) throw py::value_error(cat("act_grad: dy must be [M, N], got ", shape_of(dy_)));
+  if (z1.defined() && !z.defined()) throw py::value_error("act_grad: z1 goes with z");
+  if (bias1 && !z1.defined()) throw py::value_error("act_grad: the second bias gradient needs z1");
+  check_kept("z", z, dy_);
+  check_kept("z1", z1, dy_);
+  if (z1.defined() && z1.stride(0) != z.stride(0) && z.size(0) > 1)
+    throw py::value_error("act_grad: z and z1 must have the same row stride");
   ActGrad g;
   if (!z.defined() && !bias) {
     g.dz = dy_;
@@ -249,10 +272,31 @@ ActGrad act_grad_raw(const Tensor& dy_, const Tensor& z, const Tensor& z1, int a
   return g;
 }
 
-Tensor linear_dx_raw(const Tensor& dz_, const Tensor& w_, const Tensor& dz1, const Tensor& w1_) {
+// dz and w (or x) of a backward product, and dz's twin: 2-D tensors of one type on one device.
+void check_product(const char* what, const Tensor& dz, const char* name, const Tensor& t, const Tensor& dz1) {
+  const OptTensor to(t), d1(dz1);
+  check_text(what, dz, false, {{name, &to}, {"dz1", &d1}});
+  if (dz.dim() != 2 || t.dim() != 2) throw py::value_error(cat(what, ": dz ", shape_of(dz), " and ", name, " ", shape_of(t), " must be matrices"));
+  if (dz1.defined() && dz1.sizes() != dz.sizes()) throw py::value_error(cat(what, ": dz1 ", shape_of(dz1), " does not match dz ", shape_of(dz)));
+}
+// dz and dz1 as matrix operands with one leading dimension.
+void same_rows(Tensor& dz, Tensor& dz1) {
+  if (!dz1.defined() || ld(dz) == ld(dz1)) return;
+  for (Tensor* t : {&dz, &dz1}) *t = at::empty({t->size(0), pad(t->size(1), 8)}, t->options()).narrow(1, 0, t->size(1)).copy_(*t);
+}
+
+Tensor linear_dx_raw(const Tensor& dz_, const Tensor& w_, const Tensor& dz1_, const Tensor& w1_) {
+  check_product("linear_dx", dz_, "w", w_, dz1_);
+  if (dz1_.defined() != w1_.defined()) throw py::value_error("linear_dx: dz1 and w1 go together");
+  if (w1_.defined()) {
+    check_product("linear_dx", dz_, "w1", w1_, dz1_);
+    if (w1_.sizes() != w_.sizes()) throw py::value_error(cat("linear_dx: w1 ", shape_of(w1_), " does not match w ", shape_of(w_)));
+  }
+  if (dz_.size(1) != w_.size(0)) throw py::value_error(cat("linear_dx: dz ", shape_of(dz_), " does not match w ", shape_of(w_)));
   Launch at_(dz_);
-  Tensor dz = dz_, w = w_, w1 = w1_;
-  matrix_operands({&dz, &w, &w1});
+  Tensor dz = dz_, w = w_, dz1 = dz1_, w1 = w1_;
+  matrix_operands({&dz, &w, &dz1, &w1});
+  same_rows(dz, dz1);
   const int64_t M = dz.size(0), N = dz.size(1), K = w.size(1);
   Tensor dx = at::empty({M, K}, dz.options());
   check(dc_linear_dx(ptr(dz), ptr(dz1), ld(dz), ptr(w), ld(w), ptr(w1), w1.defined() ? ld(w1) : 0, ptr(dx), K,
@@ -260,10 +304,13 @@ Tensor linear_dx_raw(const Tensor& dz_, const Tensor& w_, const Tensor& dz1, con
   return dx;
 }
 
-std::pair<Tensor, Tensor> linear_dw_raw(const Tensor& dz_, const Tensor& x_, const Tensor& dz1) {
+std::pair<Tensor, Tensor> linear_dw_raw(const Tensor& dz_, const Tensor& x_, const Tensor& dz1_) {
+  check_product("linear_dw", dz_, "x", x_, dz1_);
+  if (dz_.size(0) != x_.size(0)) throw py::value_error(cat("linear_dw: dz ", shape_of(dz_), " does not match x ", shape_of(x_)));
   Launch at_(dz_);
-  Tensor dz = dz_, x = x_;
-  matrix_operands({&dz, &x});
+  Tensor dz = dz_, x = x_, dz1 = dz1_;
+  matrix_operands({&dz, &x, &dz1});
+  same_rows(dz, dz1);
   const int64_t M = dz.size(0), N = dz.size(1), K = x.size(1);
   Tensor dw = at::empty({N, K}, x.options()), dw1;
   if (dz1.defined()) dw1 = at::empty({N, K}, x.options());
@@ -293,6 +340,7 @@ at::ScalarType norm_affine(const char* what, const Tensor& x, OptTensor& w, OptT
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x_, OptTensor w, OptTensor b, double eps, bool keep_stats) {
   const int dt = check_text("layer_norm", x_, true);
+  if (x_.dim() != 2) throw py::value_error(cat("layer_norm: x must be [M, D], got ", shape_of(x_)));
   Launch at_(x_);
   const at::ScalarType kind = norm_affine("layer_norm", x_, w, b);
   const Tensor x = unit_rows(x_);
@@ -307,27 +355,44 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x_, OptTensor w,
   return {y, mean, rstd};
 }
 
-// dw and db come in `kind` (x's type or fp32).
-std::tuple<Tensor, Tensor, Tensor> layer_norm_grad_raw(const Tensor& dy_, const Tensor& x_, const OptTensor& w_, const Tensor& mean,
-                                                       const Tensor& rstd, bool weight, bool bias, at::ScalarType kind) {
+// A row statistic [M] that layer_norm_raw kept.
+Tensor kept_stat(const char* name, const Tensor& t, const Tensor& x) {
+  if (t.scalar_type() != at::kFloat || t.device() != x.device())
+    throw py::type_error(cat("layer_norm_grad: ", name, " is ", t.scalar_type(), " on ", t.device(), ", expected fp32 on ", x.device()));
+  if (t.dim() != 1 || t.size(0) != x.size(0))
+    throw py::value_error(cat("layer_norm_grad: ", name, " must have shape (", x.size(0), ",), got ", shape_of(t)));
+  return t.contiguous();
+}
+
+// dw and db come in `kind` (x's type or fp32), computed in fp32 where w is fp32.
+std::tuple<Tensor, Tensor, Tensor> layer_norm_grad_raw(const Tensor& dy_, const Tensor& x_, const OptTensor& w_, const Tensor& mean_,
+                                                       const Tensor& rstd_, bool weight, bool bias, at::ScalarType kind) {
   const OptTensor xo(x_);
   const int dt = check_text("layer_norm_grad", dy_, true, {{"x", &xo}});
+  if (x_.dim() != 2 || dy_.sizes() != x_.sizes())
+    throw py::value_error(cat("layer_norm_grad: dy ", shape_of(dy_), " does not match x ", shape_of(x_), ", [M, D]"));
   Launch at_(x_);
-  OptTensor w;
-  if (has(w_)) w = w_->to(kind).contiguous();
+  OptTensor w = w_, none;
+  at::ScalarType sums = norm_affine("layer_norm_grad", x_, w, none);
+  if (kind != x_.scalar_type() && kind != at::kFloat)
+    throw py::type_error(cat("layer_norm_grad: gradients in ", kind, ", expected ", x_.scalar_type(), " or fp32"));
+  if (kind == at::kFloat) sums = kind;
+  if (has(w)) w = w->to(sums);
+  const Tensor mean = kept_stat("mean", mean_, x_), rstd = kept_stat("rstd", rstd_, x_);
   const Tensor dy = unit_rows(dy_), x = unit_rows(x_);
   const int64_t M = x.size(0), D = x.size(1);
   Tensor dx = at::empty({M, D}, x.options()), dw, db, ws;
   size_t bytes = 0;
   if (weight || bias) {
-    dw = at::empty({D}, x.options().dtype(kind));
-    if (bias) db = at::empty({D}, x.options().dtype(kind));
+    dw = at::empty({D}, x.options().dtype(sums));
+    if (bias) db = at::empty({D}, x.options().dtype(sums));
     check(dc_layer_norm_grad_workspace(M, D, &bytes));
     ws = workspace(x, bytes);
   }
-  check(dc_layer_norm_grad(ptr(dy), row_stride(dy), ptr(x), row_stride(x), ptr(w), dtype_code(kind), fptr(mean), fptr(rstd), ptr(dx),
+  check(dc_layer_norm_grad(ptr(dy), row_stride(dy), ptr(x), row_stride(x), ptr(w), dtype_code(sums), fptr(mean), fptr(rstd), ptr(dx),
                            D, ptr(dw), ptr(db), ptr(ws), bytes, dt, M, D, at_.stream));
-  if (!weight) dw = Tensor();
+  dw = weight ? dw.to(kind) : Tensor();
+  if (bias) db = db.to(kind);
   return {dx, dw, db};
 }
 
@@ -340,6 +405,7 @@ Tensor check_ids(const char* what, const Tensor& ids, const Tensor& like) {
 
 Tensor embedding_raw(const Tensor& ids_, const Tensor& table_, double scale) {
   const int dt = check_text("embedding", table_, true);
+  if (table_.dim() != 2) throw py::value_error(cat("embedding: table must be [V, D], got ", shape_of(table_)));
   const Tensor ids = check_ids("embedding", ids_, table_);
   Launch at_(table_);
   const int64_t V = table_.size(0), D = table_.size(1), T = ids.size(0);
@@ -353,6 +419,7 @@ Tensor embedding_raw(const Tensor& ids_, const Tensor& table_, double scale) {
 
 Tensor embedding_grad_raw(const Tensor& dy_, const Tensor& ids_, int64_t V, double scale, int64_t padding) {
   const int dt = check_text("embedding_grad", dy_, true);
+  if (dy_.dim() != 2) throw py::value_error(cat("embedding_grad: dy must be [T, D], got ", shape_of(dy_)));
   const Tensor ids = check_ids("embedding_grad", ids_, dy_);
   const int64_t T = dy_.size(0), D = dy_.size(1);
   if (ids.size(0) != T) throw py::value_error(cat("embedding_grad: ", ids.size(0), " ids for ", T, " rows"));
@@ -594,6 +661,7 @@ PYBIND11_MODULE(_text_ext, m) {
   m.def("layer_norm", &layer_norm, Free());
   m.def("embedding", &embedding, Free());
   m.def("matrix_operand", [](Tensor t) {
+    if (t.dim() != 2) throw py::value_error(cat("matrix_operand: expected a matrix, got ", shape_of(t)));
     matrix_operands({&t});
     return t;
   });
