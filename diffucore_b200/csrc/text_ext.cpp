@@ -47,9 +47,23 @@ int dtype_code(at::ScalarType t) {
 
 using Named = std::pair<const char*, const OptTensor*>;
 
+// A forward-mode tangent would not reach the result: the kernels see the primal values alone.
+void refuse_tangent(const char* what, const Tensor& t) {
+  if (t._fw_grad(0).defined())
+    throw std::runtime_error(cat("diffucore_b200: ", what, " has no forward-mode derivative (an argument is a dual tensor); differentiate it in "
+                                 "reverse mode"));
+}
+void refuse_tangents(const char* what, std::initializer_list<const OptTensor*> ts) {
+  for (const OptTensor* t : ts)
+    if (has(*t)) refuse_tangent(what, **t);
+}
+
 // dtype code of `lead`, a CUDA tensor in bf16 or fp16 (or fp32 where `floats`); the others share its
-// type and device.
+// type and device. No tensor carries a forward-mode tangent.
 int check_text(const char* what, const Tensor& lead, bool floats, std::initializer_list<Named> others = {}) {
+  refuse_tangent(what, lead);
+  for (const Named& n : others)
+    if (has(*n.second)) refuse_tangent(what, **n.second);
   if (!lead.is_cuda())
     throw std::runtime_error(cat("diffucore_b200 kernels run on CUDA tensors only (got a ", c10::DeviceTypeName(lead.device().type(), true),
                                  " tensor); there is no CPU path"));
@@ -325,6 +339,7 @@ at::ScalarType norm_affine(const char* what, const Tensor& x, OptTensor& w, OptT
   std::optional<at::ScalarType> kind;
   for (auto& [name, t] : {std::pair<const char*, OptTensor*>{"weight", &w}, {"bias", &b}}) {
     if (!has(*t)) continue;
+    refuse_tangent(what, **t);
     if ((*t)->device() != x.device() || ((*t)->scalar_type() != x.scalar_type() && (*t)->scalar_type() != at::kFloat))
       throw py::type_error(cat(what, ": ", name, " is ", (*t)->scalar_type(), " on ", (*t)->device(), ", expected ",
                                x.scalar_type(), " or fp32 on ", x.device()));
@@ -605,6 +620,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias, int64_t a
     res = flat(*residual);
   }
   const OptTensor xo(x), wo(w);
+  refuse_tangents("linear", {&xo, &wo, &bias, &residual});
   const Tensor x2 = flat(x);
   const Tensor y = wants_grad({&xo, &wo, &bias, &residual})
                        ? LinearNode::apply(x2, w, bias, res, act)
@@ -616,6 +632,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const O
   if (wg.dim() != 2) throw py::value_error(cat("gated_linear: w_gate must be [N, K], got ", shape_of(wg)));
   check_width("gated_linear", x, wg.size(1));
   const OptTensor xo(x), go(wg), uo(wu);
+  refuse_tangents("gated_linear", {&xo, &go, &uo, &bg, &bu});
   const Tensor x2 = flat(x);
   const Tensor h = wants_grad({&xo, &go, &uo, &bg, &bu})
                        ? GatedNode::apply(x2, wg, wu, bg, bu, act)
@@ -626,6 +643,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const O
 Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
   if (x.dim() < 1) throw py::value_error("layer_norm: expected at least one dimension");
   const OptTensor xo(x);
+  refuse_tangents("layer_norm", {&xo, &w, &b});
   const Tensor x2 = flat(x);
   const Tensor y = wants_grad({&xo, &w, &b}) ? LayerNormNode::apply(x2, w, b, eps) : std::get<0>(layer_norm_raw(x2, w, b, eps, false));
   return unflat(y, x, x.size(-1));
@@ -641,6 +659,7 @@ Tensor embedding(const Tensor& ids, const Tensor& table, double scale, std::opti
     pad_id = *padding < 0 ? *padding + V : *padding;
   }
   const OptTensor to(table);
+  refuse_tangents("embedding", {&to});
   const Tensor flat_ids = ids.dim() == 1 ? ids : ids.reshape({-1});
   const Tensor y = wants_grad({&to}) ? EmbeddingNode::apply(flat_ids, table, scale, pad_id) : embedding_raw(flat_ids, table, scale);
   if (ids.dim() == 1) return y;

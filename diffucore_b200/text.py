@@ -11,7 +11,8 @@ All take CUDA tensors with any leading dimensions and run on the current stream 
 device. The projections take bf16 and fp16, the norm and the embedding fp32 as well. Sums are fp32
 (products, norm statistics, weight gradients) in a fixed order, so results repeat bit for bit;
 outputs and gradients are rounded once to their type. Argument checks, allocation and the autograd
-nodes are native (``_text_ext.so``). The gradients cannot be differentiated again. Pre-activations are kept for the backward pass
+nodes are native (``_text_ext.so``). The gradients cannot be differentiated again, and there is no
+forward-mode derivative: a dual tensor is refused. Pre-activations are kept for the backward pass
 in fp32: a 16-bit copy would round every gradient a second time.
 """
 

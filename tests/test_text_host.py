@@ -137,3 +137,21 @@ def test_pad_rows_arguments():
     refused(pad(ld=-1), b"leading dimension")
     assert pad(rows=0, src=None) == 0
     refused(pad(), b"")                                     # no device here
+
+
+def test_forward_mode_tangents_are_refused():
+    """Before anything else, so that no path drops a tangent."""
+    import torch.autograd.forward_ad as fwd
+    x, w = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.bfloat16)
+    b, ids = torch.zeros(4, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.long)
+    for reverse in (False, True):
+        with fwd.dual_level():
+            def dual(t):
+                return fwd.make_dual(t.clone().requires_grad_(reverse), torch.ones_like(t))
+
+            for call in (lambda: text.linear(dual(x), w), lambda: text.linear(x, dual(w)), lambda: text.linear(x, w, dual(b)),
+                         lambda: text.gated_linear(x, w, dual(w)), lambda: text.layer_norm(dual(x)),
+                         lambda: text.layer_norm(x, dual(x[0])), lambda: text.embedding(ids, dual(w)),
+                         lambda: kernels.linear_dx(dual(x), w), lambda: kernels.linear_dw(x, dual(w))):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
