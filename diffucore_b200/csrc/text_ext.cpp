@@ -8,6 +8,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <initializer_list>
@@ -451,19 +452,21 @@ Tensor embedding_grad_raw(const Tensor& dy_, const Tensor& ids_, int64_t V, doub
 
 // ------------------------------------------------------------------ autograd
 
-// Gradients of a node run under create_graph: usable, but differentiating them again is an error.
-variable_list grads_once(bool create_graph, variable_list grads) {
+// Gradients of a node run under create_graph: usable, but differentiating them again is an error. The
+// node that raises it hangs on the inputs of the differentiated node and on its incoming gradient `dy`,
+// so the engine comes through it wherever a second derivative would go, also for a loss that reaches the
+// same input by another way.
+variable_list grads_once(bool create_graph, const Tensor& dy, variable_list grads) {
   if (!create_graph) return grads;
-  at::AutoGradMode on(true);
-  variable_list present;
-  for (Tensor& g : grads)
-    if (g.defined()) present.push_back(g.detach().requires_grad_());
-  auto node = std::make_shared<torch::autograd::DelayedError>("a diffucore_b200 text operator cannot be differentiated twice",
-                                                              static_cast<int64_t>(present.size()));
-  present = (*node)(std::move(present));
-  size_t i = 0;
-  for (Tensor& g : grads)
-    if (g.defined()) g = present[i++];
+  torch::autograd::edge_list edges = torch::autograd::get_current_node()->next_edges();
+  if (dy.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(dy));
+  const auto node = std::make_shared<torch::autograd::Error>("a diffucore_b200 text operator cannot be differentiated twice",
+                                                             std::move(edges));
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    torch::autograd::set_history(g, node);
+  }
   return grads;
 }
 
@@ -511,7 +514,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         if (want[1]) dw = linear_dw_raw(dz, x, Tensor()).first;
       }
     }
-    return grads_once(create, {dx, dw, db, want[3] ? dy : Tensor(), Tensor()});
+    return grads_once(create, dy, {dx, dw, db, want[3] ? dy : Tensor(), Tensor()});
   }
 };
 
@@ -550,7 +553,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
       else if (want[1]) dwg = linear_dw_raw(g.dz, x, Tensor()).first;
       else if (want[2]) dwu = linear_dw_raw(g.dz1, x, Tensor()).first;
     }
-    return grads_once(create, {dx, dwg, dwu, dbg, dbu, Tensor()});
+    return grads_once(create, dh, {dx, dwg, dwu, dbg, dbu, Tensor()});
   }
 };
 
@@ -584,7 +587,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
       if (want[1]) dw = dw.to(static_cast<at::ScalarType>(wk));
       if (want[2]) db = db.to(static_cast<at::ScalarType>(bk));
     }
-    return grads_once(create, {dx, dw, db, Tensor()});
+    return grads_once(create, dy, {dx, dw, db, Tensor()});
   }
 };
 
@@ -601,7 +604,7 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
     at::AutoGradMode off(false);
     const Tensor d = embedding_grad_raw(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
                                         ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt());
-    return grads_once(create, {Tensor(), d, Tensor(), Tensor()});
+    return grads_once(create, grads[0], {Tensor(), d, Tensor(), Tensor()});
   }
 };
 

@@ -75,3 +75,29 @@ def test_function_transforms_are_refused(transform):
                 transform(lambda t: call(t).sum())(x)
             else:
                 transform(call)(x)
+
+
+def test_second_derivative_is_refused_where_the_loss_reaches_the_input_by_another_way_too():
+    """loss = sum(dx^2) + sum(x^2): without the first term's derivative the gradient would be 2 x."""
+    for name, args, call in calls():
+        for i in range(len(args)):
+            leaves = [a.clone().requires_grad_() for a in args]
+            y = call(*leaves)
+            first = torch.autograd.grad(y.float().square().sum(), leaves, create_graph=True)
+            for g in first:
+                with pytest.raises(RuntimeError, match="differentiated twice"):
+                    torch.autograd.grad(g.float().square().sum() + leaves[i].float().square().sum(), leaves[i],
+                                        retain_graph=True)
+            # what does not pass through a gradient is differentiated as ever
+            plain, = torch.autograd.grad(leaves[i].float().square().sum(), leaves[i])
+            assert torch.equal(plain, (2 * leaves[i].detach().float()).to(plain.dtype))
+
+
+def test_second_derivative_is_refused_through_the_incoming_gradient():
+    for name, args, call in calls():
+        leaves = [a.clone().requires_grad_() for a in args]
+        y = call(*leaves)
+        dy = torch.ones_like(y).requires_grad_()
+        g, *_ = torch.autograd.grad(y, leaves, dy, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated twice"):
+            torch.autograd.grad(g.float().sum() + dy.float().sum(), dy)
