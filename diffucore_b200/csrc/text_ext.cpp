@@ -86,6 +86,15 @@ struct Launch {
   void* stream;
 };
 
+// t with its values as they are in memory: a negated view (the imaginary part of a conjugate) is
+// materialised, a zero tensor without memory too. Everything else is t itself.
+Tensor plain(const Tensor& t) {
+  if (!t.defined()) return t;
+  if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+OptTensor plain(const OptTensor& t) { return has(t) ? OptTensor(plain(*t)) : std::nullopt; }
+
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* ptr(const OptTensor& t) { return has(t) ? t->data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
@@ -161,7 +170,7 @@ OptTensor vector_arg(const char* what, const char* name, const OptTensor& t, int
   if (!has(t)) return std::nullopt;
   if (t->dim() != 1 || t->size(0) != n)
     throw py::value_error(cat(what, ": ", name, " must have shape (", n, ",), got ", shape_of(*t)));
-  return t->contiguous();
+  return plain(*t).contiguous();
 }
 
 int64_t rows_of(const Tensor& t) {
@@ -201,10 +210,10 @@ std::pair<Tensor, Tensor> linear_raw(const Tensor& x_, const Tensor& w_, const O
   if (has(residual_)) {
     if (residual_->dim() != 2 || residual_->size(0) != M || residual_->size(1) != N)
       throw py::value_error(cat("linear: residual must have shape (", M, ", ", N, "), got ", shape_of(*residual_)));
-    residual = unit_rows(*residual_);
+    residual = unit_rows(plain(*residual_));
   }
   Launch at_(x_);
-  Tensor x = x_, w = w_;
+  Tensor x = plain(x_), w = plain(w_);
   projection_operands({&x, &w}, M);
   Tensor y = at::empty({M, N}, x.options()), z;
   if (keep_z) z = at::empty({M, pad(N, kZPad)}, x.options().dtype(at::kFloat));
@@ -223,7 +232,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x_, const Tensor& wg_
   const int64_t M = x_.size(0), K = x_.size(1), N = wg_.size(0);
   const OptTensor bg = vector_arg("gated_linear", "b_gate", bg_, N), bu = vector_arg("gated_linear", "b_up", bu_, N);
   Launch at_(x_);
-  Tensor x = x_, wg = wg_, wu = wu_;
+  Tensor x = plain(x_), wg = plain(wg_), wu = plain(wu_);
   projection_operands({&x, &wg, &wu}, M);
   Tensor h = at::empty({M, N}, x.options()), zg, zu;
   const int64_t ldz = pad(N, kZPad);
@@ -245,7 +254,7 @@ void check_kept(const char* name, const Tensor& z, const Tensor& dy) {
   if (z.scalar_type() != at::kFloat || z.device() != dy.device())
     throw py::type_error(cat("act_grad: ", name, " is ", z.scalar_type(), " on ", z.device(), ", expected fp32 on ", dy.device()));
   const int64_t M = dy.size(0), N = dy.size(1);
-  if (z.dim() != 2 || z.size(0) != M || z.size(1) < N || (z.size(1) > 1 && z.stride(1) != 1))
+  if (z.dim() != 2 || z.size(0) != M || z.size(1) < N || (z.size(1) > 1 && z.stride(1) != 1) || z.is_neg() || z._is_zerotensor())
     throw py::value_error(cat("act_grad: ", name, " ", shape_of(z), " is not the kept pre-activation of dy ", shape_of(dy)));
   const int64_t room = static_cast<int64_t>(z.storage().nbytes() / sizeof(float)) - z.storage_offset();
   if (M > 0 && (M - 1) * z.stride(0) + pad(N, 4) > room)
@@ -269,7 +278,7 @@ ActGrad act_grad_raw(const Tensor& dy_, const Tensor& z, const Tensor& z1, int a
   }
   const int64_t M = dy_.size(0), N = dy_.size(1), lddz = pad(N, kDzPad);
   Launch at_(dy_);
-  Tensor dy = unit_rows(dy_);
+  Tensor dy = unit_rows(plain(dy_));
   if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
   if (z.defined()) g.dz = at::empty({M, lddz}, dy.options()).narrow(1, 0, N);
   if (z1.defined()) g.dz1 = at::empty({M, lddz}, dy.options()).narrow(1, 0, N);
@@ -309,7 +318,7 @@ Tensor linear_dx_raw(const Tensor& dz_, const Tensor& w_, const Tensor& dz1_, co
   }
   if (dz_.size(1) != w_.size(0)) throw py::value_error(cat("linear_dx: dz ", shape_of(dz_), " does not match w ", shape_of(w_)));
   Launch at_(dz_);
-  Tensor dz = dz_, w = w_, dz1 = dz1_, w1 = w1_;
+  Tensor dz = plain(dz_), w = plain(w_), dz1 = plain(dz1_), w1 = plain(w1_);
   matrix_operands({&dz, &w, &dz1, &w1});
   same_rows(dz, dz1);
   const int64_t M = dz.size(0), N = dz.size(1), K = w.size(1);
@@ -323,7 +332,7 @@ std::pair<Tensor, Tensor> linear_dw_raw(const Tensor& dz_, const Tensor& x_, con
   check_product("linear_dw", dz_, "x", x_, dz1_);
   if (dz_.size(0) != x_.size(0)) throw py::value_error(cat("linear_dw: dz ", shape_of(dz_), " does not match x ", shape_of(x_)));
   Launch at_(dz_);
-  Tensor dz = dz_, x = x_, dz1 = dz1_;
+  Tensor dz = plain(dz_), x = plain(x_), dz1 = plain(dz1_);
   matrix_operands({&dz, &x, &dz1});
   same_rows(dz, dz1);
   const int64_t M = dz.size(0), N = dz.size(1), K = x.size(1);
@@ -349,8 +358,8 @@ at::ScalarType norm_affine(const char* what, const Tensor& x, OptTensor& w, OptT
     kind = !kind || *kind == (*t)->scalar_type() ? (*t)->scalar_type() : at::kFloat;
   }
   const at::ScalarType k = kind.value_or(x.scalar_type());
-  if (has(w)) w = w->to(k).contiguous();
-  if (has(b)) b = b->to(k).contiguous();
+  if (has(w)) w = plain(*w).to(k).contiguous();
+  if (has(b)) b = plain(*b).to(k).contiguous();
   return k;
 }
 
@@ -359,7 +368,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x_, OptTensor w,
   if (x_.dim() != 2) throw py::value_error(cat("layer_norm: x must be [M, D], got ", shape_of(x_)));
   Launch at_(x_);
   const at::ScalarType kind = norm_affine("layer_norm", x_, w, b);
-  const Tensor x = unit_rows(x_);
+  const Tensor x = unit_rows(plain(x_));
   const int64_t M = x.size(0), D = x.size(1);
   Tensor y = at::empty({M, D}, x.options()), mean, rstd;
   if (keep_stats) {
@@ -377,7 +386,7 @@ Tensor kept_stat(const char* name, const Tensor& t, const Tensor& x) {
     throw py::type_error(cat("layer_norm_grad: ", name, " is ", t.scalar_type(), " on ", t.device(), ", expected fp32 on ", x.device()));
   if (t.dim() != 1 || t.size(0) != x.size(0))
     throw py::value_error(cat("layer_norm_grad: ", name, " must have shape (", x.size(0), ",), got ", shape_of(t)));
-  return t.contiguous();
+  return plain(t).contiguous();
 }
 
 // dw and db come in `kind` (x's type or fp32), computed in fp32 where w is fp32.
@@ -395,7 +404,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_grad_raw(const Tensor& dy_, const 
   if (kind == at::kFloat) sums = kind;
   if (has(w)) w = w->to(sums);
   const Tensor mean = kept_stat("mean", mean_, x_), rstd = kept_stat("rstd", rstd_, x_);
-  const Tensor dy = unit_rows(dy_), x = unit_rows(x_);
+  const Tensor dy = unit_rows(plain(dy_)), x = unit_rows(plain(x_));
   const int64_t M = x.size(0), D = x.size(1);
   Tensor dx = at::empty({M, D}, x.options()), dw, db, ws;
   size_t bytes = 0;
@@ -416,7 +425,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_grad_raw(const Tensor& dy_, const 
 Tensor check_ids(const char* what, const Tensor& ids, const Tensor& like) {
   if ((ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || ids.device() != like.device())
     throw py::type_error(cat(what, ": ids must be int64 or int32 on ", like.device(), ", got ", ids.scalar_type(), " on ", ids.device()));
-  return (ids.dim() == 1 ? ids : ids.reshape({-1})).contiguous();
+  return plain(ids.dim() == 1 ? ids : ids.reshape({-1})).contiguous();
 }
 
 Tensor embedding_raw(const Tensor& ids_, const Tensor& table_, double scale) {
@@ -425,7 +434,7 @@ Tensor embedding_raw(const Tensor& ids_, const Tensor& table_, double scale) {
   const Tensor ids = check_ids("embedding", ids_, table_);
   Launch at_(table_);
   const int64_t V = table_.size(0), D = table_.size(1), T = ids.size(0);
-  Tensor table = unit_rows(table_);
+  Tensor table = unit_rows(plain(table_));
   if (V > 1 && table.stride(0) < D) table = table.contiguous();
   Tensor out = at::empty({T, D}, table.options());
   check(dc_embedding(ptr(ids), ids.scalar_type() == at::kLong, T, ptr(table), row_stride(table), V, D, static_cast<float>(scale),
@@ -440,7 +449,7 @@ Tensor embedding_grad_raw(const Tensor& dy_, const Tensor& ids_, int64_t V, doub
   const int64_t T = dy_.size(0), D = dy_.size(1);
   if (ids.size(0) != T) throw py::value_error(cat("embedding_grad: ", ids.size(0), " ids for ", T, " rows"));
   Launch at_(dy_);
-  const Tensor dy = unit_rows(dy_);
+  const Tensor dy = unit_rows(plain(dy_));
   size_t bytes = 0;
   check(dc_embedding_grad_workspace(T, V, D, &bytes));
   const Tensor ws = workspace(dy, bytes);
@@ -483,7 +492,7 @@ struct Wants {
 struct LinearNode : torch::autograd::Function<LinearNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const OptTensor& bias, const OptTensor& residual,
                         int64_t act) {
-    Tensor x = x_, w = w_;
+    Tensor x = plain(x_), w = plain(w_);
     matrix_operands({&x, &w});                                       // padded once for both passes
     const bool keep = act != DC_ACT_NONE && (x_.requires_grad() || w_.requires_grad() || (has(bias) && bias->requires_grad()));
     auto [y, z] = linear_raw(x, w, bias, static_cast<int>(act), residual, keep);
@@ -508,20 +517,20 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       const ActGrad g = act_grad_raw(dy, z, Tensor(), static_cast<int>(ctx->saved_data["act"].toInt()), want[2], false);
       db = g.db;
       if (want[0] || want[1]) {
-        Tensor dz = g.dz;
+        Tensor dz = plain(g.dz);
         matrix_operands({&dz});
         if (want[0]) dx = linear_dx_raw(dz, w, Tensor(), Tensor());
         if (want[1]) dw = linear_dw_raw(dz, x, Tensor()).first;
       }
     }
-    return grads_once(create, dy, {dx, dw, db, want[3] ? dy : Tensor(), Tensor()});
+    return grads_once(create, dy, {dx, dw, db, want[3] ? plain(dy) : Tensor(), Tensor()});
   }
 };
 
 struct GatedNode : torch::autograd::Function<GatedNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const OptTensor& bg,
                         const OptTensor& bu, int64_t act) {
-    Tensor x = x_, wg = wg_, wu = wu_;
+    Tensor x = plain(x_), wg = plain(wg_), wu = plain(wu_);
     matrix_operands({&x, &wg, &wu});
     auto [h, zg, zu] = gated_raw(x, wg, wu, bg, bu, static_cast<int>(act), true);
     ctx->save_for_backward({x, wg, wu, zg, zu});
@@ -684,6 +693,7 @@ PYBIND11_MODULE(_text_ext, m) {
   m.def("embedding", &embedding, Free());
   m.def("matrix_operand", [](Tensor t) {
     if (t.dim() != 2) throw py::value_error(cat("matrix_operand: expected a matrix, got ", shape_of(t)));
+    t = plain(t);
     matrix_operands({&t});
     return t;
   });

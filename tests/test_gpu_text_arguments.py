@@ -1,12 +1,13 @@
 """GPU: the single steps of the text operators (diffucore_b200.kernels) refuse tensors that do not
-belong together before anything is launched, and take any layout of those that do."""
+belong together before anything is launched, and take any layout of those that do; tensors whose
+memory does not hold their values as they are (negated views, zero tensors without memory)."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from diffucore_b200 import kernels
+from diffucore_b200 import kernels, text
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -144,3 +145,40 @@ def test_norm_gradient_keeps_an_fp32_weight():
     got = kernels.layer_norm_grad(dy, x, w, mean, rstd, dtype=torch.bfloat16)
     assert torch.equal(got[0], want[0])
     assert all(g.dtype == torch.bfloat16 and torch.equal(g, e.to(torch.bfloat16)) for g, e in zip(got[1:], want[1:]))
+
+
+def test_negated_views():
+    """torch._neg_view(t) has t's memory and -t's values, as the imaginary part of a conjugate has."""
+    x, w, b, r = rand(40, 48), rand(56, 48), rand(56), rand(40, 56)
+    neg = torch._neg_view
+
+    def same(call, *args):
+        def step(leaves, dy):
+            y = call(*leaves)
+            return (call(*[a.detach() for a in leaves]), y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+        ones = torch.ones_like(call(*args))
+        want = step([a.neg().requires_grad_() for a in args], -ones)
+        got = step([neg(a).requires_grad_() for a in args], neg(ones))
+        for p, q in zip(want, got):
+            assert torch.equal(p, q) and not q.is_neg()
+
+    same(lambda x, w, b, r: text.linear(x, w, b, activation="silu", residual=r), x, w, b, r)
+    same(lambda x, w, b, r: text.linear(x[:4, 1:], w[:, 1:], b, residual=r[:4]), x, w, b, r)
+    same(text.gated_linear, x, w, rand(56, 48), b, rand(56))
+    same(text.layer_norm, x, rand(48), rand(48))
+    ids = torch.randint(0, 40, (300,), device=DEV)
+    same(lambda t: text.embedding(ids, t), x)
+    z = torch.randn(7, 32, device=DEV, dtype=torch.complex64)
+    assert z.conj().imag.is_neg()
+    assert torch.equal(text.layer_norm(z.conj().imag), text.layer_norm(-z.imag))
+
+
+def test_zero_tensors_without_memory():
+    zero = torch._efficientzerotensor((40, 48), device=DEV, dtype=torch.bfloat16)
+    w = rand(56, 48)
+    assert not text.linear(zero, w).any() and not text.gated_linear(zero, w, w).any()
+    assert not text.layer_norm(zero).any()
+    x = rand(40, 48).requires_grad_()
+    dx, = torch.autograd.grad(text.layer_norm(x), x, zero)
+    assert not dx.any()
