@@ -167,7 +167,8 @@ def i64_array(values) -> ctypes.Array:
 
 def device_error(clear: bool = True) -> int:
     """The device-global error word (0 = none): 1 and 2 from bounded in-kernel waits, 3 from an
-    embedding lookup that met a token id outside its table."""
+    embedding lookup that met a token id outside its table. Of two errors one is returned (and
+    cleared) per call. Waits for the device."""
     code = ctypes.c_uint(0)
     check(load().dc_device_error(ctypes.byref(code), 1 if clear else 0))
     return int(code.value)

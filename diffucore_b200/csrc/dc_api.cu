@@ -799,16 +799,18 @@ int dc_quant_division(void) { return g_quant_div.load(std::memory_order_relaxed)
 const char* dc_last_error(void) { return dc::err_text; }
 
 int dc_device_error(unsigned int* code, int clear) {
-  unsigned int v = 0, text = 0;
+  unsigned int v = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, dc::g_device_error, sizeof(v));
   if (e != cudaSuccess) return cuda_fail(e, "reading the device error word");
-  if (clear) {
-    const unsigned int zero = 0;
+  if (clear && v != 0) {
+    unsigned int zero = 0;
     e = cudaMemcpyToSymbol(dc::g_device_error, &zero, sizeof(zero));
     if (e != cudaSuccess) return cuda_fail(e, "clearing the device error word");
   }
-  if (int r = dc::text_device_error(&text, clear)) return r;
-  if (v == 0) v = text;
+  // The text operators' word: read, and cleared, when this one does not take its place in `code`.
+  if (v == 0 || code == nullptr) {
+    if (int r = dc::text_device_error(&v, clear)) return r;
+  }
   if (code) *code = v;
   return DC_OK;
 }

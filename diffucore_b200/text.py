@@ -54,7 +54,8 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0,
               padding_idx: int | None = None) -> torch.Tensor:
     """``scale * table[ids]`` for int64 or int32 ``ids`` of any shape and ``table`` [V, D]; the row of
     ``padding_idx`` gets no gradient. An id outside the table gives a zero row and sets the device
-    error word (``_lib.device_error()`` returns 3); it never reads outside the table."""
+    error word, which ``diffucore_b200.device_error()`` returns as 3 (it waits for the device; call it
+    where a step's results are read); it never reads outside the table."""
     return _lib.text_ext().embedding(ids, table, scale, padding_idx)
 
 

@@ -60,9 +60,10 @@ const char* dc_last_error(void);
 int dc_set_quant_division(int mode);
 int dc_quant_division(void);
 
-/* Read (and optionally clear) the device-global error word that bounded in-kernel waits set
- * when they give up (1 = a wait timed out, 2 = the timeout self-test fired), and the word an embedding lookup sets for
- * a token id outside its table (3). Synchronous. */
+/* Read (and optionally clear) the device-global error words. Two exist: the text operators' (3 = an
+ * embedding lookup met a token id outside its table, 1 = a wait timed out) and the other kernels' (1 = a
+ * wait timed out, 2 = the timeout self-test fired). One is returned per call, the latter first, and
+ * only the one returned is cleared: read until 0. With code null both are cleared. Synchronous. */
 int dc_device_error(unsigned int* code, int clear);
 
 /* Per-row symmetric int8 quantization of x [M, K] (row stride ldx elements):

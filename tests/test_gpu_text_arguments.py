@@ -7,7 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from diffucore_b200 import kernels, text
+from diffucore_b200 import _lib, device_error, kernels, text
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -182,3 +182,22 @@ def test_zero_tensors_without_memory():
     x = rand(40, 48).requires_grad_()
     dx, = torch.autograd.grad(text.layer_norm(x), x, zero)
     assert not dx.any()
+
+
+def test_both_error_words_are_reported():
+    """A wait that timed out and a token id outside its table, both before the words are read: each is
+    returned once."""
+    while device_error():
+        pass
+    text.embedding(torch.tensor([10], device=DEV), rand(10, 32))
+    status = torch.zeros(1, device=DEV, dtype=torch.int32)
+    lib = _lib.load()
+    _lib.check(lib.dc_selftest_wait_timeout(2_000_000, status.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert device_error(clear=False) == 2
+    assert device_error() == 2
+    assert device_error() == 3
+    assert device_error() == 0
+    text.embedding(torch.tensor([10], device=DEV), rand(10, 32))
+    lib.dc_device_error(None, 1)                             # clears both
+    assert device_error() == 0
