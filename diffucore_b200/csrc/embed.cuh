@@ -8,7 +8,7 @@
 // sums are the same on every call, without float atomics):
 //   sort    up to 8192 tokens: each token's place is the number of smaller (id, t) keys, counted
 //           against all keys in shared memory, one launch; more: least-significant-digit radix
-//           passes of up to 9 bits (histogram per tile, stable scatter)
+//           passes of up to 9 bits (histogram per tile, for many tiles their prefix sums, stable scatter)
 //   sum     a CTA per chunk of sorted places and slab of columns adds up the runs of equal ids that
 //           start in its chunk; a run that covers a whole chunk leaves fp32 partials per chunk
 //   join    adds the partials of those runs in order
@@ -168,10 +168,48 @@ radix_hist_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, uint32_
   for (int d = threadIdx.x; d < digits; d += blockDim.x) hist[static_cast<int64_t>(blockIdx.x) * digits + d] = h[d];
 }
 
+// In place, the counts of the tiles before each tile, and the digits' totals behind the last tile's
+// counts: for many tiles, where adding up every tile's counts in every CTA of the scatter would grow
+// with their square. A CTA takes 32 digits, its warps equal ranges of tiles, each read twice.
+constexpr int kScanWarps = 32;
+
+__global__ void __launch_bounds__(32 * kScanWarps)
+radix_scan_kernel(uint32_t* __restrict__ hist, int digits, int tiles) {
+  pdl_enter();
+  __shared__ uint32_t sums[kScanWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int d = blockIdx.x * 32 + lane;
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * warp / kScanWarps);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (warp + 1) / kScanWarps);
+  uint32_t s = 0;
+  if (d < digits) {
+#pragma unroll 16
+    for (int i = t0; i < t1; ++i) s += hist[static_cast<int64_t>(i) * digits + d];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  s = 0;
+  for (int w = 0; w < warp; ++w) s += sums[w][lane];
+  if (d >= digits) return;
+  constexpr int kAhead = 16;                    // loads in flight before their stores
+  for (int i0 = t0; i0 < t1; i0 += kAhead) {
+    uint32_t c[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) c[j] = i0 + j < t1 ? hist[static_cast<int64_t>(i0 + j) * digits + d] : 0u;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 + j < t1) hist[static_cast<int64_t>(i0 + j) * digits + d] = s;
+      s += c[j];
+    }
+  }
+  if (warp == kScanWarps - 1) hist[static_cast<int64_t>(tiles) * digits + d] = s;
+}
+
 // Stable scatter of a tile. Warp w owns keys [32 kRounds w, 32 kRounds (w + 1)) of the tile, 32 at a
 // time; a key's place is the number of smaller digits + equal digits in earlier tiles (both summed
-// here from the tiles' counts) + in earlier warps + in earlier rounds of its warp + in lower lanes.
-template <bool FIRST>
+// here from the tiles' counts, or taken from their prefix sums: SCANNED) + in earlier warps + in earlier
+// rounds of its warp + in lower lanes.
+template <bool FIRST, bool SCANNED>
 __global__ void __launch_bounds__(32 * kRadixWarps)
 radix_scatter_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ idx,
                      const uint32_t* __restrict__ hist, uint32_t* __restrict__ keys_out,
@@ -202,7 +240,10 @@ radix_scatter_kernel(const EmbedIds ids, const uint32_t* __restrict__ keys, cons
   for (int j = 0; j < kPerThread; ++j) {
     const int d = threadIdx.x * kPerThread + j;
     total[j] = 0; before_tile[j] = 0;
-    if (d < digits) {
+    if (SCANNED && d < digits) {
+      total[j] = hist[static_cast<int64_t>(tiles) * digits + d];
+      before_tile[j] = hist[static_cast<int64_t>(blockIdx.x) * digits + d];
+    } else if (d < digits) {
 #pragma unroll 16
       for (int i = 0; i < tiles; ++i) {
         const uint32_t c = hist[static_cast<int64_t>(i) * digits + d];
