@@ -118,11 +118,19 @@ def ext_missing() -> str | None:
     return None
 
 
+def _ext_stamp() -> str:
+    """What a built binding is bound to besides its source: the torch and the Python it was compiled for."""
+    import torch
+    return f"torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} python {sys.version}\n"
+
+
 def build_ext(force: bool = False, verbose: bool = False) -> Path:
     """Compile ``csrc/text_ext.cpp`` against the installed torch into ``_text_ext.so``, linked to the
     library beside it, unless it is up to date."""
     src = CSRC / "text_ext.cpp"
-    if not force and EXT.exists():
+    OBJECTS.mkdir(exist_ok=True)
+    stamp = OBJECTS / "text_ext.stamp"
+    if not force and EXT.exists() and stamp.exists() and stamp.read_text() == _ext_stamp():
         built = EXT.stat().st_mtime
         if all(p.stat().st_mtime <= built for p in _includes(src.resolve(), set())):
             return EXT
@@ -135,6 +143,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
           f"-L{PKG}", "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN", f"-L{lib_dir}", f"-Wl,-rpath,{lib_dir}",
           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"], verbose)
     os.replace(tmp, EXT)
+    stamp.write_text(_ext_stamp())
     return EXT
 
 

@@ -44,3 +44,14 @@ def test_library_alone_without_what_the_binding_needs(compilers, monkeypatch, ca
     assert build.build() == build.LIB and build.LIB.exists() and not build.EXT.exists()
     assert compilers == ["nvcc"] * 3
     assert f"{lacks} not found" in capsys.readouterr().err
+
+
+def test_binding_is_rebuilt_for_another_torch(compilers, monkeypatch):
+    monkeypatch.setattr(build, "ext_missing", lambda: None)
+    build.build()
+    stamp = build._ext_stamp()
+    monkeypatch.setattr(build, "_ext_stamp", lambda: stamp.replace("torch ", "torch 0."))
+    build.build()
+    assert compilers[4:] == ["g++"]
+    build.build()
+    assert len(compilers) == 5
