@@ -155,3 +155,24 @@ def test_forward_mode_tangents_are_refused():
                          lambda: kernels.linear_dx(dual(x), w), lambda: kernels.linear_dw(x, dual(w))):
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     call()
+
+
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (300, 9, 5000), (8192, (1 << 19) - 1, 8), (8193, 1000, 8), (8192, 1 << 19, 8),
+                                   (98304, 1000, 8), (98305, 600000, 2048), (1 << 20, 262143, 64), (1 << 22, 262144, 1)])
+def test_embedding_workspace_is_what_the_launches_write(T, V, D):
+    """The sum's partials have chunks of 8 sorted places, doubled up to 64 while there are 16 CTAs for each
+    of 148 SMs; the radix passes' counts have a row per 1024 tokens, one more where they are scanned."""
+    n = ctypes.c_size_t(0)
+    assert _lib.load().dc_embedding_grad_workspace(T, V, D, ctypes.byref(n)) == 0
+    slabs, chunk = -(-D // 1024), 8
+    while chunk < 64 and -(-T // (2 * chunk)) * slabs >= 16 * 148:
+        chunk *= 2
+    partials = -(-T // chunk) * 2 * D * 4
+    if T <= 8192 and V < 1 << 19:
+        need = [T * 4, T * 4, partials]
+    else:
+        bits = V.bit_length()                               # keys 0 .. V
+        passes = -(-bits // 9)
+        tiles = -(-T // 1024)
+        need = [T * 4] * 4 + [(tiles + (tiles >= 96)) * 4 << -(-bits // passes), partials]
+    assert sum(need) <= n.value <= sum(need) + 256 * len(need)
