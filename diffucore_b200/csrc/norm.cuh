@@ -5,7 +5,7 @@
 // Bound by HBM: forward one read and one write of x, backward two reads and one write. Every value is
 // read once and held in registers while its row's sums are formed; the variance is the mean of
 // squared deviations from the mean (no cancellation). Only rows beyond the widest register layout
-// are read again from cache.
+// are read again from cache. rstd is rsqrtf's, good to 2 units in the last place of fp32.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -144,9 +144,9 @@ struct NormParams {
 
 template <int TPR> struct NormCta { static constexpr int kThreads = TPR == 32 ? 256 : TPR; };
 
-// Forward, rows in registers: TPR threads per row, NU units each. A unit is 16 bytes (VEC) or one
-// value, kept packed until it is used, so a warp holds a row of 4096 16-bit values in 64 registers
-// per lane: 16 loads in flight per lane and no barrier at all.
+// Forward of few rows, in registers: TPR threads per row, NU units each, all loaded at once. A unit is
+// 16 bytes (VEC) or one value, kept packed until it is used. Rows of 32 threads need no barrier, wider
+// ones two; bound by latency (one row of 4096 6 us a call, most of it the host's).
 template <typename T, bool VEC, int NU, int TPR>
 __global__ void __launch_bounds__(NormCta<TPR>::kThreads)
 norm_fwd_kernel(const NormParams p) {

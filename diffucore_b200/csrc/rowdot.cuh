@@ -1,5 +1,5 @@
 // The projections of a few rows (decoded tokens, conditioning vectors): y = act(x . w^T + b) + r and
-// the gated form for up to 32 rows. The weights, read once, are all the traffic that counts, so this
+// the gated form for up to 16 rows. The weights, read once, are all the traffic that counts, so this
 // kernel is built around that stream instead of shared-memory tiles.
 //
 // A warp owns 16 weight rows (16 output columns; gated: 8 columns, their gate rows and their up
@@ -11,7 +11,8 @@
 // HBM, and for narrow layers by latency, which is why `ks` warps divide the k of one group of rows.
 // Their partial sums are added in a fixed order.
 //
-// Weights whose rows a 16-byte load cannot take are read by single values instead of being copied.
+// Weights whose rows a 16-byte load cannot take are read by single values instead of being copied; so
+// are aligned weights beside an x (of up to 8 rows) whose own rows are not aligned.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

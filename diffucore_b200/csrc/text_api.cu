@@ -106,10 +106,12 @@ int pair_override() {
 //   cluster   5200 + (S > 1: 900 + 200 S rows / 128) + load * k-blocks / S * 1.29 (rows + 128)
 // with bn the pair's tile width, S the CTAs that divide a cluster tile's k-blocks, rows the tile's
 // rows of A (at most 128), and load the CTAs per SM (at least one; two are resident, so a second
-// wave counts as two more). Measured against the estimate, us: 300 x 4096 x 4096, pair 128 wide 22.1
-// (20.9), cluster S = 2 22.3 (20.2); 1024^3, pair 128 wide 9.5 (9.6), 256 wide 11.3 (11.4); 700 x 1280
-// x 5120, cluster S = 4 17.2 (17.6), pair 24.8 (24.6); 512 x 512 x 8192, cluster S = 8 14.4 (13.0), S = 4
-// 17.9 (17.5); 64 x 1024 x 1024, cluster S = 4 6.4 (7.5).
+// wave counts as two more). Measured (M x N x K, one captured graph of calls, operands in L2 / from HBM)
+// against the estimate, us; the choice first: 300 x 4096 x 4096 cluster S = 2 20.2 / 21.4 (20.2), pair 128
+// wide 20.5 / 21.0 (20.9); 700 x 5120 x 1280 pair 12.2 / 12.8, cluster 14.5 / 15.3; 256 x 1024 x 4096 cluster
+// 10.5 / 11.4, pair 19.4 / 20.4; 512 x 512 x 8192 cluster S = 8 13.2 / 14.5 (13.0), pair 34 / 36; 64 x 1024 x 1024
+// cluster S = 8 5.1 / 5.6 (7.4), pair 7.8 / 8.3. Near its crossings the choice can be the slower one by a tenth:
+// 1024^3 cluster S = 2 8.7 / 9.6 (9.1), pair 128 wide 8.4 / 8.8 (9.6).
 struct HChoice { bool pair; int bn, splits; };
 
 HChoice choose_hgemm(int64_t M, int stack, int64_t cols, int64_t k, int sms) {

@@ -87,6 +87,9 @@ __device__ __forceinline__ void pairs_of(const Float8& v, Pair (&f)[4]) {
 // Bound by HBM: 2 B (dy) + 4 or 8 B (z) read and 2 or 4 B written per element. kAhead rows per thread
 // are loaded, as they are in memory, ahead of their arithmetic: made into pairs where they are
 // loaded they wait for each row in turn (57.3 us against 41.8 for 8192 x 4096 without an activation).
+// dz is rounded to the 16 bits that the tensor core's operands have; the column sums are of dz before
+// that. Against 64 bits it takes the relative error of dx and dw from 0.0017 (their own rounding to bf16) to
+// 0.0023, from 0.00021 to 0.00029 in fp16; dz in two 16-bit halves would cost a second product each.
 // Three CTAs per SM where registers allow it (gelu_tanh 45.7 us, 49.3 with two); at 8192 x 4096
 // 41.8 us without an activation (6430 GB/s), 45.9 with GELU, 4.9 more with the bias's gradient;
 // gated 4173 x 5464 with SiLU 51.6 us (6190 GB/s). Rows of dy that 16-byte accesses do not fit are read

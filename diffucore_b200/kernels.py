@@ -471,7 +471,8 @@ def matrix_operand(t: torch.Tensor) -> torch.Tensor:
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None,
            residual: torch.Tensor | None = None, keep_z: bool = False):
     """``(y, z)``: ``y = act(z) + residual``, ``z = x @ w.T + bias`` for 16-bit ``x`` [M, K] and ``w``
-    [N, K] (``dc_linear``). ``z`` is the fp32 pre-activation (rows padded to 4) when ``keep_z``."""
+    [N, K] (``dc_linear``). ``z`` is the fp32 pre-activation when ``keep_z``: ``[M, N rounded up to 16]``,
+    of which the first N columns are written."""
     return _lib.text_ext().linear_raw(x, w, bias, act_code(act), residual, keep_z)
 
 

@@ -12,8 +12,10 @@ device. The projections take bf16 and fp16, the norm and the embedding fp32 as w
 (products, norm statistics, weight gradients) in a fixed order, so results repeat bit for bit;
 outputs and gradients are rounded once to their type. Argument checks, allocation and the autograd
 nodes are native (``_text_ext.so``). The gradients cannot be differentiated again, and there is no
-forward-mode derivative: a dual tensor is refused. Pre-activations are kept for the backward pass
-in fp32: a 16-bit copy would round every gradient a second time.
+forward-mode derivative: a dual tensor is refused. They are not traceable: ``torch.compile`` breaks the
+graph at them, and function transforms (vmap, jvp) refuse them. Pre-activations are kept for the
+backward pass in fp32: a 16-bit copy would round every gradient a second time. dz, the gradient before
+the activation, is rounded to 16 bits for the two products that read it.
 """
 
 from __future__ import annotations
