@@ -68,8 +68,20 @@ inline int make_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const vo
                                                 (unsigned long long)strides_bytes[i]);
     s[i] = strides_bytes[i];
   }
-  CUresult r = fn(map, dt, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, dt, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread whose first use of the driver this is (the autograd engine's, say): setting its current
+    // device binds the device's context to it.
+    int dev = 0;
+    cudaError_t ce = cudaGetDevice(&dev);
+    if (ce == cudaSuccess) ce = cudaSetDevice(dev);
+    if (ce != cudaSuccess) return cuda_fail(ce, "binding a context to the calling thread");
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
   return DC_OK;
 }
